@@ -253,6 +253,22 @@ ZYNFER_CU_API int zynfer_cu_set_sampling(ZynferCuCtx *ctx, float temperature, ui
 ZYNFER_CU_API int zynfer_cu_sample(ZynferCuCtx *ctx, const float *logits, uint32_t rows, uint32_t vocab,
                                    const uint32_t *slots, const uint32_t *positions, float temperature,
                                    uint32_t top_k, float top_p, uint64_t seed, uint32_t *out_ids);
+struct ZynferCuDrawRule;
+/* Append the next n tokens (n <= max_prefill) of a prompt to `seq` from
+ * position = its length, every layer's attention with the window and sinks of
+ * zynfer_cu_attn_window (ZYNFER_CU_WINDOW_ALL: causal). K and V are read back
+ * from the bf16 cache. last_logits [vocab] and argmax of the last row may be
+ * NULL; the argmax is the largest logit whatever zynfer_cu_set_sampling says. */
+ZYNFER_CU_API int zynfer_cu_prefill_chunk(ZynferCuCtx *ctx, uint32_t seq, const uint32_t *tokens, uint32_t n,
+                                          uint32_t window, uint32_t sinks, float *last_logits, uint32_t *argmax);
+/* One decode step for `batch` sequences as zynfer_cu_decode_step, with the
+ * attention of zynfer_cu_attn_shared (window ZYNFER_CU_WINDOW_ALL) or
+ * zynfer_cu_attn_window, and the tokens drawn by zynfer_cu_sample_rows's rule
+ * from uniforms[batch]. All arrays, the rule's included, are host arrays; rule
+ * and logprobs may be NULL. */
+ZYNFER_CU_API int zynfer_cu_decode_drawn(ZynferCuCtx *ctx, const uint32_t *seqs, const uint32_t *tokens,
+                                         uint32_t batch, uint32_t window, uint32_t sinks, const float *uniforms,
+                                         const struct ZynferCuDrawRule *rule, uint32_t *ids, float *logprobs);
 /* One transformer block (qwen_block.forward, qwen_block.zig:161-235) of layer
  * `layer` on host hidden states x [t][hidden] at pos0 = the sequence's length;
  * out [t][hidden]. Appends to the sequence's cache for that layer. */
@@ -338,6 +354,80 @@ ZYNFER_CU_API int zynfer_cu_attn_decode(ZynferCuCtx *ctx, uint32_t layer, const 
  * pos0 + rows <= max_seq_len. Synchronises. */
 ZYNFER_CU_API int zynfer_cu_rmsnorm_qk_rope(ZynferCuCtx *ctx, const float *qkv, uint32_t rows, const float *q_norm,
                                             const float *k_norm, uint32_t pos0, float *q_out, float *k_out);
+/* ---- serving attention and draws (device pointers) ----
+ * These calls read the cache that prefill, decode and zynfer_cu_kv_write
+ * fill. They return once their kernels are enqueued on the context stream
+ * (zynfer_cu_sync waits, and reports a failed device check); the batch's
+ * lengths and slots are taken at the call. dtype is ZYNFER_CU_DT_F32 or
+ * ZYNFER_CU_DT_BF16, for q and out alike; row i of q starts i * q_stride
+ * elements in and holds [n_q][head_dim]; out is laid out the same with
+ * out_stride and does not overlap q. Strides are at least n_q * head_dim and
+ * multiples of 8, pointers 16-byte aligned. q is rotated and normalised
+ * already (zynfer_cu_rmsnorm_qk_rope); scores are q . k / sqrt(head_dim).
+ * Softmax statistics and sums are f32 (attentionInto, ops.zig:285-354). The
+ * first calls, and calls larger than any before, allocate workspace. */
+
+/* Every position is visible: the window argument for full causal attention. */
+#define ZYNFER_CU_WINDOW_ALL 0xFFFFFFFFu
+
+/* K and V rows [n_kv][n][head_dim] (f32, rounded to nearest even, or bf16; K
+ * normalised and rotated) into positions pos .. pos + n - 1 of `seq`'s cache
+ * of one layer, blocks added as needed: a cache that was computed elsewhere, or
+ * the rows of new tokens. The sequence's length becomes max(length, pos + n);
+ * pos <= length, and no written position lies in a block that another
+ * sequence holds (INVALID). The counterpart of zynfer_cu_kv_read (KvCache,
+ * kv_cache.zig:14-33). Asynchronous as above. */
+ZYNFER_CU_API int zynfer_cu_kv_write(ZynferCuCtx *ctx, uint32_t seq, uint32_t layer, uint32_t pos, uint32_t n,
+                                     const void *k, const void *v, int dtype);
+/* Decode attention of one query per sequence (row i: seqs[i], distinct, each
+ * at least one position long) over all its cached positions, its own token's
+ * K/V already appended. Rows whose sequences hold the same leading blocks
+ * (zynfer_cu_seq_fork) read those once for all of them. No counterpart in the
+ * reference, which runs one sequence (attentionInto, ops.zig:285-354). */
+ZYNFER_CU_API int zynfer_cu_attn_shared(ZynferCuCtx *ctx, uint32_t layer, const uint32_t *seqs, uint32_t batch,
+                                        const void *q, uint64_t q_stride, void *out, uint64_t out_stride, int dtype);
+/* Attention with a sliding window and sinks. The last `tokens` cached
+ * positions of each sequence are queries (row i * tokens + t: seqs[i] at
+ * position length - tokens + t; every sequence at least `tokens` long), and
+ * the query at position p sees positions j <= p with j < sinks or
+ * j > p - window. window ZYNFER_CU_WINDOW_ALL: causal attention. A query that
+ * sees nothing (window 0, no sink at or before it) gives zeros. tokens = 1 is
+ * a decode step, more a chunk of a prompt. */
+ZYNFER_CU_API int zynfer_cu_attn_window(ZynferCuCtx *ctx, uint32_t layer, const uint32_t *seqs, uint32_t batch,
+                                        uint32_t tokens, uint32_t window, uint32_t sinks, const void *q,
+                                        uint64_t q_stride, void *out, uint64_t out_stride, int dtype);
+/* A rule per row for zynfer_cu_sample_rows (device arrays [rows]) and
+ * zynfer_cu_decode_drawn (host arrays [batch]); a null array is its neutral
+ * value in every row. */
+typedef struct ZynferCuDrawRule {
+    const float *temperature;  /* 1; <= 0 or NaN takes the largest logit */
+    const int32_t *top_k;      /* 0 (or less): every token */
+    const float *top_p;        /* 1 (or more, or NaN): every token; <= 0: the first */
+    const float *min_p;        /* 0 (or less, or NaN): every token; at most 1 */
+} ZynferCuDrawRule;
+/* The next token of each of `rows` rows of logits (f32 or bf16, `stride`
+ * elements apart, vocab <= 262144 of them) from the random number
+ * uniforms[row] in [0, 1). Token i weighs
+ * w_i = rint(exp((l_i - max l) / temperature) 2^33), 0 where the exponential
+ * is below min_p and for logits that are NaN or -inf. In descending order of
+ * the logits (the lower index first among equals, topK's order,
+ * qwen_forward.zig:177-193), of the first top_k tokens with weight the
+ * shortest run is kept whose sum reaches top_p of theirs, and the first token
+ * is drawn whose running sum exceeds floor(u S), S the kept run's sum. The
+ * weights are whole numbers: the same inputs give the same tokens. A row
+ * without any weight gives id 0. logprobs (nullable) receives the drawn
+ * token's (l - max l) / temperature - ln(S / 2^33) (-inf without weight).
+ * Needs no model. Asynchronous, on the context stream; arrays 4-byte
+ * aligned, logits aligned to their type. */
+ZYNFER_CU_API int zynfer_cu_sample_rows(ZynferCuCtx *ctx, const void *logits, int dtype, uint64_t stride,
+                                        uint32_t rows, uint32_t vocab, const float *uniforms,
+                                        const ZynferCuDrawRule *rule, uint32_t *ids, float *logprobs);
+/* Order between the context stream and a caller's cudaStream_t (NULL = the
+ * default stream): wait_stream makes the context's later work wait for what
+ * `stream` holds now, stream_wait the other way round. */
+ZYNFER_CU_API int zynfer_cu_wait_stream(ZynferCuCtx *ctx, void *stream);
+ZYNFER_CU_API int zynfer_cu_stream_wait(ZynferCuCtx *ctx, void *stream);
+
 /* siluMul (ops.zig:36-42): out[i] = silu(gate[i]) * up[i], device pointers,
  * the arithmetic of every SwiGLU epilogue. */
 ZYNFER_CU_API int zynfer_cu_swiglu(ZynferCuCtx *ctx, const float *gate, const float *up, uint64_t n, float *out);

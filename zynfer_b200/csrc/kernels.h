@@ -136,6 +136,58 @@ struct SampleArgs {
 void prepare_sample_kernels();
 void launch_sample(const SampleArgs& a, cudaStream_t st);
 
+// draw.cu: the next tokens of `rows` rows from given random numbers, a rule
+// per row (device arrays, nullable: the rule's neutral value)
+struct DrawArgs {
+    const void* logits;        // [rows] rows of `vocab` f32 or bf16 values, `stride` elements apart
+    int bf16;
+    unsigned long long stride;
+    int rows, vocab;           // vocab <= kDrawMaxVocab
+    const float* uniforms;     // [rows]
+    const float* temperature;  // 1
+    const int* top_k;          // 0 = all
+    const float* top_p;        // 1
+    const float* min_p;        // 0
+    uint32_t* ids;             // [rows]
+    float* logprobs;           // nullable [rows]
+};
+constexpr int kDrawMaxVocab = 1 << 18;
+void prepare_draw_kernels();
+void launch_draw(const DrawArgs& a, cudaStream_t st);
+
+// serve_attn.cu: attention of the serving paths over the paged cache. The
+// batch's sequences travel as a kernel parameter: a call copies nothing.
+constexpr int kServeMaxBatch = 1024;
+struct ServeRows {
+    int slot[kServeMaxBatch];  // sequence slot (block-table row)
+    int len[kServeMaxBatch];   // cached positions, the queries' own among them
+};
+struct ServeAttnArgs {
+    const uint16_t* kv_layer;  // [n_kv][blocks][K, V][16][d], rows chunk-swizzled (kv_swizzle)
+    const int* block_table;    // [seqs][max_blocks]
+    int max_blocks, n_pool_blocks, n_kv;
+    const void* q;             // row (b, t) at (b tokens + t) q_stride: [n_q][d] f32 or bf16
+    void* out;                 // the same with out_stride
+    unsigned long long q_stride, out_stride;  // elements
+    int bf16;
+    int batch, tokens;         // query (b, t) sits at position len[b] - tokens + t
+    uint32_t window;           // it sees the last `window` positions up to its own ..
+    int sinks;                 // .. and the first `sinks` of the sequence
+    uint32_t* err;
+};
+struct KvWriteArgs {
+    uint16_t* kv_layer;
+    const int* table_row;      // the sequence's device block-table row
+    int n_pool_blocks, n_kv;
+    int pos, n;
+    const void *k, *v;         // [n_kv][n][d] f32 or bf16
+    int bf16;
+    uint32_t* err;
+};
+void prepare_serve_attn_kernels();
+void launch_serve_attn(const ServeRows& rows, const ServeAttnArgs& a, cudaStream_t st);
+void launch_kv_write(const KvWriteArgs& a, cudaStream_t st);
+
 // gemv.cu (N <= 8)
 void launch_gemv(const LinearArgs& a, cudaStream_t st);
 // The GEMV stages its N activation rows of K values in shared memory: true

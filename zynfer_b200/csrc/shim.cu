@@ -179,6 +179,9 @@ struct ZynferCuCtx {
     int step_launches = 0;  // kernels enqueued by the last decode step
     uint64_t h2d_bytes = 0, d2h_bytes = 0;  // host<->device bytes of decode/generate calls
     cudaEvent_t ev0 = nullptr, ev1 = nullptr;
+    cudaEvent_t ev_order = nullptr;  // order between the context stream and a caller's
+    float* ddraw = nullptr;          // zynfer_cu_decode_drawn: [uniforms, T, top_k, top_p, min_p][max_batch], logprobs
+    float* hdraw = nullptr;          // the same, pinned
     uint64_t last_step_ns = 0;
 
     // per-kernel timing
@@ -746,6 +749,60 @@ void enqueue_prefill_layers(ZynferCuCtx* c, uint32_t seq, int T, uint32_t l0, ui
     }
 }
 
+// ---- serving attention (serve_attn.cu)
+
+// The checks of a serving-attention call's batch; rows receives its slots and
+// lengths, `extra` positions past the cached ones included.
+int serve_rows(ZynferCuCtx* c, const uint32_t* seqs, uint32_t batch, uint32_t tokens, uint32_t extra, ServeRows* rows) {
+    if (batch == 0 || batch > c->d.max_batch) return fail(c, ZYNFER_CU_INVALID, "batch must be 1..max_batch");
+    if (tokens == 0) return fail(c, ZYNFER_CU_INVALID, "tokens must be at least 1");
+    for (uint32_t i = 0; i < batch; ++i) {
+        if (seqs[i] >= c->d.max_seqs) return fail(c, ZYNFER_CU_INVALID, "sequence id out of range");
+        if (c->seq_len[seqs[i]] + extra < tokens)
+            return fail(c, ZYNFER_CU_INVALID, "a sequence is shorter than the queries' positions");
+        rows->slot[i] = (int)seqs[i];
+        rows->len[i] = (int)(c->seq_len[seqs[i]] + extra);
+    }
+    return ZYNFER_CU_OK;
+}
+
+// Changed block-table rows to the device; the pinned copy may be rewritten by
+// the next call, so an upload is waited for (appending within a block changes none).
+int settle_tables(ZynferCuCtx* c, const uint32_t* seqs, uint32_t n) {
+    bool dirty = false;
+    for (uint32_t i = 0; i < n; ++i) dirty = dirty || c->table_dirty[seqs[i]];
+    if (!dirty) return ZYNFER_CU_OK;
+    int rc = upload_table_rows(c, seqs, n);
+    if (rc) return rc;
+    ZC_CHECK(c, cudaStreamSynchronize(c->stream), "block table upload");
+    return ZYNFER_CU_OK;
+}
+
+ServeAttnArgs serve_args(const ZynferCuCtx* c, uint32_t layer, uint32_t batch, uint32_t tokens, uint32_t window,
+                         uint32_t sinks, const void* q, uint64_t q_stride, void* out, uint64_t out_stride, bool bf16) {
+    ServeAttnArgs a{};
+    a.kv_layer = c->kv + layer * c->kv_layer_elems;
+    a.block_table = c->table_dev; a.max_blocks = c->max_blocks; a.n_pool_blocks = c->n_blocks;
+    a.n_kv = (int)c->d.n_kv;
+    a.q = q; a.out = out; a.q_stride = q_stride; a.out_stride = out_stride; a.bf16 = bf16 ? 1 : 0;
+    a.batch = (int)batch; a.tokens = (int)tokens;
+    a.window = window; a.sinks = (int)std::min<uint32_t>(sinks, c->d.max_seq_len);
+    a.err = c->derr;
+    return a;
+}
+
+int check_serve_tensors(ZynferCuCtx* c, uint32_t layer, const void* q, uint64_t q_stride, const void* out,
+                        uint64_t out_stride, int dtype) {
+    if (layer >= c->d.layers) return fail(c, ZYNFER_CU_INVALID, "layer out of range");
+    if (dtype != ZYNFER_CU_DT_F32 && dtype != ZYNFER_CU_DT_BF16)
+        return fail(c, ZYNFER_CU_UNSUPPORTED, "q and out must be f32 or bf16");
+    if (q_stride < (uint64_t)c->qd || out_stride < (uint64_t)c->qd || q_stride % 8 || out_stride % 8)
+        return fail(c, ZYNFER_CU_INVALID, "strides must be multiples of 8, at least n_q * head_dim");
+    if (reinterpret_cast<uintptr_t>(q) % 16 || reinterpret_cast<uintptr_t>(out) % 16)
+        return fail(c, ZYNFER_CU_INVALID, "q and out must be 16-byte aligned");
+    return ZYNFER_CU_OK;
+}
+
 }  // namespace
 
 namespace zc {
@@ -812,6 +869,7 @@ int zynfer_cu_create(int device, ZynferCuCtx** out) {
     }
     cudaEventCreate(&c->ev0);
     cudaEventCreate(&c->ev1);
+    cudaEventCreateWithFlags(&c->ev_order, cudaEventDisableTiming);
     prepare_all_kernels();  // function attributes now, never during a graph capture
     parse_fail_spec(c, getenv("ZYNFER_CUDA_FAIL_AT"));
     *out = c;
@@ -831,6 +889,7 @@ void zynfer_cu_destroy(ZynferCuCtx* c) {
         }
         if (c->ev0) cudaEventDestroy(c->ev0);
         if (c->ev1) cudaEventDestroy(c->ev1);
+        if (c->ev_order) cudaEventDestroy(c->ev_order);
         for (void* p : c->allocs) cudaFree(p);
         for (void* p : c->pinned) cudaFreeHost(p);
         if (c->stream) cudaStreamDestroy(c->stream);
@@ -1207,6 +1266,7 @@ int zynfer_cu_kv_read(ZynferCuCtx* c, uint32_t seq, uint32_t layer, int which_v,
     cudaSetDevice(c->device);
     const int d = c->d.head_dim, nkv = c->d.n_kv;
     const uint32_t len = c->seq_len[seq];
+    ZC_CHECK(c, cudaStreamSynchronize(c->stream), "kv read");  // zynfer_cu_kv_write is asynchronous
     std::vector<uint16_t> blk((size_t)kKvBlock * d);
     for (uint32_t p0 = 0; p0 < len; p0 += kKvBlock) {
         const int b = c->seq_blocks[seq][p0 / kKvBlock];
@@ -1348,6 +1408,281 @@ int zynfer_cu_attn_decode(ZynferCuCtx* c, uint32_t layer, const uint32_t* seqs, 
     if (e != cudaSuccess) return cuda_fail(c, e, "attention launch");
     if ((rc = check_device_error(c))) return rc;
     set_path(c, "attn_decode", 0, nullptr);
+    return ZYNFER_CU_OK;
+}
+
+int zynfer_cu_kv_write(ZynferCuCtx* c, uint32_t seq, uint32_t layer, uint32_t pos, uint32_t n, const void* k,
+                       const void* v, int dtype) {
+    if (!c || !c->ready) return c ? fail(c, ZYNFER_CU_INVALID, "model not initialised") : ZYNFER_CU_INVALID;
+    if (seq >= c->d.max_seqs || layer >= c->d.layers) return fail(c, ZYNFER_CU_INVALID, "index out of range");
+    if (dtype != ZYNFER_CU_DT_F32 && dtype != ZYNFER_CU_DT_BF16)
+        return fail(c, ZYNFER_CU_UNSUPPORTED, "K and V must be f32 or bf16");
+    if (pos > c->seq_len[seq]) return fail(c, ZYNFER_CU_INVALID, "kv_write: pos is past the sequence's length");
+    if ((uint64_t)pos + n > c->d.max_seq_len) return fail(c, ZYNFER_CU_INVALID, "KV cache full");
+    if (n == 0) return ZYNFER_CU_OK;
+    if (!k || !v) return fail(c, ZYNFER_CU_INVALID, "null argument");
+    if (reinterpret_cast<uintptr_t>(k) % 16 || reinterpret_cast<uintptr_t>(v) % 16)
+        return fail(c, ZYNFER_CU_INVALID, "K and V must be 16-byte aligned");
+    const std::vector<int>& bl = c->seq_blocks[seq];
+    for (size_t i = pos / kKvBlock; i < bl.size() && i <= (size_t)(pos + n - 1) / kKvBlock; ++i)
+        if (c->block_refs[bl[i]] > 1)
+            return fail(c, ZYNFER_CU_INVALID, "kv_write: a written block is shared with another sequence");
+    if (take_launch_fault(c)) return ZYNFER_CU_LAUNCH;
+    cudaSetDevice(c->device);
+    int rc = ensure_blocks(c, seq, pos + n);
+    if (rc) return rc;
+    if ((rc = settle_tables(c, &seq, 1))) return rc;
+    KvWriteArgs a{};
+    a.kv_layer = c->kv + layer * c->kv_layer_elems; a.table_row = c->table_dev + (size_t)seq * c->max_blocks;
+    a.n_pool_blocks = c->n_blocks; a.n_kv = (int)c->d.n_kv; a.pos = (int)pos; a.n = (int)n; a.k = k; a.v = v;
+    a.bf16 = dtype == ZYNFER_CU_DT_BF16; a.err = c->derr;
+    launch_kv_write(a, c->stream);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return cuda_fail(c, e, "kv write launch");
+    c->seq_len[seq] = std::max(c->seq_len[seq], pos + n);
+    set_path(c, "kv_write", 0, nullptr);
+    return ZYNFER_CU_OK;
+}
+
+int zynfer_cu_attn_window(ZynferCuCtx* c, uint32_t layer, const uint32_t* seqs, uint32_t batch, uint32_t tokens,
+                          uint32_t window, uint32_t sinks, const void* q, uint64_t q_stride, void* out,
+                          uint64_t out_stride, int dtype) {
+    if (!c || !c->ready) return c ? fail(c, ZYNFER_CU_INVALID, "model not initialised") : ZYNFER_CU_INVALID;
+    if (!seqs || !q || !out) return fail(c, ZYNFER_CU_INVALID, "null argument");
+    int rc = check_serve_tensors(c, layer, q, q_stride, out, out_stride, dtype);
+    if (rc) return rc;
+    ServeRows rows;
+    if ((rc = serve_rows(c, seqs, batch, tokens, 0, &rows))) return rc;
+    if (take_launch_fault(c)) return ZYNFER_CU_LAUNCH;
+    cudaSetDevice(c->device);
+    if ((rc = settle_tables(c, seqs, batch))) return rc;
+    launch_serve_attn(rows, serve_args(c, layer, batch, tokens, window, sinks, q, q_stride, out, out_stride,
+                                       dtype == ZYNFER_CU_DT_BF16), c->stream);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return cuda_fail(c, e, "attention launch");
+    set_path(c, "attn_window", 0, nullptr);
+    return ZYNFER_CU_OK;
+}
+
+int zynfer_cu_attn_shared(ZynferCuCtx* c, uint32_t layer, const uint32_t* seqs, uint32_t batch, const void* q,
+                          uint64_t q_stride, void* out, uint64_t out_stride, int dtype) {
+    if (!c || !c->ready) return c ? fail(c, ZYNFER_CU_INVALID, "model not initialised") : ZYNFER_CU_INVALID;
+    if (!seqs || !q || !out) return fail(c, ZYNFER_CU_INVALID, "null argument");
+    int rc = check_serve_tensors(c, layer, q, q_stride, out, out_stride, dtype);
+    if (rc) return rc;
+    ServeRows rows;
+    if ((rc = serve_rows(c, seqs, batch, 1, 0, &rows))) return rc;
+    if ((rc = validate_batch(c, seqs, batch, 0))) return rc;
+    if (take_launch_fault(c)) return ZYNFER_CU_LAUNCH;
+    cudaSetDevice(c->device);
+    if ((rc = settle_tables(c, seqs, batch))) return rc;
+    launch_serve_attn(rows, serve_args(c, layer, batch, 1, ZYNFER_CU_WINDOW_ALL, 0, q, q_stride, out, out_stride,
+                                       dtype == ZYNFER_CU_DT_BF16), c->stream);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return cuda_fail(c, e, "attention launch");
+    set_path(c, "attn_shared", 0, nullptr);
+    return ZYNFER_CU_OK;
+}
+
+int zynfer_cu_sample_rows(ZynferCuCtx* c, const void* logits, int dtype, uint64_t stride, uint32_t rows, uint32_t vocab,
+                          const float* uniforms, const ZynferCuDrawRule* rule, uint32_t* ids, float* logprobs) {
+    if (!c || c->device < 0) return ZYNFER_CU_INVALID;
+    if (!logits || !uniforms || !ids || rows == 0 || vocab == 0)
+        return fail(c, ZYNFER_CU_INVALID, "bad sample_rows arguments");
+    if (dtype != ZYNFER_CU_DT_F32 && dtype != ZYNFER_CU_DT_BF16)
+        return fail(c, ZYNFER_CU_UNSUPPORTED, "logits must be f32 or bf16");
+    if (vocab > (uint32_t)kDrawMaxVocab) return fail(c, ZYNFER_CU_UNSUPPORTED, "vocab above 262144");
+    if (stride < vocab) return fail(c, ZYNFER_CU_INVALID, "stride is shorter than a row");
+    if (rows > 65535) return fail(c, ZYNFER_CU_INVALID, "rows above 65535");
+    const ZynferCuDrawRule none{};
+    if (!rule) rule = &none;
+    const uintptr_t esz = dtype == ZYNFER_CU_DT_F32 ? 4 : 2;
+    const void* arrays[7] = {uniforms, rule->temperature, rule->top_k, rule->top_p, rule->min_p, ids, logprobs};
+    for (const void* p : arrays)
+        if (reinterpret_cast<uintptr_t>(p) % 4) return fail(c, ZYNFER_CU_INVALID, "arrays must be 4-byte aligned");
+    if (reinterpret_cast<uintptr_t>(logits) % esz) return fail(c, ZYNFER_CU_INVALID, "logits are misaligned");
+    if (take_launch_fault(c)) return ZYNFER_CU_LAUNCH;
+    cudaSetDevice(c->device);
+    DrawArgs a{};
+    a.logits = logits; a.bf16 = dtype == ZYNFER_CU_DT_BF16; a.stride = stride; a.rows = (int)rows; a.vocab = (int)vocab;
+    a.uniforms = uniforms; a.temperature = rule->temperature; a.top_k = rule->top_k; a.top_p = rule->top_p;
+    a.min_p = rule->min_p; a.ids = ids; a.logprobs = logprobs;
+    launch_draw(a, c->stream);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return cuda_fail(c, e, "draw launch");
+    set_path(c, "sample_rows", 0, nullptr);
+    return ZYNFER_CU_OK;
+}
+
+int zynfer_cu_wait_stream(ZynferCuCtx* c, void* stream) {
+    if (!c || c->device < 0) return ZYNFER_CU_INVALID;
+    cudaSetDevice(c->device);
+    ZC_CHECK(c, cudaEventRecord(c->ev_order, static_cast<cudaStream_t>(stream)), "wait_stream");
+    ZC_CHECK(c, cudaStreamWaitEvent(c->stream, c->ev_order, 0), "wait_stream");
+    return ZYNFER_CU_OK;
+}
+
+int zynfer_cu_stream_wait(ZynferCuCtx* c, void* stream) {
+    if (!c || c->device < 0) return ZYNFER_CU_INVALID;
+    cudaSetDevice(c->device);
+    ZC_CHECK(c, cudaEventRecord(c->ev_order, c->stream), "stream_wait");
+    ZC_CHECK(c, cudaStreamWaitEvent(static_cast<cudaStream_t>(stream), c->ev_order, 0), "stream_wait");
+    return ZYNFER_CU_OK;
+}
+
+int zynfer_cu_prefill_chunk(ZynferCuCtx* c, uint32_t seq, const uint32_t* tokens, uint32_t n, uint32_t window,
+                            uint32_t sinks, float* last_logits, uint32_t* argmax) {
+    if (!c || !c->ready) return c ? fail(c, ZYNFER_CU_INVALID, "model not initialised") : ZYNFER_CU_INVALID;
+    if (seq >= c->d.max_seqs) return fail(c, ZYNFER_CU_INVALID, "sequence id out of range");
+    if (n == 0 || !tokens) return fail(c, ZYNFER_CU_INVALID, "empty prompt");
+    const uint32_t pos0 = c->seq_len[seq];
+    if (n > c->d.max_prefill || (uint64_t)pos0 + n > c->d.max_seq_len)
+        return fail(c, ZYNFER_CU_INVALID, "chunk longer than max_prefill, or past max_seq_len");
+    for (uint32_t i = 0; i < n; ++i)
+        if (tokens[i] >= c->d.vocab) return fail(c, ZYNFER_CU_INVALID, "token id >= vocab");
+    if (take_launch_fault(c)) return ZYNFER_CU_LAUNCH;
+    cudaSetDevice(c->device);
+    int rc = ensure_blocks(c, seq, pos0 + n);
+    if (rc) return rc;
+    if ((rc = settle_tables(c, &seq, 1))) return rc;
+    ServeRows rows;
+    if ((rc = serve_rows(c, &seq, 1, n, n, &rows))) return rc;
+    const ZynferCuModelDesc& m = c->d;
+    const int H = m.hidden, T = (int)n;
+    ZC_CHECK(c, cudaMemcpyAsync(c->ptok, tokens, (size_t)n * 4, cudaMemcpyHostToDevice, c->stream), "prompt upload");
+    cudaEventRecord(c->ev0, c->stream);
+    c->step_paths = 0;
+    launch_embed(c->embed, c->sembed, c->wkind, c->ptok, T, H, m.vocab, c->px, c->derr, c->stream);
+    for (uint32_t l = 0; l < m.layers; ++l) {
+        const LayerDev& Ld = c->L[l];
+        linear(c, ZYNFER_CU_K_LINEAR, Ld.wqkv, Ld.sqkv, &Ld.tm_qkv, c->qkv_rows, H, c->px, T, c->pqkv, kEpiNone,
+               nullptr, Ld.input_ln, nullptr);
+        QkvArgs qa{};
+        qa.qkv = c->pqkv; qa.T = T; qa.n_q = m.n_q; qa.n_kv = m.n_kv; qa.d = m.head_dim;
+        qa.q_norm = Ld.q_norm; qa.k_norm = Ld.k_norm; qa.eps = m.eps;
+        qa.rope = c->rope; qa.rope_max_pos = (int)m.max_seq_len;
+        qa.pos0 = (int)pos0; qa.seq0 = (int)seq;
+        qa.kv_layer = c->kv + l * c->kv_layer_elems; qa.block_table = c->table_dev;
+        qa.max_blocks = c->max_blocks; qa.n_pool_blocks = c->n_blocks;
+        qa.q_out = c->pq; qa.err = c->derr;
+        launch_qkv_post(qa, c->stream);
+        launch_serve_attn(rows, serve_args(c, l, 1, n, window, sinks, c->pq, c->qd, c->pattn, c->qd, false), c->stream);
+        linear(c, ZYNFER_CU_K_LINEAR, Ld.wo, Ld.so, &Ld.tm_o, H, c->qd, c->pattn, T, c->px1, kEpiResid, c->px, nullptr,
+               nullptr);
+        linear(c, ZYNFER_CU_K_LINEAR, Ld.wgu, Ld.sgu, &Ld.tm_gu, 2 * (int)m.inter, H, c->px1, T, c->ph, kEpiSwiGLU,
+               nullptr, Ld.post_ln, nullptr);
+        linear(c, ZYNFER_CU_K_LINEAR, Ld.wd, Ld.sd, &Ld.tm_d, H, (int)m.inter, c->ph, T, c->px, kEpiResid, c->px1,
+               nullptr, nullptr);
+    }
+    linear(c, ZYNFER_CU_K_LMHEAD, c->embed, c->sembed, &c->tm_embed, m.vocab, H, c->px + (size_t)(n - 1) * H, 1,
+           last_logits ? c->dlogits : nullptr, kEpiArgmax, nullptr, c->final_norm, c->dkeys);
+    FinalizeArgs fa{};
+    fa.keys = c->dkeys; fa.ids_out = c->dids; fa.B = 1;
+    launch_finalize(fa, c->stream);
+    cudaEventRecord(c->ev1, c->stream);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return cuda_fail(c, e, "prefill launch");
+    if (last_logits)
+        ZC_CHECK(c, cudaMemcpyAsync(last_logits, c->dlogits, (size_t)m.vocab * 4, cudaMemcpyDeviceToHost, c->stream), "logits");
+    ZC_CHECK(c, cudaMemcpyAsync(c->hids, c->dids, 4, cudaMemcpyDeviceToHost, c->stream), "argmax");
+    if ((rc = check_device_error(c))) return rc;
+    float ms = 0.0f;
+    cudaEventElapsedTime(&ms, c->ev0, c->ev1);
+    c->last_step_ns = (uint64_t)(ms * 1e6);
+    if (argmax) *argmax = c->hids[0];
+    c->seq_len[seq] = pos0 + n;
+    set_path(c, "prefill_chunk", c->step_paths, nullptr);
+    return ZYNFER_CU_OK;
+}
+
+int zynfer_cu_decode_drawn(ZynferCuCtx* c, const uint32_t* seqs, const uint32_t* tokens, uint32_t batch,
+                           uint32_t window, uint32_t sinks, const float* uniforms, const ZynferCuDrawRule* rule,
+                           uint32_t* ids, float* logprobs) {
+    if (!c || !c->ready) return c ? fail(c, ZYNFER_CU_INVALID, "model not initialised") : ZYNFER_CU_INVALID;
+    if (!seqs || !tokens || !uniforms || !ids) return fail(c, ZYNFER_CU_INVALID, "null argument");
+    int rc = validate_batch(c, seqs, batch, 1);
+    if (rc) return rc;
+    if (c->d.vocab > (uint32_t)kDrawMaxVocab) return fail(c, ZYNFER_CU_UNSUPPORTED, "vocab above 262144");
+    if (take_launch_fault(c)) return ZYNFER_CU_LAUNCH;
+    cudaSetDevice(c->device);
+    const size_t B = batch, cap = c->d.max_batch;
+    if (!c->hdraw && (rc = halloc(c, &c->hdraw, 6 * cap))) return rc;
+    if (!c->ddraw && (rc = dalloc(c, &c->ddraw, 6 * cap))) return rc;
+    for (uint32_t i = 0; i < batch; ++i)
+        if ((rc = ensure_blocks(c, seqs[i], c->seq_len[seqs[i]] + 1))) return rc;
+    if ((rc = settle_tables(c, seqs, batch))) return rc;
+    ServeRows rows;
+    if ((rc = serve_rows(c, seqs, batch, 1, 1, &rows))) return rc;
+    set_io_views(c, (int)batch);
+    if ((rc = stage_batch(c, seqs, tokens, batch))) return rc;
+    const ZynferCuDrawRule none{};
+    const ZynferCuDrawRule& r = rule ? *rule : none;
+    for (size_t i = 0; i < B; ++i) {
+        c->hdraw[i] = uniforms[i];
+        c->hdraw[B + i] = r.temperature ? r.temperature[i] : 1.0f;
+        const int32_t k = r.top_k ? r.top_k[i] : 0;
+        memcpy(&c->hdraw[2 * B + i], &k, 4);
+        c->hdraw[3 * B + i] = r.top_p ? r.top_p[i] : 1.0f;
+        c->hdraw[4 * B + i] = r.min_p ? r.min_p[i] : 0.0f;
+    }
+    ZC_CHECK(c, cudaMemcpyAsync(c->ddraw, c->hdraw, 5 * B * 4, cudaMemcpyHostToDevice, c->stream), "stage draws");
+    c->h2d_bytes += 5 * B * 4;
+    const ZynferCuModelDesc& m = c->d;
+    const int H = m.hidden, I = m.inter, N = (int)batch;
+    cudaEventRecord(c->ev0, c->stream);
+    c->step_paths = 0;
+    c->step_launches = 0;
+    launch_embed(c->embed, c->sembed, c->wkind, c->dtok, N, H, m.vocab, c->dx, c->derr, c->stream);
+    for (uint32_t l = 0; l < m.layers; ++l) {
+        const LayerDev& Ld = c->L[l];
+        set_prefetch(c, Ld.wo, Ld.so, H, c->qd);
+        linear(c, ZYNFER_CU_K_LINEAR, Ld.wqkv, Ld.sqkv, &Ld.tm_qkv, c->qkv_rows, H, c->dx, N, c->dqkv, kEpiNone, nullptr,
+               Ld.input_ln, nullptr);
+        QkvArgs qa{};
+        qa.qkv = c->dqkv; qa.T = N; qa.n_q = m.n_q; qa.n_kv = m.n_kv; qa.d = m.head_dim;
+        qa.q_norm = Ld.q_norm; qa.k_norm = Ld.k_norm; qa.eps = m.eps;
+        qa.rope = c->rope; qa.rope_max_pos = (int)m.max_seq_len;
+        qa.row_pos = c->dpos; qa.row_seq = c->dseq;
+        qa.kv_layer = c->kv + l * c->kv_layer_elems; qa.block_table = c->table_dev;
+        qa.max_blocks = c->max_blocks; qa.n_pool_blocks = c->n_blocks;
+        qa.q_out = c->dq; qa.err = c->derr;
+        launch_qkv_post(qa, c->stream);
+        launch_serve_attn(rows, serve_args(c, l, batch, 1, window, sinks, c->dq, c->qd, c->dattn, c->qd, false), c->stream);
+        c->step_launches += 2;
+        set_prefetch(c, Ld.wgu, Ld.sgu, 2 * I, H);
+        linear(c, ZYNFER_CU_K_LINEAR, Ld.wo, Ld.so, &Ld.tm_o, H, c->qd, c->dattn, N, c->dx1, kEpiResid, c->dx, nullptr,
+               nullptr);
+        set_prefetch(c, Ld.wd, Ld.sd, H, I);
+        linear(c, ZYNFER_CU_K_LINEAR, Ld.wgu, Ld.sgu, &Ld.tm_gu, 2 * I, H, c->dx1, N, c->dh, kEpiSwiGLU, nullptr,
+               Ld.post_ln, nullptr);
+        if (l + 1 < m.layers) set_prefetch(c, c->L[l + 1].wqkv, c->L[l + 1].sqkv, c->qkv_rows, H);
+        linear(c, ZYNFER_CU_K_LINEAR, Ld.wd, Ld.sd, &Ld.tm_d, H, I, c->dh, N, c->dx, kEpiResid, c->dx1, nullptr, nullptr);
+    }
+    linear(c, ZYNFER_CU_K_LMHEAD, c->embed, c->sembed, &c->tm_embed, m.vocab, H, c->dx, N, c->dlogits, kEpiArgmax,
+           nullptr, c->final_norm, c->dkeys);
+    cudaMemsetAsync(c->dkeys, 0, B * 8, c->stream);  // the argmax is not taken
+    DrawArgs a{};
+    a.logits = c->dlogits; a.stride = m.vocab; a.rows = N; a.vocab = (int)m.vocab;
+    a.uniforms = c->ddraw; a.temperature = c->ddraw + B; a.top_k = reinterpret_cast<const int*>(c->ddraw + 2 * B);
+    a.top_p = c->ddraw + 3 * B; a.min_p = c->ddraw + 4 * B; a.ids = c->dids; a.logprobs = c->ddraw + 5 * B;
+    launch_draw(a, c->stream);
+    c->step_launches += 2;
+    cudaEventRecord(c->ev1, c->stream);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return cuda_fail(c, e, "decode launch");
+    ZC_CHECK(c, cudaMemcpyAsync(c->hids, c->dids, B * 4, cudaMemcpyDeviceToHost, c->stream), "ids");
+    ZC_CHECK(c, cudaMemcpyAsync(c->hdraw + 5 * B, c->ddraw + 5 * B, B * 4, cudaMemcpyDeviceToHost, c->stream), "logprobs");
+    c->d2h_bytes += 2 * B * 4;
+    if ((rc = check_device_error(c))) return rc;
+    float ms = 0.0f;
+    cudaEventElapsedTime(&ms, c->ev0, c->ev1);
+    c->last_step_ns = (uint64_t)(ms * 1e6);
+    for (uint32_t i = 0; i < batch; ++i) {
+        ids[i] = c->hids[i];
+        if (logprobs) logprobs[i] = c->hdraw[5 * B + i];
+        c->seq_len[seqs[i]] += 1;
+    }
+    set_path(c, "decode_drawn", c->step_paths, "eager");
     return ZYNFER_CU_OK;
 }
 

@@ -52,6 +52,8 @@ void prepare_all_kernels() {
     prepare_tc_kernels();
     prepare_sample_kernels();
     prepare_fewrow_kernels();
+    prepare_draw_kernels();
+    prepare_serve_attn_kernels();
 }
 
 int device_sm_count() {

@@ -8,6 +8,7 @@ in-tree library and nothing else: there is no CPU path here.
 from __future__ import annotations
 
 import atexit
+import contextlib
 import ctypes as C
 import os
 import weakref
@@ -20,6 +21,8 @@ LIB_PATH = os.path.join(_HERE, "libzynfer_cuda.so")
 
 OK, NO_DEVICE, OOM, INVALID, UNSUPPORTED, LAUNCH, TIMEOUT, INTERNAL = range(8)
 W_Q8, W_BF16 = 0, 1
+DT_F32, DT_BF16 = 0, 2
+WINDOW_ALL = 0xFFFFFFFF  # the window of full causal attention
 K_ATTN, K_LINEAR, K_LMHEAD, K_OTHER = range(4)
 
 
@@ -74,6 +77,10 @@ class ModelDesc(C.Structure):
                 ("max_prefill", C.c_uint32), ("prefill_kv_f32", C.c_uint32)]
 
 
+class DrawRule(C.Structure):
+    _fields_ = [("temperature", C.c_void_p), ("top_k", C.c_void_p), ("top_p", C.c_void_p), ("min_p", C.c_void_p)]
+
+
 VP = C.c_void_p
 U32 = C.c_uint32
 U64 = C.c_uint64
@@ -112,6 +119,14 @@ _SIGS = {
     "zynfer_cu_linear_q8_static": (C.c_int, [VP, VP, VP, U32, U32, U32, VP, VP]),
     "zynfer_cu_linear_q8_static_status": (C.c_int, [C.c_int]),
     "zynfer_cu_attn_decode": (C.c_int, [VP, U32, VP, U32, VP, VP]),
+    "zynfer_cu_kv_write": (C.c_int, [VP, U32, U32, U32, U32, VP, VP, C.c_int]),
+    "zynfer_cu_attn_shared": (C.c_int, [VP, U32, VP, U32, VP, U64, VP, U64, C.c_int]),
+    "zynfer_cu_attn_window": (C.c_int, [VP, U32, VP, U32, U32, U32, U32, VP, U64, VP, U64, C.c_int]),
+    "zynfer_cu_sample_rows": (C.c_int, [VP, VP, C.c_int, U64, U32, U32, VP, C.POINTER(DrawRule), VP, VP]),
+    "zynfer_cu_wait_stream": (C.c_int, [VP, VP]),
+    "zynfer_cu_stream_wait": (C.c_int, [VP, VP]),
+    "zynfer_cu_prefill_chunk": (C.c_int, [VP, U32, VP, U32, U32, U32, VP, VP]),
+    "zynfer_cu_decode_drawn": (C.c_int, [VP, VP, VP, U32, U32, U32, VP, C.POINTER(DrawRule), VP, VP]),
     "zynfer_cu_rmsnorm_qk_rope": (C.c_int, [VP, VP, U32, VP, VP, U32, VP, VP]),
     "zynfer_cu_swiglu": (C.c_int, [VP, VP, VP, U64, VP]),
     "zynfer_cu_pack_q8": (C.c_int, [VP, VP, U32, U32, VP, VP]),
@@ -161,6 +176,19 @@ def _ptr(a) -> C.c_void_p | None:
     if hasattr(a, "data_ptr"):  # torch tensor (device pointer)
         return C.c_void_p(a.data_ptr())
     return a.ctypes.data_as(C.c_void_p)
+
+
+def _dtype(t) -> int:
+    """ZYNFER_CU_DT_* of a device tensor the serving calls take."""
+    name = str(t.dtype).rsplit(".", 1)[-1]
+    if name not in ("float32", "bfloat16"):
+        raise Unsupported(f"float32 or bfloat16 tensors, not {name}")
+    return DT_F32 if name == "float32" else DT_BF16
+
+
+def _require(ok: bool, what: str):
+    if not ok:
+        raise InvalidArgument(what)
 
 
 STATIC_MAX_ROWS, STATIC_MAX_K = 64, 4096
@@ -279,6 +307,44 @@ class Gpu:
         self.check(lib().zynfer_cu_sample(self.h, _ptr(logits), rows, vocab, _ptr(s), _ptr(p), temperature, top_k,
                                           top_p, seed, _ptr(out)))
         return out
+
+    def sample_rows(self, logits, uniforms, ids, logprobs=None, temperature=None, top_k=None, top_p=None, min_p=None,
+                    stream=None):
+        """The next token of each row of device logits [rows, vocab] (f32 or bf16, rows at any stride) from the
+        random numbers uniforms [rows] into ids [rows] (32-bit) and, where given, logprobs [rows]; temperature,
+        top_k (int32), top_p and min_p are device tensors [rows] or None (zynfer_cu_sample_rows). Asynchronous;
+        `stream` (a torch stream) orders the call after its work and its later work after the call."""
+        _require(len(logits.shape) == 2 and logits.stride(1) == 1, "logits must be [rows, vocab] with unit inner stride")
+        rows, vocab = logits.shape
+        per_row = [("uniforms", uniforms, "float32"), ("ids", ids, "int32"), ("logprobs", logprobs, "float32"),
+                   ("temperature", temperature, "float32"), ("top_k", top_k, "int32"), ("top_p", top_p, "float32"),
+                   ("min_p", min_p, "float32")]
+        for name, t, kind in per_row:
+            if t is not None:
+                got = str(t.dtype).rsplit(".", 1)[-1]
+                _require(got in (kind, "u" + kind) and tuple(t.shape) == (rows,) and (rows == 1 or t.stride(0) == 1),
+                         f"{name} must be a dense {kind} tensor of one value per row")
+        rule = DrawRule(*(None if t is None else t.data_ptr() for t in (temperature, top_k, top_p, min_p)))
+        stride = logits.stride(0) if rows > 1 else vocab
+        with self._ordered(stream):
+            self.check(lib().zynfer_cu_sample_rows(self.h, _ptr(logits), _dtype(logits), stride, rows, vocab,
+                                                   _ptr(uniforms), C.byref(rule), _ptr(ids), _ptr(logprobs)))
+
+    def wait_stream(self, stream):
+        """Later work of this context waits for what `stream` (a torch stream or a cudaStream_t) holds now."""
+        self.check(lib().zynfer_cu_wait_stream(self.h, VP(int(getattr(stream, "cuda_stream", stream or 0)))))
+
+    def stream_wait(self, stream):
+        """Later work of `stream` waits for what this context has enqueued so far."""
+        self.check(lib().zynfer_cu_stream_wait(self.h, VP(int(getattr(stream, "cuda_stream", stream or 0)))))
+
+    @contextlib.contextmanager
+    def _ordered(self, stream):
+        if stream is not None:
+            self.wait_stream(stream)
+        yield
+        if stream is not None:
+            self.stream_wait(stream)
 
     def phase_trace(self):
         """Phase timestamps (ns) of the last persistent decode step run with timing on."""
@@ -420,6 +486,49 @@ class Model:
         s = np.ascontiguousarray(seqs, np.uint32)
         self.gpu.check(lib().zynfer_cu_attn_decode(self.gpu.h, layer, _ptr(s), s.size, _ptr(qkv), _ptr(out)))
 
+    def kv_write(self, seq: int, layer: int, pos: int, k, v, stream=None):
+        """K and V rows (device, dense [n_kv, n, head_dim], f32 or bf16) into positions pos .. pos + n - 1 of a
+        sequence's cache of one layer. Asynchronous."""
+        a = self.arch
+        _require(len(k.shape) == 3 and k.shape == v.shape and k.shape[0] == a.n_kv and k.shape[2] == a.head_dim and
+                 k.dtype == v.dtype and k.is_contiguous() and v.is_contiguous(),
+                 "k and v must be dense [n_kv, n, head_dim] tensors of one type")
+        with self.gpu._ordered(stream):
+            self.gpu.check(lib().zynfer_cu_kv_write(self.gpu.h, seq, layer, pos, k.shape[1], _ptr(k), _ptr(v), _dtype(k)))
+
+    def _serve_rows(self, t, lead):
+        """Row stride of a [.., n_q, head_dim] tensor whose leading dimensions `lead` are rows at one stride."""
+        a, shape, st = self.arch, tuple(t.shape), t.stride()
+        _require(shape == (*lead, a.n_q, a.head_dim), f"expected a tensor of shape {(*lead, a.n_q, a.head_dim)}, not {shape}")
+        _require(st[-1] == 1 and st[-2] == a.head_dim, "a row's heads must be dense")
+        rows = [(n, s) for n, s in zip(lead, st) if n > 1]
+        for (_, outer), (n, inner) in zip(rows, rows[1:]):
+            _require(outer == n * inner, "rows must lie at one stride")
+        return rows[-1][1] if rows else a.n_q * a.head_dim
+
+    def attn_shared(self, layer: int, seqs, q, out, stream=None):
+        """Decode attention of one query per sequence (device q and out [B, n_q, head_dim], f32 or bf16, rows at
+        any stride) over all cached positions; leading blocks that sequences share are read once. Asynchronous."""
+        s = np.ascontiguousarray(seqs, np.uint32)
+        _require(q.dtype == out.dtype, "q and out must have one type")
+        qs, os_ = self._serve_rows(q, (s.size,)), self._serve_rows(out, (s.size,))
+        with self.gpu._ordered(stream):
+            self.gpu.check(lib().zynfer_cu_attn_shared(self.gpu.h, layer, _ptr(s), s.size, _ptr(q), qs, _ptr(out), os_,
+                                                       _dtype(q)))
+
+    def attn_window(self, layer: int, seqs, q, out, window: int = WINDOW_ALL, sinks: int = 0, stream=None):
+        """Attention of the last T cached positions of each sequence (device q and out [B, T, n_q, head_dim], or
+        [B, n_q, head_dim] for T = 1) over the last `window` positions up to each and the first `sinks`. Asynchronous."""
+        s = np.ascontiguousarray(seqs, np.uint32)
+        _require(q.dtype == out.dtype, "q and out must have one type")
+        _require(len(q.shape) in (3, 4) and window >= 0 and sinks >= 0, "q must be [B, n_q, d] or [B, T, n_q, d]")
+        lead = (s.size,) if len(q.shape) == 3 else (s.size, q.shape[1])
+        qs, os_ = self._serve_rows(q, lead), self._serve_rows(out, lead)
+        with self.gpu._ordered(stream):
+            self.gpu.check(lib().zynfer_cu_attn_window(self.gpu.h, layer, _ptr(s), s.size, lead[1] if len(lead) > 1 else 1,
+                                                       min(window, WINDOW_ALL), min(sinks, WINDOW_ALL), _ptr(q), qs,
+                                                       _ptr(out), os_, _dtype(q)))
+
     def rmsnorm_qk_rope(self, qkv, rows: int, q_norm, k_norm, pos0: int, q_out, k_out):
         """Per-head q/k RMSNorm + RoPE of `rows` tokens (device pointers, heads-major outputs)."""
         self.gpu.check(lib().zynfer_cu_rmsnorm_qk_rope(self.gpu.h, _ptr(qkv), rows, _ptr(q_norm), _ptr(k_norm),
@@ -457,6 +566,34 @@ class Model:
         ms = C.c_float()
         self.gpu.check(lib().zynfer_cu_generate(self.gpu.h, _ptr(s), _ptr(f), s.size, steps, _ptr(out), C.byref(ms)))
         return out, float(ms.value)
+
+    def prefill_chunk(self, seq: int, tokens, window: int = WINDOW_ALL, sinks: int = 0, want_logits: bool = True):
+        """Append a chunk of a prompt to a sequence, with windowed attention; the last token's logits and argmax."""
+        t = np.ascontiguousarray(tokens, np.uint32)
+        logits = np.empty(self.arch.vocab, np.float32) if want_logits else None
+        am = np.zeros(1, np.uint32)
+        self.gpu.check(lib().zynfer_cu_prefill_chunk(self.gpu.h, seq, _ptr(t), t.size, window, sinks, _ptr(logits), _ptr(am)))
+        return (logits, int(am[0])) if want_logits else int(am[0])
+
+    def decode_drawn(self, seqs, tokens, uniforms, temperature=None, top_k=None, top_p=None, min_p=None,
+                     window: int = WINDOW_ALL, sinks: int = 0):
+        """One decode step whose attention shares common leading blocks (or is windowed) and whose tokens are drawn
+        from `uniforms` by a rule per row (scalars or host arrays): ids and log-probabilities."""
+        s = np.ascontiguousarray(seqs, np.uint32)
+        t = np.ascontiguousarray(tokens, np.uint32)
+        u = np.ascontiguousarray(uniforms, np.float32)
+        _require(t.size == s.size and u.size == s.size, "one token and one random number per sequence")
+
+        def per_row(x, kind):
+            return None if x is None else np.ascontiguousarray(np.broadcast_to(np.asarray(x, kind), (s.size,)))
+
+        arrays = [per_row(temperature, np.float32), per_row(top_k, np.int32), per_row(top_p, np.float32),
+                  per_row(min_p, np.float32)]
+        rule = DrawRule(*(None if x is None else x.ctypes.data for x in arrays))
+        ids, lp = np.zeros(s.size, np.uint32), np.zeros(s.size, np.float32)
+        self.gpu.check(lib().zynfer_cu_decode_drawn(self.gpu.h, _ptr(s), _ptr(t), s.size, window, sinks, _ptr(u),
+                                                    C.byref(rule), _ptr(ids), _ptr(lp)))
+        return ids, lp
 
     def block_forward(self, layer: int, seq: int, x):
         x = np.ascontiguousarray(x, np.float32)
