@@ -182,9 +182,10 @@ def prepare(case, seed):
 def _prepare_sample(case, g, normal, dtype):
     rows, vocab, rule = case["rows"], case["vocab"], case["rule"]
     logits = normal(rows, vocab, scale=2.5)
-    # a model's logits: a broad body and a few tokens well above it
+    # a model's logits: a broad body and a few tokens well above it (the larger where two meet: a plain scatter would
+    # take either, and the inputs would not follow from the seed)
     at = torch.randint(vocab, (rows, 24), generator=g, device="cuda")
-    logits.scatter_(1, at, 6.0 + 2.5 * torch.randn((rows, 24), generator=g, device="cuda"))
+    logits.scatter_reduce_(1, at, 6.0 + 2.5 * torch.randn((rows, 24), generator=g, device="cuda"), "amax")
     logits = logits.to(dtype)
     if rule == "mixed":  # some vocabulary entries are ruled out, as by a grammar
         logits[::3, ::7] = float("-inf")
