@@ -59,6 +59,8 @@ def window_seen(length, tokens, window, sinks):
 def check(got, want, v, dtype):
     tol = (1e-4 if dtype == "f32" else 2.0 ** -8) * float(v.float().abs().max())
     assert got.dtype == DTYPES[dtype]
+    if not got.numel():
+        return
     off = float((got.double() - want).abs().max())
     assert off <= tol, (off, tol)
 
@@ -309,3 +311,58 @@ def test_pool_exhaustion_is_reported():
     k = normal(1, 2, 33, D)
     with pytest.raises(zc.OutOfMemory):
         m.kv_write(0, 0, 0, k, k)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_masked_nan_and_infinity_do_not_spread(value, dtype):
+    """A position's NaN or infinity (in V, in K) reaches exactly the queries that see it."""
+    m = make(n_kv=2)
+    n, tokens, window, sinks = 300, 200, 40, 3
+    for which, where in (("v", 171), ("k", 230), ("v", 299), ("v", 1)):
+        k, v = normal(11, 2, n, D, dtype=torch.bfloat16), normal(12, 2, n, D, dtype=torch.bfloat16)
+        clean_k, clean_v = k.clone(), v.clone()
+        (v if which == "v" else k)[1, where, 5:9] = value
+        m.seq_reset(0)
+        m.kv_write(0, 0, 0, k, v)
+        q = normal(13, 1, tokens, 4, D, dtype=DTYPES[dtype])
+        out = torch.empty_like(q)
+        torch.cuda.synchronize()
+        m.attn_window(0, [0], q, out, window=window, sinks=sinks)
+        m.gpu.sync()
+        seen = window_seen(n, tokens, window, sinks)
+        want = reference(q[0], clean_k, clean_v, seen)
+        sees = seen[:, where]
+        check(out[0, :, :2], want[:, :2], clean_v, dtype)                     # the other kv head
+        check(out[0, ~sees][:, 2:], want[~sees][:, 2:], clean_v, dtype)       # queries that do not see it
+        hit = out[0, sees][:, 2:]
+        if which == "v":
+            assert not torch.isfinite(hit[..., 5:9]).any()
+            rest = torch.cat([hit[..., :5], hit[..., 9:]], -1)
+            w = want[sees][:, 2:]
+            check(rest, torch.cat([w[..., :5], w[..., 9:]], -1), clean_v, dtype)
+        elif value != value:
+            assert torch.isnan(hit).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_shared_prompt_nan_stays_in_its_dims(dtype):
+    m = make(n_kv=2)
+    k, v = normal(21, 2, 400, D, dtype=torch.bfloat16), normal(22, 2, 400, D, dtype=torch.bfloat16)
+    clean = v.clone()
+    v[0, 37, 64] = float("nan")
+    m.kv_write(0, 0, 0, k, v)
+    for s in range(1, 6):
+        m.seq_fork(s, 0, 400)
+    q = normal(23, 6, 4, D, dtype=DTYPES[dtype])
+    out = torch.empty_like(q)
+    torch.cuda.synchronize()
+    m.attn_shared(0, range(6), q, out)
+    m.gpu.sync()
+    seen = torch.ones(1, 400, dtype=torch.bool, device="cuda")
+    for i in range(6):
+        want = reference(q[i:i + 1], k, clean, seen)
+        assert torch.isnan(out[i, :2, 64]).all()
+        keep = torch.tensor([d for d in range(D) if d != 64], device="cuda")
+        check(out[i:i + 1][..., keep], want[..., keep], clean, dtype)
+        check(out[i:i + 1, 2:], want[:, 2:], clean, dtype)

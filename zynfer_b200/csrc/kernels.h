@@ -155,17 +155,31 @@ constexpr int kDrawMaxVocab = 1 << 18;
 void prepare_draw_kernels();
 void launch_draw(const DrawArgs& a, cudaStream_t st);
 
-// serve_attn.cu: attention of the serving paths over the paged cache. The
-// batch's sequences travel as a kernel parameter: a call copies nothing.
+// serve_attn.cu, attn_tile.cu: attention of the serving paths over the paged
+// cache. The batch's sequences travel as a kernel parameter: a call copies
+// nothing to the device.
 constexpr int kServeMaxBatch = 1024;
+constexpr int kServeRecord = 132;  // words of a partial result: m, l, -, -, acc[128]
 struct ServeRows {
     int slot[kServeMaxBatch];  // sequence slot (block-table row)
     int len[kServeMaxBatch];   // cached positions, the queries' own among them
+    int row[kServeMaxBatch];   // row of q and out (one query per sequence)
+    int skip[kServeMaxBatch];  // leading blocks that the row's tile takes
+    int nrec[kServeMaxBatch];  // partial results that the tile leaves
+};
+// Rows that share leading blocks, in tiles of up to 64.
+constexpr int kServeMaxTiles = kServeMaxBatch / 2;
+struct TileList {
+    int n;                         // 0: tiles are chunks of sequences instead
+    int item0[kServeMaxTiles + 1]; // first work item; (item0[e + 1] - item0[e]) / n_kv splits of its blocks
+    short first[kServeMaxTiles], count[kServeMaxTiles];  // rows of ServeRows
+    int blocks[kServeMaxTiles];    // common leading blocks
 };
 struct ServeAttnArgs {
     const uint16_t* kv_layer;  // [n_kv][blocks][K, V][16][d], rows chunk-swizzled (kv_swizzle)
     const int* block_table;    // [seqs][max_blocks]
     int max_blocks, n_pool_blocks, n_kv;
+    int kv_row0, kv_rows;      // the layer's first row and the number of rows of the pool's tensor map
     const void* q;             // row (b, t) at (b tokens + t) q_stride: [n_q][d] f32 or bf16
     void* out;                 // the same with out_stride
     unsigned long long q_stride, out_stride;  // elements
@@ -173,8 +187,14 @@ struct ServeAttnArgs {
     int batch, tokens;         // query (b, t) sits at position len[b] - tokens + t
     uint32_t window;           // it sees the last `window` positions up to its own ..
     int sinks;                 // .. and the first `sinks` of the sequence
+    int nsplit;                // chunk: CTAs that share a tile's blocks
+    float* part;               // [row][n_q][max_segs][kServeRecord]
+    int max_segs;
     uint32_t* err;
 };
+void prepare_attn_tile_kernels();
+void launch_serve_simple(const ServeRows& rows, const ServeAttnArgs& a, cudaStream_t st);
+void launch_serve_merge(const ServeRows& rows, const ServeAttnArgs& a, cudaStream_t st);
 struct KvWriteArgs {
     uint16_t* kv_layer;
     const int* table_row;      // the sequence's device block-table row
@@ -185,7 +205,6 @@ struct KvWriteArgs {
     uint32_t* err;
 };
 void prepare_serve_attn_kernels();
-void launch_serve_attn(const ServeRows& rows, const ServeAttnArgs& a, cudaStream_t st);
 void launch_kv_write(const KvWriteArgs& a, cudaStream_t st);
 
 // gemv.cu (N <= 8)

@@ -6,79 +6,70 @@
 // Both compute o = sum_j softmax_j(q . k_j / sqrt(d)) v_j per query head, with
 // the maximum, the sum and the accumulators in f32 (attentionInto,
 // src/backends/cpu/ops.zig:285-354, is the case without sharing or window).
-#include "common.cuh"
-#include "kernels.h"
+#include <algorithm>
+
+#include "serve_common.cuh"
 
 namespace zc {
 
 namespace {
 
-constexpr int kD = 128, kG = 2;  // head dim, query heads per kv head
-constexpr int kBlockElems = kKvBlock * kD;
+using namespace serve;
 
-__device__ __forceinline__ float load_q(const void* p, size_t i, int bf16) {
-    return bf16 ? bf16lo(static_cast<const uint16_t*>(p)[i]) : static_cast<const float*>(p)[i];
-}
-
-// One warp per (query row, kv head): every visible position in turn, lane l
-// holding dims 4 l .. 4 l + 3 of both query heads.
-__global__ void __launch_bounds__(128) serve_attn_simple_kernel(const __grid_constant__ ServeRows rows, ServeAttnArgs a) {
+// One warp per (query row, query head) over the blocks after the row's common
+// ones, position by position.
+__global__ void __launch_bounds__(128) serve_attn_simple_kernel(const __grid_constant__ ServeRows rows,
+                                                               const __grid_constant__ ServeAttnArgs a) {
     pdl_wait();
     pdl_launch_dependents();
-    const int lane = threadIdx.x % kWarp;
+    const int n_q = a.n_kv * kG;
     const long long w = ((long long)blockIdx.x * blockDim.x + threadIdx.x) / kWarp;
-    if (w >= (long long)a.batch * a.tokens * a.n_kv) return;
-    const int head = (int)(w % a.n_kv);
-    const long long qrow = w / a.n_kv;
-    const int b = (int)(qrow / a.tokens), t = (int)(qrow % a.tokens);
-    const int len = rows.len[b], pos = len - a.tokens + t;
-    const int* table = a.block_table + (size_t)rows.slot[b] * a.max_blocks;
-    float q[kG][4], acc[kG][4] = {}, m[kG], l[kG] = {0.0f, 0.0f};
-    const float scale = 1.0f / sqrtf((float)kD);
-#pragma unroll
-    for (int h = 0; h < kG; ++h) {
-        m[h] = -INFINITY;
-        for (int e = 0; e < 4; ++e)
-            q[h][e] = load_q(a.q, (size_t)qrow * a.q_stride + (head * kG + h) * kD + 4 * lane + e, a.bf16) * scale;
+    if (w >= (long long)a.batch * a.tokens * n_q) return;
+    const int hq = (int)(w % n_q);
+    const int qi = (int)(w / n_q);
+    const int b = qi / a.tokens, pos = rows.len[b] - a.tokens + qi % a.tokens;
+    const Span span = span_of(pos, pos, a.window, a.sinks, rows.skip[b]);
+    const int qrow = a.tokens == 1 ? rows.row[b] : qi;
+    const SlowRow r = slow_row(a, qrow, hq, rows.slot[b], pos, window_low(pos, a.window), a.sinks, span, 0, span.total);
+    if (rows.nrec[b] == 0) store_row(a, qrow, hq, r);
+    else store_record(a.part + (((size_t)b * n_q + hq) * a.max_segs + rows.nrec[b]) * kRecord, r);
+}
+
+// The records of a (row, query head) joined: o = sum acc 2^(m - M) / sum l 2^(m - M).
+// A warp per (row, query head); rows with one partial result wrote the output.
+__global__ void __launch_bounds__(128) serve_merge_kernel(const __grid_constant__ ServeRows rows,
+                                                          const __grid_constant__ ServeAttnArgs a) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const int n_q = a.n_kv * kG, lane = threadIdx.x % kWarp;
+    const long long w = ((long long)blockIdx.x * blockDim.x + threadIdx.x) / kWarp;
+    if (w >= (long long)a.batch * a.tokens * n_q) return;
+    const int hq = (int)(w % n_q);
+    const int qi = (int)(w / n_q);
+    int n = a.nsplit, qrow = qi;
+    if (a.tokens == 1) {
+        qrow = rows.row[qi];
+        if (a.nsplit <= 1) n = rows.nrec[qi] + 1;
     }
-    const long long low = (long long)pos - a.window + 1;  // first position inside the window
-    for (int j = 0; j <= pos; ++j) {
-        if (j >= a.sinks && j < low) {
-            j = (int)low - 1;
-            continue;
-        }
-        const int id = table[j / kKvBlock];
-        if (id < 0 || id >= a.n_pool_blocks) {
-            if (lane == 0 && a.err) atomicOr(a.err, kErrBadIndex);
-            return;
-        }
-        const uint16_t* k = a.kv_layer + ((size_t)head * a.n_pool_blocks + id) * 2 * kBlockElems;
-        const uint2 kb = *reinterpret_cast<const uint2*>(k + kv_swizzle(j % kKvBlock, 4 * lane));
-        const uint2 vb = *reinterpret_cast<const uint2*>(k + kBlockElems + kv_swizzle(j % kKvBlock, 4 * lane));
-        const float kf[4] = {bf16lo(kb.x), bf16hi(kb.x), bf16lo(kb.y), bf16hi(kb.y)};
-        const float vf[4] = {bf16lo(vb.x), bf16hi(vb.x), bf16lo(vb.y), bf16hi(vb.y)};
-#pragma unroll
-        for (int h = 0; h < kG; ++h) {
-            float s = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s += q[h][e] * kf[e];
-            s = warp_sum(s);
-            const float mn = fmaxf(m[h], s);
-            const float c = mn == -INFINITY ? 1.0f : expf(m[h] - mn), p = mn == -INFINITY ? 0.0f : expf(s - mn);
-            m[h] = mn;
-            l[h] = l[h] * c + p;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[h][e] = acc[h][e] * c + p * vf[e];
-        }
+    if (n == 1) return;
+    const float* rec = a.part + ((size_t)qi * n_q + hq) * a.max_segs * kRecord;
+    float M = -INFINITY;
+    for (int i = lane; i < n; i += kWarp) M = fmaxf(M, __ldcg(rec + (size_t)i * kRecord));
+    M = warp_max(M);
+    float l = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+        const float2 ml = __ldcg(reinterpret_cast<const float2*>(rec + (size_t)i * kRecord));
+        const float4 x = __ldcg(reinterpret_cast<const float4*>(rec + (size_t)i * kRecord + 4 + 4 * lane));
+        if (ml.x == -INFINITY) continue;
+        const float c = exp2f(ml.x - M);
+        l += ml.y * c;
+        acc[0] += x.x * c;
+        acc[1] += x.y * c;
+        acc[2] += x.z * c;
+        acc[3] += x.w * c;
     }
-#pragma unroll
-    for (int h = 0; h < kG; ++h)
-        for (int e = 0; e < 4; ++e) {
-            const float o = l[h] > 0.0f ? acc[h][e] / l[h] : (l[h] == 0.0f ? 0.0f : acc[h][e] / l[h]);
-            const size_t at = (size_t)qrow * a.out_stride + (head * kG + h) * kD + 4 * lane + e;
-            if (a.bf16) static_cast<uint16_t*>(a.out)[at] = f32_to_bf16_rne(o);
-            else static_cast<float*>(a.out)[at] = o;
-        }
+    store_out4(a, qrow, hq, acc, l);
 }
 
 // K and V rows [n_kv][n][128] (f32 rounded to nearest even, or bf16) into
@@ -117,9 +108,14 @@ __global__ void __launch_bounds__(256) kv_write_kernel(KvWriteArgs a) {
 
 }  // namespace
 
-void launch_serve_attn(const ServeRows& rows, const ServeAttnArgs& a, cudaStream_t st) {
-    const long long warps = (long long)a.batch * a.tokens * a.n_kv;
+void launch_serve_simple(const ServeRows& rows, const ServeAttnArgs& a, cudaStream_t st) {
+    const long long warps = (long long)a.batch * a.tokens * a.n_kv * kG;
     launch_pdl(serve_attn_simple_kernel, (unsigned)((warps + 3) / 4), 128, 0, st, rows, a);
+}
+
+void launch_serve_merge(const ServeRows& rows, const ServeAttnArgs& a, cudaStream_t st) {
+    const long long warps = (long long)a.batch * a.tokens * a.n_kv * kG;
+    launch_pdl(serve_merge_kernel, (unsigned)((warps + 3) / 4), 128, 0, st, rows, a);
 }
 
 void launch_kv_write(const KvWriteArgs& a, cudaStream_t st) {
@@ -130,6 +126,7 @@ void launch_kv_write(const KvWriteArgs& a, cudaStream_t st) {
 
 void prepare_serve_attn_kernels() {
     configure_kernel((const void*)serve_attn_simple_kernel, 0);
+    configure_kernel((const void*)serve_merge_kernel, 0);
     configure_kernel((const void*)kv_write_kernel, 0);
 }
 

@@ -142,6 +142,12 @@ struct ZynferCuCtx {
     uint32_t* hids = nullptr;  // pinned [max_batch]
 
     CUtensorMap tm_embed;
+    CUtensorMap tm_kv;                  // the KV pool (serving attention)
+    float* serve_part = nullptr;        // its partial results
+    size_t serve_part_words = 0;
+    std::vector<int> serve_mark;        // [pool blocks] scratch of plan_shared: group of a first block, -1
+    ServeRows serve_rows;               // the batch of the call (host)
+    TileList serve_tiles;
     // tcgen05 linear scratch: activation planes and per-row exponents, plus
     // B-operand descriptors per (kind, K, NT)
     uint8_t* planes = nullptr;
@@ -751,19 +757,177 @@ void enqueue_prefill_layers(ZynferCuCtx* c, uint32_t seq, int T, uint32_t l0, ui
 
 // ---- serving attention (serve_attn.cu)
 
-// The checks of a serving-attention call's batch; rows receives its slots and
-// lengths, `extra` positions past the cached ones included.
-int serve_rows(ZynferCuCtx* c, const uint32_t* seqs, uint32_t batch, uint32_t tokens, uint32_t extra, ServeRows* rows) {
+// The checks of a serving-attention call's batch; c->serve_rows receives its
+// slots and lengths, `extra` positions past the cached ones included.
+int serve_batch(ZynferCuCtx* c, const uint32_t* seqs, uint32_t batch, uint32_t tokens, uint32_t extra) {
     if (batch == 0 || batch > c->d.max_batch) return fail(c, ZYNFER_CU_INVALID, "batch must be 1..max_batch");
     if (tokens == 0) return fail(c, ZYNFER_CU_INVALID, "tokens must be at least 1");
+    ServeRows& rows = c->serve_rows;
     for (uint32_t i = 0; i < batch; ++i) {
         if (seqs[i] >= c->d.max_seqs) return fail(c, ZYNFER_CU_INVALID, "sequence id out of range");
         if (c->seq_len[seqs[i]] + extra < tokens)
             return fail(c, ZYNFER_CU_INVALID, "a sequence is shorter than the queries' positions");
-        rows->slot[i] = (int)seqs[i];
-        rows->len[i] = (int)(c->seq_len[seqs[i]] + extra);
+        rows.slot[i] = (int)seqs[i];
+        rows.len[i] = (int)(c->seq_len[seqs[i]] + extra);
+        rows.row[i] = (int)i;
+        rows.skip[i] = rows.nrec[i] = 0;
     }
     return ZYNFER_CU_OK;
+}
+
+// Leading blocks that two sequences hold in common. Sequences come to hold one
+// block only through zynfer_cu_seq_fork, which takes every block before it
+// too, so equal blocks are a prefix and a binary search finds its end.
+int common_blocks(const std::vector<int>& a, const std::vector<int>& b) {
+    size_t lo = 0, hi = std::min(a.size(), b.size());
+    while (lo < hi) {
+        const size_t mid = (lo + hi) / 2;
+        if (a[mid] == b[mid]) lo = mid + 1;
+        else hi = mid;
+    }
+    return (int)lo;
+}
+
+// Rows [r0, r1) whose neighbours hold common[r] blocks together (row r and r +
+// 1): cut into runs so that the most block reads are saved. A run of n rows with
+// d blocks in common saves (n - 1) d; it is taken whole unless its parts
+// between the least common neighbours save more. leaf(r0, r1, d) takes a run.
+template <typename Leaf>
+long long cut_runs(const int* common, int r0, int r1, bool emit, Leaf&& leaf) {
+    if (r1 - r0 < 2) return 0;
+    int lo = common[r0], hi = lo;
+    for (int r = r0; r + 1 < r1; ++r) {
+        lo = std::min(lo, common[r]);
+        hi = std::max(hi, common[r]);
+    }
+    const long long whole = (long long)(r1 - r0 - 1) * lo;
+    long long parts = -1;
+    if (hi > lo) {
+        parts = 0;
+        for (int a = r0, r = r0; r < r1; ++r)
+            if (r + 1 == r1 || common[r] == lo) {
+                parts += cut_runs(common, a, r + 1, false, leaf);
+                a = r + 1;
+            }
+    }
+    if (emit) {
+        if (whole >= parts) {
+            if (lo > 0) leaf(r0, r1, lo);
+        } else {
+            for (int a = r0, r = r0; r < r1; ++r)
+                if (r + 1 == r1 || common[r] == lo) {
+                    cut_runs(common, a, r + 1, true, leaf);
+                    a = r + 1;
+                }
+        }
+    }
+    return std::max(whole, parts);
+}
+
+// Common leading blocks of the rows of c->serve_rows (one query each): the
+// rows reordered so that rows with the same first block are neighbours, in the
+// caller's order otherwise; the runs that share blocks as tiles of 64 rows,
+// each tile's blocks split over CTAs so that all tiles fill the GPU once.
+// Returns the work items (0: nothing is shared).
+int plan_shared(ZynferCuCtx* c, uint32_t batch, bool bf16, int* max_segs) {
+    ServeRows& rows = c->serve_rows;
+    TileList& list = c->serve_tiles;
+    list.n = 0;
+    *max_segs = 1;
+    if (batch < 2) return 0;
+    // counting sort by first block
+    int group[kServeMaxBatch], count[kServeMaxBatch + 1] = {0}, at[kServeMaxBatch], n = 0;
+    for (uint32_t i = 0; i < batch; ++i) {
+        int& mark = c->serve_mark[c->seq_blocks[rows.slot[i]][0]];
+        if (mark < 0) mark = n++;
+        group[i] = mark;
+        count[mark + 1] += 1;
+    }
+    for (uint32_t i = 0; i < batch; ++i) c->serve_mark[c->seq_blocks[rows.slot[i]][0]] = -1;
+    if (n == (int)batch) return 0;
+    for (int g = 0; g < n; ++g) count[g + 1] += count[g];
+    int order[kServeMaxBatch], common[kServeMaxBatch];
+    for (int g = 0; g < n; ++g) at[g] = count[g];
+    for (uint32_t i = 0; i < batch; ++i) order[at[group[i]]++] = (int)i;
+    int slot[kServeMaxBatch], len[kServeMaxBatch];
+    std::copy(rows.slot, rows.slot + batch, slot);
+    std::copy(rows.len, rows.len + batch, len);
+    for (uint32_t i = 0; i < batch; ++i) {
+        rows.slot[i] = slot[order[i]];
+        rows.len[i] = len[order[i]];
+        rows.row[i] = order[i];
+    }
+    for (uint32_t i = 0; i + 1 < batch; ++i)
+        common[i] = group[order[i]] == group[order[i + 1]]
+                        ? common_blocks(c->seq_blocks[rows.slot[i]], c->seq_blocks[rows.slot[i + 1]]) : 0;
+    const int tile_blocks = attn_tile_blocks(bf16);
+    long long work = 0;
+    for (int g = 0; g < n; ++g)
+        cut_runs(common, count[g], count[g + 1], true, [&](int r0, int r1, int d) {
+            for (int r = r0; r < r1; r += 64) {
+                const int e = list.n++;
+                list.first[e] = (short)r;
+                list.count[e] = (short)std::min(64, r1 - r);
+                list.blocks[e] = d;
+                work += (long long)((d + tile_blocks - 1) / tile_blocks) * c->d.n_kv;
+            }
+        });
+    const int sms = c->caps.sm_count > 0 ? c->caps.sm_count : 148;
+    const int per = (int)std::max<long long>(2, (work + sms - 1) / sms);
+    int items = 0;
+    for (int e = 0; e < list.n; ++e) {
+        const int tiles = (list.blocks[e] + tile_blocks - 1) / tile_blocks, split = (tiles + per - 1) / per;
+        list.item0[e] = items;
+        items += split * (int)c->d.n_kv;
+        *max_segs = std::max(*max_segs, split + 1);
+        for (int r = list.first[e]; r < list.first[e] + list.count[e]; ++r) {
+            rows.skip[r] = list.blocks[e];
+            rows.nrec[r] = split;
+        }
+    }
+    list.item0[list.n] = items;
+    return items;
+}
+
+int serve_scratch(ZynferCuCtx* c, size_t words) {
+    if (words <= c->serve_part_words) return ZYNFER_CU_OK;
+    int rc = dalloc(c, &c->serve_part, words);  // the smaller buffer stays in c->allocs until destroy
+    if (rc == ZYNFER_CU_OK) c->serve_part_words = words;
+    else c->serve_part_words = 0;
+    return rc;
+}
+
+// The launches of a planned call (items from plan_shared; tokens > 1 or a
+// window: a chunk, whose plan is made here).
+struct ServePlan {
+    bool chunk = false;
+    int items = 0, nsplit = 1, max_segs = 1;
+};
+
+int plan_serve(ZynferCuCtx* c, uint32_t batch, uint32_t tokens, uint32_t window, uint32_t sinks, bool shared, bool bf16,
+               ServePlan* p) {
+    *p = ServePlan{};
+    if (shared) {
+        p->items = plan_shared(c, batch, bf16, &p->max_segs);
+    } else if (tokens > 1) {
+        p->chunk = true;
+        c->serve_tiles.n = 0;
+        const long long tiles = (long long)batch * ((tokens + 63) / 64) * c->d.n_kv;
+        p->items = (int)tiles;
+    }
+    if (p->max_segs > 1) return serve_scratch(c, (size_t)batch * tokens * c->d.n_q * p->max_segs * kServeRecord);
+    (void)window; (void)sinks;
+    return ZYNFER_CU_OK;
+}
+
+void enqueue_serve(ZynferCuCtx* c, const ServePlan& p, ServeAttnArgs a) {
+    a.nsplit = p.nsplit;
+    a.max_segs = p.max_segs;
+    a.part = c->serve_part;
+    if (p.items) launch_attn_tile(c->tm_kv, c->serve_rows, c->serve_tiles, a, p.items, c->stream);
+    if (p.chunk && p.nsplit == 1) return;
+    if (!p.chunk) launch_serve_simple(c->serve_rows, a, c->stream);
+    if (p.max_segs > 1) launch_serve_merge(c->serve_rows, a, c->stream);
 }
 
 // Changed block-table rows to the device; the pinned copy may be rewritten by
@@ -784,6 +948,8 @@ ServeAttnArgs serve_args(const ZynferCuCtx* c, uint32_t layer, uint32_t batch, u
     a.kv_layer = c->kv + layer * c->kv_layer_elems;
     a.block_table = c->table_dev; a.max_blocks = c->max_blocks; a.n_pool_blocks = c->n_blocks;
     a.n_kv = (int)c->d.n_kv;
+    a.kv_rows = (int)((size_t)c->d.layers * c->d.n_kv * c->n_blocks * 2 * kKvBlock);
+    a.kv_row0 = (int)((size_t)layer * c->d.n_kv * c->n_blocks * 2 * kKvBlock);
     a.q = q; a.out = out; a.q_stride = q_stride; a.out_stride = out_stride; a.bf16 = bf16 ? 1 : 0;
     a.batch = (int)batch; a.tokens = (int)tokens;
     a.window = window; a.sinks = (int)std::min<uint32_t>(sinks, c->d.max_seq_len);
@@ -1054,6 +1220,10 @@ int zynfer_cu_model_init(ZynferCuCtx* c, const ZynferCuModelDesc* desc) {
             !make_tmap_k_major(&Ld.tm_d, Ld.wd, c->wkind, I, H, 128))
             return fail(c, ZYNFER_CU_INTERNAL, "cuTensorMapEncodeTiled failed for a weight matrix");
     }
+    if (!make_tmap_kv(&c->tm_kv, c->kv, (uint64_t)m.layers * m.n_kv * c->n_blocks * 2 * kKvBlock))
+        return fail(c, ZYNFER_CU_INTERNAL, "cuTensorMapEncodeTiled failed for the KV pool");
+    cudaMemset(c->kv, 0, c->kv_layer_elems * m.layers * 2);  // unused rows of a block are read (and weigh nothing)
+    c->serve_mark.assign(c->n_blocks, -1);
     if (!make_tmap_k_major(&c->tm_embed, c->embed, c->wkind, H, V, 128))
         return fail(c, ZYNFER_CU_INTERNAL, "cuTensorMapEncodeTiled failed for the embedding");
     // persistent dataflow decode kernel: weight pointers per layer, its sync
@@ -1451,13 +1621,14 @@ int zynfer_cu_attn_window(ZynferCuCtx* c, uint32_t layer, const uint32_t* seqs, 
     if (!seqs || !q || !out) return fail(c, ZYNFER_CU_INVALID, "null argument");
     int rc = check_serve_tensors(c, layer, q, q_stride, out, out_stride, dtype);
     if (rc) return rc;
-    ServeRows rows;
-    if ((rc = serve_rows(c, seqs, batch, tokens, 0, &rows))) return rc;
+    if ((rc = serve_batch(c, seqs, batch, tokens, 0))) return rc;
     if (take_launch_fault(c)) return ZYNFER_CU_LAUNCH;
     cudaSetDevice(c->device);
     if ((rc = settle_tables(c, seqs, batch))) return rc;
-    launch_serve_attn(rows, serve_args(c, layer, batch, tokens, window, sinks, q, q_stride, out, out_stride,
-                                       dtype == ZYNFER_CU_DT_BF16), c->stream);
+    const bool bf16 = dtype == ZYNFER_CU_DT_BF16;
+    ServePlan plan;
+    if ((rc = plan_serve(c, batch, tokens, window, sinks, false, bf16, &plan))) return rc;
+    enqueue_serve(c, plan, serve_args(c, layer, batch, tokens, window, sinks, q, q_stride, out, out_stride, bf16));
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_fail(c, e, "attention launch");
     set_path(c, "attn_window", 0, nullptr);
@@ -1470,14 +1641,15 @@ int zynfer_cu_attn_shared(ZynferCuCtx* c, uint32_t layer, const uint32_t* seqs, 
     if (!seqs || !q || !out) return fail(c, ZYNFER_CU_INVALID, "null argument");
     int rc = check_serve_tensors(c, layer, q, q_stride, out, out_stride, dtype);
     if (rc) return rc;
-    ServeRows rows;
-    if ((rc = serve_rows(c, seqs, batch, 1, 0, &rows))) return rc;
+    if ((rc = serve_batch(c, seqs, batch, 1, 0))) return rc;
     if ((rc = validate_batch(c, seqs, batch, 0))) return rc;
     if (take_launch_fault(c)) return ZYNFER_CU_LAUNCH;
     cudaSetDevice(c->device);
     if ((rc = settle_tables(c, seqs, batch))) return rc;
-    launch_serve_attn(rows, serve_args(c, layer, batch, 1, ZYNFER_CU_WINDOW_ALL, 0, q, q_stride, out, out_stride,
-                                       dtype == ZYNFER_CU_DT_BF16), c->stream);
+    const bool bf16 = dtype == ZYNFER_CU_DT_BF16;
+    ServePlan plan;
+    if ((rc = plan_serve(c, batch, 1, ZYNFER_CU_WINDOW_ALL, 0, true, bf16, &plan))) return rc;
+    enqueue_serve(c, plan, serve_args(c, layer, batch, 1, ZYNFER_CU_WINDOW_ALL, 0, q, q_stride, out, out_stride, bf16));
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_fail(c, e, "attention launch");
     set_path(c, "attn_shared", 0, nullptr);
@@ -1545,8 +1717,9 @@ int zynfer_cu_prefill_chunk(ZynferCuCtx* c, uint32_t seq, const uint32_t* tokens
     int rc = ensure_blocks(c, seq, pos0 + n);
     if (rc) return rc;
     if ((rc = settle_tables(c, &seq, 1))) return rc;
-    ServeRows rows;
-    if ((rc = serve_rows(c, &seq, 1, n, n, &rows))) return rc;
+    if ((rc = serve_batch(c, &seq, 1, n, n))) return rc;
+    ServePlan plan;
+    if ((rc = plan_serve(c, 1, n, window, sinks, false, false, &plan))) return rc;
     const ZynferCuModelDesc& m = c->d;
     const int H = m.hidden, T = (int)n;
     ZC_CHECK(c, cudaMemcpyAsync(c->ptok, tokens, (size_t)n * 4, cudaMemcpyHostToDevice, c->stream), "prompt upload");
@@ -1566,7 +1739,7 @@ int zynfer_cu_prefill_chunk(ZynferCuCtx* c, uint32_t seq, const uint32_t* tokens
         qa.max_blocks = c->max_blocks; qa.n_pool_blocks = c->n_blocks;
         qa.q_out = c->pq; qa.err = c->derr;
         launch_qkv_post(qa, c->stream);
-        launch_serve_attn(rows, serve_args(c, l, 1, n, window, sinks, c->pq, c->qd, c->pattn, c->qd, false), c->stream);
+        enqueue_serve(c, plan, serve_args(c, l, 1, n, window, sinks, c->pq, c->qd, c->pattn, c->qd, false));
         linear(c, ZYNFER_CU_K_LINEAR, Ld.wo, Ld.so, &Ld.tm_o, H, c->qd, c->pattn, T, c->px1, kEpiResid, c->px, nullptr,
                nullptr);
         linear(c, ZYNFER_CU_K_LINEAR, Ld.wgu, Ld.sgu, &Ld.tm_gu, 2 * (int)m.inter, H, c->px1, T, c->ph, kEpiSwiGLU,
@@ -1611,8 +1784,9 @@ int zynfer_cu_decode_drawn(ZynferCuCtx* c, const uint32_t* seqs, const uint32_t*
     for (uint32_t i = 0; i < batch; ++i)
         if ((rc = ensure_blocks(c, seqs[i], c->seq_len[seqs[i]] + 1))) return rc;
     if ((rc = settle_tables(c, seqs, batch))) return rc;
-    ServeRows rows;
-    if ((rc = serve_rows(c, seqs, batch, 1, 1, &rows))) return rc;
+    if ((rc = serve_batch(c, seqs, batch, 1, 1))) return rc;
+    ServePlan plan;
+    if ((rc = plan_serve(c, batch, 1, window, sinks, window == ZYNFER_CU_WINDOW_ALL, false, &plan))) return rc;
     set_io_views(c, (int)batch);
     if ((rc = stage_batch(c, seqs, tokens, batch))) return rc;
     const ZynferCuDrawRule none{};
@@ -1647,7 +1821,7 @@ int zynfer_cu_decode_drawn(ZynferCuCtx* c, const uint32_t* seqs, const uint32_t*
         qa.max_blocks = c->max_blocks; qa.n_pool_blocks = c->n_blocks;
         qa.q_out = c->dq; qa.err = c->derr;
         launch_qkv_post(qa, c->stream);
-        launch_serve_attn(rows, serve_args(c, l, batch, 1, window, sinks, c->dq, c->qd, c->dattn, c->qd, false), c->stream);
+        enqueue_serve(c, plan, serve_args(c, l, batch, 1, window, sinks, c->dq, c->qd, c->dattn, c->qd, false));
         c->step_launches += 2;
         set_prefetch(c, Ld.wgu, Ld.sgu, 2 * I, H);
         linear(c, ZYNFER_CU_K_LINEAR, Ld.wo, Ld.so, &Ld.tm_o, H, c->qd, c->dattn, N, c->dx1, kEpiResid, c->dx, nullptr,

@@ -54,6 +54,7 @@ void prepare_all_kernels() {
     prepare_fewrow_kernels();
     prepare_draw_kernels();
     prepare_serve_attn_kernels();
+    prepare_attn_tile_kernels();
 }
 
 int device_sm_count() {

@@ -49,6 +49,13 @@ struct TcLaunch {
 int tc_tile_tokens(int wkind, int M, int T);  // NT: tokens per N tile of an M x K by T linear
 bool make_tmap_k_major(CUtensorMap* map, const void* base, int wkind, uint64_t k_elems, uint64_t rows,
                        uint32_t box_rows);
+// The KV pool as rows of 128 bf16, boxes of 16 rows x half a row, not swizzled
+// (the pool's own swizzle is the MMA's).
+bool make_tmap_kv(CUtensorMap* map, const void* pool, uint64_t rows);
+// attn_tile.cu: `items` = CTAs; cache blocks of a tile of keys
+inline int attn_tile_blocks(bool bf16) { return bf16 ? 8 : 4; }
+void launch_attn_tile(const CUtensorMap& kv_map, const ServeRows& rows, const TileList& list, const ServeAttnArgs& a,
+                      int items, cudaStream_t st);
 void launch_prep_planes(const PlanesArgs& a, cudaStream_t st);
 void launch_tc_gemm(const TcLaunch& L, cudaStream_t st);
 // Cluster split-K variant for problems with too few (M, N) tiles to fill the
