@@ -190,10 +190,19 @@ struct ServeAttnArgs {
     int nsplit;                // chunk: CTAs that share a tile's blocks
     float* part;               // [row][n_q][max_segs][kServeRecord]
     int max_segs;
+    unsigned* counters;        // [row][n_kv], zero between launches
+    int min_per;               // span kernel: blocks a warp takes at least
+    int early;                 // span kernel: launched behind a tile kernel
     uint32_t* err;
 };
 void prepare_attn_tile_kernels();
-void launch_serve_simple(const ServeRows& rows, const ServeAttnArgs& a, cudaStream_t st);
+void prepare_attn_span_kernels();
+// attn_span.cu: single tokens. A (row, kv head) meets at most
+// blocks / (kSpanWarps min_per) + 2 CTAs.
+constexpr int kSpanWarps = 8;
+void launch_attn_span(const ServeRows& rows, const ServeAttnArgs& a, int ctas, cudaStream_t st);
+// Cache blocks that a query at `pos` sees after the first `skip`.
+int serve_span_blocks(int pos, uint32_t window, int sinks, int skip);
 void launch_serve_merge(const ServeRows& rows, const ServeAttnArgs& a, cudaStream_t st);
 struct KvWriteArgs {
     uint16_t* kv_layer;

@@ -16,25 +16,6 @@ namespace {
 
 using namespace serve;
 
-// One warp per (query row, query head) over the blocks after the row's common
-// ones, position by position.
-__global__ void __launch_bounds__(128) serve_attn_simple_kernel(const __grid_constant__ ServeRows rows,
-                                                               const __grid_constant__ ServeAttnArgs a) {
-    pdl_wait();
-    pdl_launch_dependents();
-    const int n_q = a.n_kv * kG;
-    const long long w = ((long long)blockIdx.x * blockDim.x + threadIdx.x) / kWarp;
-    if (w >= (long long)a.batch * a.tokens * n_q) return;
-    const int hq = (int)(w % n_q);
-    const int qi = (int)(w / n_q);
-    const int b = qi / a.tokens, pos = rows.len[b] - a.tokens + qi % a.tokens;
-    const Span span = span_of(pos, pos, a.window, a.sinks, rows.skip[b]);
-    const int qrow = a.tokens == 1 ? rows.row[b] : qi;
-    const SlowRow r = slow_row(a, qrow, hq, rows.slot[b], pos, window_low(pos, a.window), a.sinks, span, 0, span.total);
-    if (rows.nrec[b] == 0) store_row(a, qrow, hq, r);
-    else store_record(a.part + (((size_t)b * n_q + hq) * a.max_segs + rows.nrec[b]) * kRecord, r);
-}
-
 // The records of a (row, query head) joined: o = sum acc 2^(m - M) / sum l 2^(m - M).
 // A warp per (row, query head); rows with one partial result wrote the output.
 __global__ void __launch_bounds__(128) serve_merge_kernel(const __grid_constant__ ServeRows rows,
@@ -108,10 +89,7 @@ __global__ void __launch_bounds__(256) kv_write_kernel(KvWriteArgs a) {
 
 }  // namespace
 
-void launch_serve_simple(const ServeRows& rows, const ServeAttnArgs& a, cudaStream_t st) {
-    const long long warps = (long long)a.batch * a.tokens * a.n_kv * kG;
-    launch_pdl(serve_attn_simple_kernel, (unsigned)((warps + 3) / 4), 128, 0, st, rows, a);
-}
+int serve_span_blocks(int pos, uint32_t window, int sinks, int skip) { return span_of(pos, pos, window, sinks, skip).total; }
 
 void launch_serve_merge(const ServeRows& rows, const ServeAttnArgs& a, cudaStream_t st) {
     const long long warps = (long long)a.batch * a.tokens * a.n_kv * kG;
@@ -125,7 +103,6 @@ void launch_kv_write(const KvWriteArgs& a, cudaStream_t st) {
 }
 
 void prepare_serve_attn_kernels() {
-    configure_kernel((const void*)serve_attn_simple_kernel, 0);
     configure_kernel((const void*)serve_merge_kernel, 0);
     configure_kernel((const void*)kv_write_kernel, 0);
 }

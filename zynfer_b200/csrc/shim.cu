@@ -897,37 +897,55 @@ int serve_scratch(ZynferCuCtx* c, size_t words) {
     return rc;
 }
 
-// The launches of a planned call (items from plan_shared; tokens > 1 or a
-// window: a chunk, whose plan is made here).
+// The launches of a planned call.
 struct ServePlan {
-    bool chunk = false;
-    int items = 0, nsplit = 1, max_segs = 1;
+    bool chunk = false;  // more than one query per sequence: tiles alone
+    int items = 0;       // CTAs of the tile kernel
+    int nsplit = 1;      // chunk: CTAs that share a tile's blocks
+    int ctas = 0;        // of the span kernel
+    int min_per = 1, max_segs = 1;
 };
 
 int plan_serve(ZynferCuCtx* c, uint32_t batch, uint32_t tokens, uint32_t window, uint32_t sinks, bool shared, bool bf16,
                ServePlan* p) {
     *p = ServePlan{};
-    if (shared) {
-        p->items = plan_shared(c, batch, bf16, &p->max_segs);
-    } else if (tokens > 1) {
+    const ServeRows& rows = c->serve_rows;
+    const int sms = c->caps.sm_count > 0 ? c->caps.sm_count : 148;
+    if (tokens > 1) {
         p->chunk = true;
         c->serve_tiles.n = 0;
-        const long long tiles = (long long)batch * ((tokens + 63) / 64) * c->d.n_kv;
-        p->items = (int)tiles;
+        p->items = (int)((long long)batch * ((tokens + 63) / 64) * c->d.n_kv);
+        return ZYNFER_CU_OK;
     }
-    if (p->max_segs > 1) return serve_scratch(c, (size_t)batch * tokens * c->d.n_q * p->max_segs * kServeRecord);
-    (void)window; (void)sinks;
-    return ZYNFER_CU_OK;
+    c->serve_tiles.n = 0;
+    int tile_segs = 1;
+    if (shared) p->items = plan_shared(c, batch, bf16, &tile_segs);
+    // the span kernel's list of blocks, at least min_per to a warp
+    long long blocks = 0;
+    int longest = 1;
+    for (uint32_t i = 0; i < batch; ++i) {
+        const int pos = rows.len[i] - 1;
+        const int n = std::max(1, serve_span_blocks(pos, window, (int)std::min<uint32_t>(sinks, c->d.max_seq_len), rows.skip[i]));
+        blocks += n;
+        longest = std::max(longest, n);
+    }
+    const long long total = blocks * c->d.n_kv, share = (long long)kSpanWarps * p->min_per;
+    p->ctas = (int)std::min<long long>(sms, (total + share - 1) / share);
+    const long long per = std::max<long long>(p->min_per, (total + (long long)p->ctas * kSpanWarps - 1) / ((long long)p->ctas * kSpanWarps));
+    p->max_segs = tile_segs + (int)((longest - 1) / (per * kSpanWarps) + 2);
+    return serve_scratch(c, (size_t)batch * c->d.n_q * p->max_segs * kServeRecord);
 }
 
 void enqueue_serve(ZynferCuCtx* c, const ServePlan& p, ServeAttnArgs a) {
     a.nsplit = p.nsplit;
     a.max_segs = p.max_segs;
     a.part = c->serve_part;
+    a.counters = c->dcnt;
+    a.min_per = p.min_per;
+    a.early = p.items > 0 ? 1 : 0;
     if (p.items) launch_attn_tile(c->tm_kv, c->serve_rows, c->serve_tiles, a, p.items, c->stream);
-    if (p.chunk && p.nsplit == 1) return;
-    if (!p.chunk) launch_serve_simple(c->serve_rows, a, c->stream);
-    if (p.max_segs > 1) launch_serve_merge(c->serve_rows, a, c->stream);
+    if (!p.chunk) launch_attn_span(c->serve_rows, a, p.ctas, c->stream);
+    else if (p.nsplit > 1) launch_serve_merge(c->serve_rows, a, c->stream);
 }
 
 // Changed block-table rows to the device; the pinned copy may be rewritten by

@@ -55,6 +55,7 @@ void prepare_all_kernels() {
     prepare_draw_kernels();
     prepare_serve_attn_kernels();
     prepare_attn_tile_kernels();
+    prepare_attn_span_kernels();
 }
 
 int device_sm_count() {
