@@ -17,20 +17,22 @@
 // weight of 2^-34 of the largest apart from 0 and the sum of 2^18 of them
 // below 2^53, so products with top_p and u are single f64 roundings.
 //
-// One pass over HBM: a cluster of C CTAs holds a row's logits in registers (E
-// per thread, as order keys) and selects by sums.
-//   1. the largest and smallest key of the row (one exchange over distributed
-//      shared memory; top_k = 1 is done here);
-//   2. every CTA adds its tokens' weights and counts into NB bins even in
-//      (m - l) / T, between 0 and where weights end; the CTAs then take a slice
-//      of the bins each, add up the C copies and scan them;
+// One pass over HBM: a cluster of C CTAs holds a row in shared memory and
+// selects by sums.
+//   1. the largest and smallest logit of the row (one exchange over distributed
+//      shared memory);
+//   2. every CTA adds its tokens' weights (and counts) into NB bins even in
+//      (m - l) / T, from 0 to where weights end; the CTAs then take a slice of
+//      the bins each, add up the C copies and scan them;
 //   3. a question (the top_k-th token, the token where top_p is reached, the
 //      drawn one) is answered by the bin that holds it, then by the tokens of
-//      that bin alone, which all CTAs collect in a list and rank by counting.
-//      A bin that holds more than the list (many equal logits) is divided
-//      again, by (logit, index) itself, until it fits.
-// What bounds it is the chain of exchanges and barriers, about ten of them,
-// not the bytes; so a row is spread over 8 SMs and rows run side by side.
+//      that bin, which all CTAs send to the first, where they are sorted and
+//      their weights scanned. A bin of more tokens than that list holds (many
+//      equal logits) is divided again, by (logit, index) itself, until it fits.
+// A few rows are bound by the chain of exchanges and barriers, many rows by
+// the instructions per logit (about 60, an accurate exponential among them),
+// not by the bytes: so weights are split into two 32-bit words without integer
+// conversions, and two CTAs share an SM so that one works while the other waits.
 #include <type_traits>
 
 #include "common.cuh"
@@ -40,38 +42,59 @@ namespace zc {
 
 namespace {
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / kWarp;
-constexpr int kList = 512;        // tokens of a bin that are ranked by counting
+constexpr int kList = kThreads;        // tokens of a bin that are sorted
 constexpr float kOne = 8589934592.0f;  // 2^33, the weight of the largest logit
-constexpr float kEnd = 23.6f;     // exp(-kEnd) 2^33 < 1/2: weights beyond are 0
-constexpr int kIndexBits = 18;    // vocab <= 2^18
+constexpr float kEnd = 23.6f;          // exp(-kEnd) 2^33 < 1/2: weights beyond are 0
+constexpr int kIndexBits = 18;         // vocab <= 2^18
+constexpr float kMagic = 8388608.0f;   // 2^23: x + 2^23 holds rint(x) in its low bits
 constexpr unsigned kAll = 0xFFFFFFFFu;
 using u64 = unsigned long long;
 static_assert(kDrawMaxVocab == 1 << kIndexBits, "composite keys");
 
-// Larger key = earlier in the order, equal logits (-0 and 0 among them) alike;
-// 0 for NaN and -inf.
-__device__ __forceinline__ uint32_t order_key(float l) { return (uint32_t)(argmax_key(l + 0.0f, 0u) >> 32); }
-__device__ __forceinline__ float key_logit(uint32_t k) {
+// The place of a token in the order as one number: larger = earlier.
+__device__ __forceinline__ u64 composite(float l, int idx) {
+    return ((argmax_key(l, 0u) >> 32) << kIndexBits) | (u64)((1 << kIndexBits) - 1 - idx);
+}
+__device__ __forceinline__ float composite_logit(u64 c) {
+    const uint32_t k = (uint32_t)(c >> kIndexBits);
     return __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k);
 }
-__device__ __forceinline__ float load_logit(const DrawArgs& a, size_t i) {
-    return a.bf16 ? bf16lo(__ldg(static_cast<const uint16_t*>(a.logits) + i)) : __ldg(static_cast<const float*>(a.logits) + i);
-}
-// The place of a token in the order as one number: larger = earlier.
-__device__ __forceinline__ u64 composite(uint32_t key, int idx) {
-    return ((u64)key << kIndexBits) | (u64)((1 << kIndexBits) - 1 - idx);
-}
+
+// rint(e 2^33) = hi 2^17 + lo, lo in [-2^16, 2^16): both parts by adding 2^23
+// (1.5 2^23 for the signed one). e 2^16 and the remainder are exact, and hi 2^17
+// is even, so rounding the remainder alone rounds the whole the same way. The
+// sums of 2^15 such words fit 32 bits.
+struct Weight {
+    uint32_t hi;
+    int lo;
+    __device__ __forceinline__ bool any() const { return (hi | (uint32_t)lo) != 0u; }
+    __device__ __forceinline__ u64 whole() const { return ((u64)hi << 17) + (u64)(long long)lo; }
+};
 
 struct RowRule {
-    float m, inv_t, min_p;
+    float m, inv_t, min_p, end, bin_scale;
     __device__ __forceinline__ float exponent(float l) const { return l == m ? 0.0f : (l - m) * inv_t; }
-    __device__ __forceinline__ u64 weight_at(float x) const {
-        const float e = expf(x);
-        return e >= min_p ? (u64)__float2ll_rn(e * kOne) : 0ull;
+    __device__ __forceinline__ int bin(float x) const {
+        return __float_as_int(__fmaf_rn(fminf(-x, end), bin_scale, kMagic)) - 0x4B000000;
     }
-    __device__ __forceinline__ u64 weight(uint32_t key) const { return key ? weight_at(exponent(key_logit(key))) : 0ull; }
+    // (a logit of -inf has exponent -inf, or NaN where 1 / T is 0: no weight)
+    __device__ __forceinline__ Weight weight(float l, float x) const {
+        const float e = expf(x);
+        Weight w{0u, 0};
+        if (e >= min_p && l != -INFINITY) {
+            const float s = e * 65536.0f, t = s + kMagic;
+            const float rem = (s - (t - kMagic)) * 131072.0f;
+            w.hi = (uint32_t)(__float_as_int(t) - 0x4B000000);
+            w.lo = __float_as_int(rem + 12582912.0f) - 0x4B400000;
+            if (w.lo == 65536) {
+                w.lo = -65536;
+                w.hi += 1u;
+            }
+        }
+        return w;
+    }
 };
 
 // What CTAs of a cluster tell one another.
@@ -82,15 +105,22 @@ struct Note {
 
 template <int C>
 struct Shared {
-    static constexpr int NB = C == 1 ? 1024 : 4096;  // bins
-    uint32_t count[NB], lo[NB], hi[NB];              // tokens, and their weights' low 17 and remaining bits
-    u64 list_c[kList], list_w[kList];
+    static constexpr int NB = C == 1 ? 512 : 2048;  // bins
+    static constexpr int NB_LOG = C == 1 ? 9 : 11;
+    uint32_t count[NB], hi[NB];  // tokens, and their weights' parts
+    int lo[NB];
+    u64 list[kList];
     Note note[2][C];
-    uint32_t list_n;                                  // of rank 0
-    u64 scan_m[kWarps];
-    uint32_t scan_c[kWarps], red_a[kWarps], red_b[kWarps], red_i[kWarps];
-    u64 res[2];
+    uint32_t list_n;  // of rank 0
+    u64 scan_m[kWarps], scan_x[kWarps], res[3];
+    uint32_t scan_c[kWarps];
+    float red_a[kWarps], red_b[kWarps];
+    alignas(16) float row[1];  // this CTA's logits
 };
+template <int C>
+constexpr size_t smem_bytes(int chunk) {
+    return sizeof(Shared<C>) + (size_t)chunk * sizeof(float);
+}
 
 __device__ __forceinline__ uint32_t at_rank(const void* p, uint32_t rank) {
     uint32_t r;
@@ -110,9 +140,17 @@ __device__ __forceinline__ uint32_t add_rank(uint32_t addr, uint32_t v) {
     asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(old) : "r"(addr), "r"(v) : "memory");
     return old;
 }
+__device__ __forceinline__ u64 warp_scan(u64 v) {
+#pragma unroll
+    for (int o = 1; o < kWarp; o <<= 1) {
+        const u64 x = __shfl_up_sync(kAll, v, o);
+        if ((int)(threadIdx.x % kWarp) >= o) v += x;
+    }
+    return v;
+}
 
-template <int C, int E>
-__global__ void __launch_bounds__(kThreads, 1) draw_kernel(const __grid_constant__ DrawArgs a) {
+template <int C>
+__global__ void __launch_bounds__(kThreads, 2) draw_kernel(const __grid_constant__ DrawArgs a) {
     using Sh = Shared<C>;
     constexpr int NB = Sh::NB, SLICE = NB / C;
     static_assert(SLICE <= kThreads, "a thread per bin of a slice");
@@ -130,7 +168,9 @@ __global__ void __launch_bounds__(kThreads, 1) draw_kernel(const __grid_constant
             asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
         }
     };
-    // every CTA's note (thread 0's) to every CTA; returns the slots
+    // every CTA's note (thread 0's) to every CTA; returns the slots. Two sets of
+    // slots in turn: a set is written again only after everyone passed the
+    // barrier behind its reading.
     auto exchange = [&](const Note& n) -> const Note* {
         Note* slots = sh.note[parity];
         parity ^= 1;
@@ -149,8 +189,20 @@ __global__ void __launch_bounds__(kThreads, 1) draw_kernel(const __grid_constant
         barrier();
         return slots;
     };
+    auto clear_bins = [&]() {
+        for (int i = tid; i < NB; i += kThreads) {
+            sh.count[i] = sh.hi[i] = 0u;
+            sh.lo[i] = 0;
+        }
+    };
 
-    for (int i = tid; i < NB; i += kThreads) sh.count[i] = sh.lo[i] = sh.hi[i] = 0u;
+    // no CTA writes into another before that one runs: this barrier's other half
+    // is in front of the first exchange
+    if constexpr (C > 1) {
+        __syncwarp();
+        asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    }
+    clear_bins();
     if (tid == 0) sh.list_n = 0u;
     pdl_wait();
     pdl_launch_dependents();
@@ -164,91 +216,126 @@ __global__ void __launch_bounds__(kThreads, 1) draw_kernel(const __grid_constant
     float u = a.uniforms[r];
     u = u > 0.0f ? fminf(u, 1.0f) : 0.0f;
 
-    // ---- the row: CTA `rank` holds [i0, i1), thread t the tokens i0 + 1024 e + t
-    const int chunk = (a.vocab + C - 1) / C;
-    const int i0 = rank * chunk + tid, i1 = min(a.vocab, (rank + 1) * chunk);
-    uint32_t key[E];
-    {
-        const size_t base = (size_t)r * a.stride;
-        float l[E];
-#pragma unroll
-        for (int e = 0; e < E; ++e) l[e] = i0 + e * kThreads < i1 ? load_logit(a, base + i0 + e * kThreads) : -INFINITY;
-#pragma unroll
-        for (int e = 0; e < E; ++e) key[e] = order_key(l[e]);
-    }
-    uint32_t top = 0u, least = 0xFFFFFFFFu, first = 0u;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        if (key[e] > top) {
-            top = key[e];
-            first = (uint32_t)(i0 + e * kThreads);
-        }
-        if (key[e]) least = min(least, key[e]);
-    }
-    auto warp_best = [&](uint32_t& t, uint32_t& f, uint32_t& m) {  // largest t with its least f, least m
-        const uint32_t w = __reduce_max_sync(kAll, t);
-        f = __reduce_min_sync(kAll, t == w ? f : 0xFFFFFFFFu);
-        t = w;
-        m = __reduce_min_sync(kAll, m);
+    // ---- the row: this CTA holds tokens i0 .. i0 + n - 1 (chunk is even)
+    const int i0 = min(a.vocab, rank * a.chunk), n = min(a.vocab, i0 + a.chunk) - i0;
+    float top = -INFINITY, least = INFINITY;
+    auto take = [&](float l, int i) {
+        l = fmaxf(l + 0.0f, -INFINITY);  // NaN becomes -inf, -0 becomes 0
+        sh.row[i] = l;
+        top = fmaxf(top, l);
+        least = fminf(least, l == -INFINITY ? INFINITY : l);
     };
-    warp_best(top, first, least);
+    const size_t base = (size_t)r * a.stride + i0;
+    if (a.bf16) {
+        const uint16_t* src = static_cast<const uint16_t*>(a.logits) + base;
+        if (reinterpret_cast<uintptr_t>(src) % 4 == 0) {
+            const uint32_t* two = reinterpret_cast<const uint32_t*>(src);
+            constexpr int kAhead = 8;
+            for (int j = tid; j < n / 2; j += kAhead * kThreads) {
+                uint32_t x[kAhead];
+#pragma unroll
+                for (int v = 0; v < kAhead; ++v) x[v] = j + v * kThreads < n / 2 ? __ldg(two + j + v * kThreads) : 0u;
+#pragma unroll
+                for (int v = 0; v < kAhead; ++v)
+                    if (j + v * kThreads < n / 2) {
+                        take(bf16lo(x[v]), 2 * (j + v * kThreads));
+                        take(bf16hi(x[v]), 2 * (j + v * kThreads) + 1);
+                    }
+            }
+            if ((n & 1) && tid == 0) take(bf16lo(__ldg(src + n - 1)), n - 1);
+        } else {
+            for (int i = tid; i < n; i += kThreads) take(bf16lo(__ldg(src + i)), i);
+        }
+    } else {
+        const float* src = static_cast<const float*>(a.logits) + base;
+        constexpr int kAhead = 16;
+        for (int j = tid; j < n; j += kAhead * kThreads) {
+            float x[kAhead];
+#pragma unroll
+            for (int v = 0; v < kAhead; ++v) x[v] = j + v * kThreads < n ? __ldg(src + j + v * kThreads) : 0.0f;
+#pragma unroll
+            for (int v = 0; v < kAhead; ++v)
+                if (j + v * kThreads < n) take(x[v], j + v * kThreads);
+        }
+    }
+    auto warp_range = [&]() {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            top = fmaxf(top, __shfl_xor_sync(kAll, top, o));
+            least = fminf(least, __shfl_xor_sync(kAll, least, o));
+        }
+    };
+    warp_range();
     if (lane == 0) {
         sh.red_a[warp] = top;
-        sh.red_i[warp] = first;
         sh.red_b[warp] = least;
     }
     __syncthreads();
-    top = sh.red_a[lane];
-    first = sh.red_i[lane];
-    least = sh.red_b[lane];
-    warp_best(top, first, least);
+    top = sh.red_a[lane % kWarps];
+    least = sh.red_b[lane % kWarps];
+    warp_range();
+    if constexpr (C > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     {
-        const Note* n = exchange(Note{top, first, least, 0u});
-        const Note x = n[C == 1 ? 0 : lane % C];
-        top = (uint32_t)x.a;
-        first = (uint32_t)x.b;
-        least = x.c;
-        warp_best(top, first, least);
+        const Note* x = exchange(Note{0ull, 0ull, __float_as_uint(top), __float_as_uint(least)});
+        top = __uint_as_float(x[lane % C].c);
+        least = __uint_as_float(x[lane % C].d);
+        warp_range();
     }
-    if (top == 0u || k == 1) {  // nothing but NaN and -inf; or the largest alone
+    if (top == -INFINITY) {  // nothing but NaN and -inf
         if (rank == 0 && tid == 0) {
-            a.ids[r] = top ? first : 0u;
-            if (a.logprobs) a.logprobs[r] = top ? 0.0f : -INFINITY;
+            a.ids[r] = 0u;
+            if (a.logprobs) a.logprobs[r] = -INFINITY;
         }
         return;
     }
-    const RowRule rule{key_logit(top), greedy ? 1.0f : 1.0f / T, min_p};
+    if (k == 1) {  // the first of the largest
+        uint32_t first = 0xFFFFFFFFu;
+        for (int i = tid; i < n; i += kThreads)
+            if (sh.row[i] == top) first = min(first, (uint32_t)(i0 + i));
+        first = __reduce_min_sync(kAll, first);
+        if (lane == 0) sh.scan_c[warp] = first;
+        __syncthreads();
+        first = __reduce_min_sync(kAll, sh.scan_c[lane % kWarps]);
+        const Note* x = exchange(Note{0ull, 0ull, first, 0u});
+        first = __reduce_min_sync(kAll, x[lane % C].c);
+        if (rank == 0 && tid == 0) {
+            a.ids[r] = first;
+            if (a.logprobs) a.logprobs[r] = 0.0f;
+        }
+        return;
+    }
 
     // ---- bins even in (m - l) / T, up to the last weight
-    float end = fminf(-rule.exponent(key_logit(least)), kEnd);
-    if (!(end >= 0.0f)) end = kEnd;
-    if (min_p > 0.0f) end = fminf(end, 0.01f - logf(min_p));
-    const float bin_scale = end > 0.0f ? (float)(NB - 1) / end : 0.0f;
-    auto bin_at = [&](float x) { return min((int)(-x * bin_scale), NB - 1); };
+    RowRule rule{top, 1.0f / T, min_p, 0.0f, 0.0f};
+    rule.end = fminf(-rule.exponent(least), kEnd);
+    if (!(rule.end >= 0.0f)) rule.end = kEnd;
+    if (min_p > 0.0f) rule.end = fminf(rule.end, 0.01f - logf(min_p));
+    rule.bin_scale = rule.end > 0.0f ? (float)(NB - 1) / rule.end : 0.0f;
+    const bool counts = k > 0;
 
     // Adds this CTA's tokens into the bins (bin0 >= 0: those of that bin between
     // c_hi and c_lo, into bins of 2^shift places) and scans the sums: thread
     // t < SLICE has bin rank SLICE + t.
-    u64 mass_ex, mass, all_mass;
+    u64 mass_ex, mass, all_mass, c_hi = ~0ull, c_lo = 0ull;
     uint32_t count_ex, count, all_count;
-    u64 c_hi = ~0ull, c_lo = 0ull;
     int bin0 = -1, shift = 0;
     auto histogram = [&]() {
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            if (!key[e]) continue;
-            const float x = rule.exponent(key_logit(key[e]));
-            int b = bin_at(x);
+        const bool counted = counts || bin0 >= 0;
+#pragma unroll 4
+        for (int i = tid; i < n; i += kThreads) {
+            const float l = sh.row[i], x = rule.exponent(l);
+            int b = rule.bin(x);
             if (bin0 >= 0) {
-                const u64 c = composite(key[e], i0 + e * kThreads);
-                if (b != bin0 || c < c_lo || c > c_hi) continue;
+                if (b != bin0) continue;
+                const u64 c = composite(l, i0 + i);
+                if (c < c_lo || c > c_hi) continue;
                 b = (int)((c_hi - c) >> shift);
             }
-            const u64 w = rule.weight_at(x);
-            if (w) {
-                atomicAdd(&sh.count[b], 1u);
-                atomicAdd(&sh.lo[b], (uint32_t)w & 0x1FFFFu);
-                atomicAdd(&sh.hi[b], (uint32_t)(w >> 17));
+            const Weight w = rule.weight(l, x);
+            if (w.any()) {
+                atomicAdd(&sh.hi[b], w.hi);
+                atomicAdd(&sh.lo[b], w.lo);
+                if (counted) atomicAdd(&sh.count[b], 1u);
             }
         }
         barrier();
@@ -256,95 +343,59 @@ __global__ void __launch_bounds__(kThreads, 1) draw_kernel(const __grid_constant
         count = 0u;
         if (tid < SLICE) {
             const int b = rank * SLICE + tid;
-            if constexpr (C == 1) {
-                count = sh.count[b];
-                mass = ((u64)sh.hi[b] << 17) + sh.lo[b];
-            } else {
-                uint32_t x[C], y[C], z[C];
+            uint32_t x[C], y[C], z[C];
 #pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    const uint32_t at = at_rank(&sh.count[b], c);
-                    x[c] = ld_rank(at);
-                    y[c] = ld_rank(at + NB * 4);
-                    z[c] = ld_rank(at + 2 * NB * 4);
-                }
+            for (int c = 0; c < C; ++c) {
+                const uint32_t at = at_rank(&sh.count[b], c);
+                x[c] = ld_rank(at);
+                y[c] = ld_rank(at + NB * 4);
+                z[c] = ld_rank(at + 2 * NB * 4);
+            }
 #pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    count += x[c];
-                    mass += ((u64)z[c] << 17) + y[c];
-                }
+            for (int c = 0; c < C; ++c) {
+                count += x[c];
+                mass += ((u64)y[c] << 17) + (u64)(long long)(int)z[c];
             }
         }
-        // scan over the CTA's slice
-        u64 m = mass;
-        uint32_t n = count;
-#pragma unroll
-        for (int o = 1; o < kWarp; o <<= 1) {
-            const u64 mm = __shfl_up_sync(kAll, m, o);
-            const uint32_t nn = __shfl_up_sync(kAll, n, o);
-            if (lane >= o) {
-                m += mm;
-                n += nn;
-            }
-        }
+        const u64 m = warp_scan(mass), nn = warp_scan(count);
         if (lane == kWarp - 1) {
             sh.scan_m[warp] = m;
-            sh.scan_c[warp] = n;
+            sh.scan_c[warp] = (uint32_t)nn;
         }
         __syncthreads();
-        u64 before_m = 0ull, cta_m = 0ull;
-        uint32_t before_n = 0u, cta_n = 0u;
-        {
-            u64 x = sh.scan_m[lane];
-            uint32_t y = sh.scan_c[lane];
-            const u64 x0 = x;
-            const uint32_t y0 = y;
-#pragma unroll
-            for (int o = 1; o < kWarp; o <<= 1) {
-                const u64 mm = __shfl_up_sync(kAll, x, o);
-                const uint32_t nn = __shfl_up_sync(kAll, y, o);
-                if (lane >= o) {
-                    x += mm;
-                    y += nn;
-                }
-            }
-            before_m = __shfl_sync(kAll, x - x0, warp);
-            before_n = __shfl_sync(kAll, y - y0, warp);
-            cta_m = __shfl_sync(kAll, x, kWarp - 1);
-            cta_n = __shfl_sync(kAll, y, kWarp - 1);
-        }
-        const Note* t = exchange(Note{cta_m, cta_n, 0u, 0u});  // (all bins are read)
+        const u64 x0 = lane < kWarps ? sh.scan_m[lane] : 0ull, y0 = lane < kWarps ? sh.scan_c[lane] : 0u;
+        const u64 x = warp_scan(x0), y = warp_scan(y0);
+        u64 before_m = __shfl_sync(kAll, x - x0, warp), before_n = __shfl_sync(kAll, y - y0, warp);
+        const Note* t = exchange(Note{__shfl_sync(kAll, x, kWarp - 1), __shfl_sync(kAll, y, kWarp - 1), 0u, 0u});  // (all bins are read)
         all_mass = 0ull;
         all_count = 0u;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             if (c < rank) {
                 before_m += t[c].a;
-                before_n += (uint32_t)t[c].b;
+                before_n += t[c].b;
             }
             all_mass += t[c].a;
             all_count += (uint32_t)t[c].b;
         }
         mass_ex = before_m + m - mass;
-        count_ex = before_n + n - count;
+        count_ex = (uint32_t)(before_n + nn) - count;
     };
 
     // ---- the questions: where the running count (of top_k) or weight sum (of
-    // top_p, of the draw) reaches `want`
+    // top_p, of the draw) reaches `want`. S becomes the sum up to and with that
+    // token.
     u64 S = 0ull, drawn = 0ull;
     int held = 0;  // bins: 0 clear, 1 of the whole row, 2 of a divided bin
     for (int q = 0; q < 3; ++q) {
         const bool by_mass = q > 0;
-        u64 want = (u64)k;
-        if (q > 0 && held) {
-            if (q == 1) {
-                if (!(p < 1.0f)) continue;
-                const double reach = ceil((double)S * (double)p);
-                want = reach > 1.0 ? (u64)reach : 1ull;
-            } else {
-                want = (u64)((double)u * (double)S);
-                want = min(want, S - 1) + 1;
-            }
+        u64 want = (u64)(uint32_t)k;
+        if (q == 1) {
+            if (!(p < 1.0f)) continue;
+            const double reach = ceil((double)S * (double)p);
+            want = reach > 1.0 ? (u64)reach : 1ull;
+        } else if (q == 2) {
+            want = min((u64)((double)u * (double)S), S - 1) + 1;
         }
         u64 before_m = 0ull;
         uint32_t before_n = 0u;
@@ -352,47 +403,37 @@ __global__ void __launch_bounds__(kThreads, 1) draw_kernel(const __grid_constant
         for (;;) {
             if (bin0 >= 0 || held != 1) {
                 if (held) {
-                    for (int i = tid; i < NB; i += kThreads) sh.count[i] = sh.lo[i] = sh.hi[i] = 0u;
+                    clear_bins();
                     __syncthreads();
                 }
                 histogram();
                 held = bin0 < 0 ? 1 : 2;
                 if (q == 0 && bin0 < 0) {
                     S = all_mass;
-                    if (!(k > 0 && all_count > (uint32_t)k)) break;  // every token stays
+                    if (!(counts && all_count > (uint32_t)k)) break;  // every token stays
                 }
             }
             // the bin that holds it: only its thread speaks up
             const bool mine = tid < SLICE && (by_mass ? before_m + mass_ex < want && want <= before_m + mass_ex + mass
                                                       : before_n + count_ex < want && want <= before_n + count_ex + count);
-            Note n{0ull, 0ull, 0u, 0u};
             if (mine) {
                 sh.res[0] = mass_ex;
                 sh.res[1] = ((u64)(uint32_t)(rank * SLICE + tid + 1) << 32) | count;
-                sh.red_a[0] = count_ex;
+                sh.res[2] = count_ex;
             }
             const bool here = __syncthreads_or(mine);
-            if (here) n = Note{sh.res[0], sh.res[1], sh.red_a[0], 1u};
-            const Note* t = exchange(n);
-            u64 m_ex = 0ull, bc = 0ull;
-            uint32_t n_ex = 0u;
+            Note note{0ull, 0ull, 0u, 0u};
+            if (here) note = Note{sh.res[0], sh.res[1], (uint32_t)sh.res[2], 1u};
+            const Note* t = exchange(note);
+            u64 bc = 0ull;
 #pragma unroll
             for (int c = 0; c < C; ++c)
                 if (t[c].d) {
-                    m_ex = t[c].a;
+                    before_m += t[c].a;
                     bc = t[c].b;
-                    n_ex = t[c].c;
+                    before_n += t[c].c;
                 }
             const int b = (int)(bc >> 32) - 1;
-            const uint32_t inside = (uint32_t)bc;
-            auto chosen = [&](int e) {  // token e of this thread is in the bin
-                if (!key[e]) return false;
-                const u64 c = composite(key[e], i0 + e * kThreads);
-                if (c < c_lo || c > c_hi) return false;
-                return bin_at(rule.exponent(key_logit(key[e]))) == bin0;
-            };
-            before_m += m_ex;
-            before_n += n_ex;
             if (bin0 < 0) {
                 bin0 = b;
                 c_hi = ~0ull;
@@ -403,66 +444,82 @@ __global__ void __launch_bounds__(kThreads, 1) draw_kernel(const __grid_constant
                 c_lo = max(c_lo, hi - ((1ull << shift) - 1ull));
                 c_hi = hi;
             }
-            if (inside <= kList) {
-                // collect the bin's tokens in every CTA's list, then rank them
-                const uint32_t counter = C == 1 ? 0u : at_rank(&sh.list_n, 0);
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    if (!chosen(e)) continue;
-                    const u64 w = rule.weight(key[e]);
-                    if (!w) continue;
-                    const u64 c = composite(key[e], i0 + e * kThreads);
+            u64 mx = 0ull, mn = ~0ull;
+            uint32_t sent = 0u;
+            const bool counted = counts || held == 2;
+            const uint32_t counter = C == 1 ? 0u : at_rank(&sh.list_n, 0), list = C == 1 ? 0u : at_rank(sh.list, 0);
+            const bool fits = counted && (uint32_t)bc <= kList;
+            if (!counted || fits) {
+                // to the first CTA's list, as far as it goes
+#pragma unroll 4
+                for (int i = tid; i < n; i += kThreads) {
+                    const float l = sh.row[i], x = rule.exponent(l);
+                    if (rule.bin(x) != bin0) continue;
+                    const u64 c = composite(l, i0 + i);
+                    if (c < c_lo || c > c_hi || !rule.weight(l, x).any()) continue;
                     if constexpr (C == 1) {
                         const uint32_t s = atomicAdd(&sh.list_n, 1u);
-                        sh.list_c[s] = c;
-                        sh.list_w[s] = w;
+                        if (s < kList) sh.list[s] = c;
                     } else {
                         const uint32_t s = add_rank(counter, 1u);
-#pragma unroll
-                        for (int q = 0; q < C; ++q) {
-                            st_rank(at_rank(&sh.list_c[s], q), c);
-                            st_rank(at_rank(&sh.list_w[s], q), w);
-                        }
+                        if (s < kList) st_rank(list + 8 * s, c);
                     }
                 }
                 barrier();
-                if (rank == 0 && tid == 0) sh.list_n = 0u;  // (added to again after the next exchange)
-                for (uint32_t i = warp; i < inside; i += kWarps) {
-                    const u64 c = sh.list_c[i], w = sh.list_w[i];
-                    u64 m = 0ull;
-                    uint32_t n2 = 0u;
-                    for (uint32_t j = lane; j < inside; j += kWarp)
-                        if (sh.list_c[j] > c) {
-                            m += sh.list_w[j];
-                            n2 += 1u;
+                sent = C == 1 ? sh.list_n : ld_rank(counter);
+            }
+            if (fits || (!counted && sent <= kList)) {
+                if (rank == 0) {
+                    // sort the list (largest first), scan the weights
+                    const uint32_t len = sent;
+                    int size2 = kWarp;
+                    while (size2 < (int)len) size2 <<= 1;
+                    u64 c = tid < (int)len ? sh.list[tid] : 0ull;
+                    for (int size = 2; size <= size2; size <<= 1)
+                        for (int stride = size >> 1; stride > 0; stride >>= 1) {
+                            u64 other;
+                            if (stride < kWarp) {
+                                other = __shfl_xor_sync(kAll, c, stride);
+                            } else {
+                                __syncthreads();
+                                sh.list[tid] = c;
+                                __syncthreads();
+                                other = sh.list[tid ^ stride];
+                            }
+                            const bool larger = ((tid & size) == 0) == ((tid & stride) == 0);
+                            c = larger ? max(c, other) : min(c, other);
                         }
-#pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) m += __shfl_xor_sync(kAll, m, o);
-                    n2 = __reduce_add_sync(kAll, n2);
-                    m += before_m;
-                    n2 += before_n;
-                    if (by_mass ? m < want && want <= m + w : n2 + 1u == want) {
-                        if (lane == 0) {
-                            sh.scan_m[0] = c;
-                            sh.scan_m[1] = m + w;
-                        }
+                    const float l = composite_logit(c);
+                    const u64 w = c ? rule.weight(l, rule.exponent(l)).whole() : 0ull;
+                    const u64 m = warp_scan(w);
+                    if (lane == kWarp - 1) sh.scan_x[warp] = m;
+                    __syncthreads();
+                    const u64 x0 = lane < kWarps ? sh.scan_x[lane] : 0ull;
+                    const u64 upto = before_m + m + __shfl_sync(kAll, warp_scan(x0) - x0, warp);
+                    if (c && (by_mass ? upto - w < want && want <= upto : before_n + (uint32_t)tid + 1u == (uint32_t)want)) {
+                        sh.res[0] = upto;
+                        sh.res[1] = c;
                     }
+                    __syncthreads();
                 }
-                __syncthreads();
-                drawn = sh.scan_m[0];
-                if (q < 2) S = sh.scan_m[1];
-                __syncthreads();
+                if (q < 2) {
+                    S = exchange(Note{sh.res[0], 0ull, 0u, 0u})[0].a;
+                    if (rank == 0 && tid == 0) sh.list_n = 0u;  // (every CTA has read it)
+                } else {
+                    if constexpr (C > 1) barrier();  // no CTA leaves while its counter may be read
+                    if (rank == 0) drawn = sh.res[1];
+                }
                 break;
             }
             // too many: divide the bin by (logit, index) between its extremes
-            u64 mx = 0ull, mn = ~0ull;
-#pragma unroll
-            for (int e = 0; e < E; ++e)
-                if (chosen(e) && rule.weight(key[e])) {
-                    const u64 c = composite(key[e], i0 + e * kThreads);
-                    mx = max(mx, c);
-                    mn = min(mn, c);
-                }
+            for (int i = tid; i < n; i += kThreads) {
+                const float l = sh.row[i], x = rule.exponent(l);
+                if (rule.bin(x) != bin0) continue;
+                const u64 c = composite(l, i0 + i);
+                if (c < c_lo || c > c_hi || !rule.weight(l, x).any()) continue;
+                mx = max(mx, c);
+                mn = min(mn, c);
+            }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) {
                 mx = max(mx, __shfl_xor_sync(kAll, mx, o));
@@ -471,11 +528,11 @@ __global__ void __launch_bounds__(kThreads, 1) draw_kernel(const __grid_constant
             __syncthreads();
             if (lane == 0) {
                 sh.scan_m[warp] = mx;
-                sh.list_c[warp] = mn;
+                sh.scan_x[warp] = mn;
             }
             __syncthreads();
-            mx = sh.scan_m[lane];
-            mn = sh.list_c[lane];
+            mx = sh.scan_m[lane % kWarps];
+            mn = sh.scan_x[lane % kWarps];
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) {
                 mx = max(mx, __shfl_xor_sync(kAll, mx, o));
@@ -487,24 +544,25 @@ __global__ void __launch_bounds__(kThreads, 1) draw_kernel(const __grid_constant
                 mx = max(mx, x[c].a);
                 mn = min(mn, x[c].b);
             }
+            if (rank == 0 && tid == 0) sh.list_n = 0u;  // (every CTA has read it)
             c_hi = mx;
             c_lo = mn;
-            shift = max(0, 64 - __clzll((long long)(c_hi - c_lo)) - (C == 1 ? 10 : 12));
+            shift = max(0, 64 - __clzll((long long)(c_hi - c_lo)) - Sh::NB_LOG);
         }
     }
     if (rank == 0 && tid == 0) {
         a.ids[r] = (uint32_t)((1 << kIndexBits) - 1) - (uint32_t)(drawn & ((1u << kIndexBits) - 1u));
-        if (a.logprobs)
-            a.logprobs[r] = rule.exponent(key_logit((uint32_t)(drawn >> kIndexBits))) - (float)log((double)S / (double)kOne);
+        if (a.logprobs) a.logprobs[r] = rule.exponent(composite_logit(drawn)) - (float)log((double)S / (double)kOne);
     }
 }
 
-template <int C, int E>
-void launch(const DrawArgs& a, cudaStream_t st) {
+template <int C>
+void launch(DrawArgs a, cudaStream_t st) {
+    a.chunk = (((a.vocab + C - 1) / C) + 1) & ~1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)a.rows * C);
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = sizeof(Shared<C>);
+    cfg.dynamicSmemBytes = smem_bytes<C>(a.chunk);
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -514,30 +572,21 @@ void launch(const DrawArgs& a, cudaStream_t st) {
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = C == 1 ? 1 : 2;
-    cudaLaunchKernelEx(&cfg, draw_kernel<C, E>, a);
+    cudaLaunchKernelEx(&cfg, draw_kernel<C>, a);
 }
 
-template <int C, int E>
-void prepare() {
-    configure_kernel((const void*)draw_kernel<C, E>, sizeof(Shared<C>));
-}
+constexpr int kOneCta = 16384;  // largest vocabulary that one CTA takes
 
 }  // namespace
 
 void launch_draw(const DrawArgs& a, cudaStream_t st) {
-    if (a.vocab <= 4 * kThreads) launch<1, 4>(a, st);
-    else if (a.vocab <= 16 * kThreads) launch<1, 16>(a, st);
-    else if (a.vocab <= 8 * 8 * kThreads) launch<8, 8>(a, st);
-    else if (a.vocab <= 8 * 20 * kThreads) launch<8, 20>(a, st);
-    else launch<8, 32>(a, st);
+    if (a.vocab <= kOneCta) launch<1>(a, st);
+    else launch<8>(a, st);
 }
 
 void prepare_draw_kernels() {
-    prepare<1, 4>();
-    prepare<1, 16>();
-    prepare<8, 8>();
-    prepare<8, 20>();
-    prepare<8, 32>();
+    configure_kernel((const void*)draw_kernel<1>, smem_bytes<1>(kOneCta));
+    configure_kernel((const void*)draw_kernel<8>, smem_bytes<8>(kDrawMaxVocab / 8));
 }
 
 }  // namespace zc

@@ -143,6 +143,7 @@ struct DrawArgs {
     int bf16;
     unsigned long long stride;
     int rows, vocab;           // vocab <= kDrawMaxVocab
+    int chunk;                 // tokens of one CTA (the launcher's)
     const float* uniforms;     // [rows]
     const float* temperature;  // 1
     const int* top_k;          // 0 = all
