@@ -85,8 +85,9 @@ __device__ __forceinline__ void join(Piece& p, int h, float m, float l, const fl
     for (int e = 0; e < 4; ++e) p.acc[h][e] = (c0 == 0.0f ? 0.0f : p.acc[h][e] * c0) + (c1 == 0.0f ? 0.0f : f[e] * c1);
 }
 
+template <int N>
 __global__ void __launch_bounds__(kThreads, 1)
-    attn_span_kernel(const __grid_constant__ ServeRows rows, const __grid_constant__ ServeAttnArgs a) {
+    attn_span_kernel(const __grid_constant__ ServeRowsT<N> rows, const __grid_constant__ ServeAttnArgs a) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
     const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
@@ -502,9 +503,15 @@ __global__ void __launch_bounds__(kThreads, 1)
 }  // namespace
 
 void launch_attn_span(const ServeRows& rows, const ServeAttnArgs& a, int ctas, cudaStream_t st) {
-    launch_pdl(attn_span_kernel, ctas, kThreads, sizeof(Smem), st, rows, a);
+    if (a.batch <= kServeSmallBatch)
+        launch_pdl(attn_span_kernel<kServeSmallBatch>, ctas, kThreads, sizeof(Smem), st, small_rows(rows), a);
+    else
+        launch_pdl(attn_span_kernel<kServeMaxBatch>, ctas, kThreads, sizeof(Smem), st, rows, a);
 }
 
-void prepare_attn_span_kernels() { configure_kernel((const void*)attn_span_kernel, sizeof(Smem)); }
+void prepare_attn_span_kernels() {
+    configure_kernel((const void*)attn_span_kernel<kServeSmallBatch>, sizeof(Smem));
+    configure_kernel((const void*)attn_span_kernel<kServeMaxBatch>, sizeof(Smem));
+}
 
 }  // namespace zc

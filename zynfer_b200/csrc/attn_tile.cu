@@ -44,7 +44,8 @@ using namespace serve;
 
 constexpr int kRows = 128;       // MMA M: 64 queries x 2 query heads, row 2 m + h
 constexpr int kMembers = kRows / kG;
-constexpr int kThreads = 320;    // warps 0-3 and 4-7: softmax; 8: TMA; 9: MMA
+constexpr int kThreads = 384;    // warps 0-3 and 4-7: softmax; 8: TMA; 9: MMA; 10, 11 fill the third warpgroup
+constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;  // 2 x 128 x 208 + 128 x 88 = 384 x 168, the launch's registers
 constexpr int kHalfDims = 64;    // dims of a 128-byte half row
 constexpr float kLag = 8.0f;     // log2 of the growth of a row's maximum that is left to lag
 
@@ -137,8 +138,8 @@ struct Job {
     int seg, nseg;     // its record among the tile's (nseg 1: the output itself)
 };
 
-template <int TILE_BLOCKS>
-__device__ __forceinline__ Job find_job(const ServeRows& rows, const TileList& list, const ServeAttnArgs& a) {
+template <int TILE_BLOCKS, int N>
+__device__ __forceinline__ Job find_job(const ServeRowsT<N>& rows, const TileListT<N>& list, const ServeAttnArgs& a) {
     Job j;
     if (list.n == 0) {  // chunk: the tiles that see most first
         const int per_seq = (a.tokens + kMembers - 1) / kMembers;
@@ -192,10 +193,10 @@ __device__ __forceinline__ void split_pair(float x0, float x1, uint32_t (&t)[TER
     }
 }
 
-template <int TERMS>
+template <int TERMS, int N>
 __global__ void __launch_bounds__(kThreads, 1)
-    attn_tile_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_constant__ ServeRows rows,
-                     const __grid_constant__ TileList list, const __grid_constant__ ServeAttnArgs a) {
+    attn_tile_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_constant__ ServeRowsT<N> rows,
+                     const __grid_constant__ TileListT<N> list, const __grid_constant__ ServeAttnArgs a) {
     using L = Lay<TERMS>;
     constexpr int TILE = L::TILE;
     extern __shared__ uint8_t smem_raw[];
@@ -238,84 +239,88 @@ __global__ void __launch_bounds__(kThreads, 1)
     pdl_launch_dependents();
     const int n = job.n;
 
-    if (warp == 8) {
-        // ---------------- K and V: one lane per half of a block of K or of V
-        constexpr int PER = 2 * L::BLOCKS;
-        const int* table = a.block_table + (size_t)job.slot * a.max_blocks;
-        const int is_v = lane / PER, blk = (lane % PER) >> 1, half = lane & 1;
-        for (int i = 0; i < n; ++i) {
-            const int s = i % L::STAGES, round = i / L::STAGES;
-            int y = a.kv_rows;  // past the end: zeros
-            const int v = (job.t_lo + i) * L::BLOCKS + blk;
-            if (lane < 2 * PER && v < job.span.total) {
-                const int id = table[job.span.block(v)];
-                if (id >= 0 && id < a.n_pool_blocks)
-                    y = a.kv_row0 + ((job.head * a.n_pool_blocks + id) * 2 + is_v) * kKvBlock;
-                else if (a.err) atomicOr(a.err, kErrBadIndex);
-            }
-            bool ok = true;
-            if (round > 0) ok = mbar_wait_bounded(&empty[s], (uint32_t)((round - 1) & 1), a.err);
-            if (!__all_sync(0xFFFFFFFFu, ok)) {
-                // the copies in flight land before the CTA ends
-                for (int k = max(0, i - L::STAGES); k < i; ++k) {
-                    mbar_wait_bounded(&full_k[k % L::STAGES], (uint32_t)((k / L::STAGES) & 1), nullptr);
-                    mbar_wait_bounded(&full_v[k % L::STAGES], (uint32_t)((k / L::STAGES) & 1), nullptr);
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+        if (warp == 8) {
+            // ---------------- K and V: one lane per half of a block of K or of V
+            constexpr int PER = 2 * L::BLOCKS;
+            const int* table = a.block_table + (size_t)job.slot * a.max_blocks;
+            const int is_v = lane / PER, blk = (lane % PER) >> 1, half = lane & 1;
+            for (int i = 0; i < n; ++i) {
+                const int s = i % L::STAGES, round = i / L::STAGES;
+                int y = a.kv_rows;  // past the end: zeros
+                const int v = (job.t_lo + i) * L::BLOCKS + blk;
+                if (lane < 2 * PER && v < job.span.total) {
+                    const int id = table[job.span.block(v)];
+                    if (id >= 0 && id < a.n_pool_blocks)
+                        y = a.kv_row0 + ((job.head * a.n_pool_blocks + id) * 2 + is_v) * kKvBlock;
+                    else if (a.err) atomicOr(a.err, kErrBadIndex);
                 }
-                break;
+                bool ok = true;
+                if (round > 0) ok = mbar_wait_bounded(&empty[s], (uint32_t)((round - 1) & 1), a.err);
+                if (!__all_sync(0xFFFFFFFFu, ok)) {
+                    // the copies in flight land before the CTA ends
+                    for (int k = max(0, i - L::STAGES); k < i; ++k) {
+                        mbar_wait_bounded(&full_k[k % L::STAGES], (uint32_t)((k / L::STAGES) & 1), nullptr);
+                        mbar_wait_bounded(&full_v[k % L::STAGES], (uint32_t)((k / L::STAGES) & 1), nullptr);
+                    }
+                    break;
+                }
+                uint8_t* ks = smem + L::Q + s * 2 * L::KV;
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(&full_k[s], L::KV);
+                    mbar_arrive_expect_tx(&full_v[s], L::KV);
+                }
+                __syncwarp();
+                if (lane < 2 * PER)
+                    tma_box(smem_addr(ks + is_v * L::KV + half * L::HALF + blk * (kKvBlock * 128)), &kv_map,
+                            half * kHalfDims, y, is_v ? &full_v[s] : &full_k[s]);
             }
-            uint8_t* ks = smem + L::Q + s * 2 * L::KV;
+        } else if (warp == 9) {
+            asm volatile("bar.sync 1, 288;" ::: "memory");  // Q is in shared memory
             if (lane == 0) {
-                mbar_arrive_expect_tx(&full_k[s], L::KV);
-                mbar_arrive_expect_tx(&full_v[s], L::KV);
+                // ---------------- MMA issuer: S of tile i, then P V of tile i - 1.
+                // MMAs run in issue order, so S(i) overwrites the P of tile i - 2
+                // after it was read.
+                constexpr uint32_t id_s = idesc(TILE, false), id_o = idesc(kD, true);
+                const uint32_t qs = smem_addr(smem);
+                for (int i = 0; i <= n; ++i) {
+                    if (i < n) {
+                        const int s = i % L::STAGES;
+                        if (!mbar_wait_bounded(&full_k[s], (uint32_t)((i / L::STAGES) & 1), a.err)) break;
+                        tc_fence_after();
+                        const uint32_t ks = smem_addr(smem + L::Q + s * 2 * L::KV);
+                        const uint32_t d = tmem + L::S_COL + (i & 1) * L::S_STEP;
+#pragma unroll
+                        for (int t = TERMS - 1; t >= 0; --t)  // the small terms first: fewer roundings at the sum's size
+#pragma unroll
+                            for (int kk = 0; kk < 8; ++kk)
+                                mma_ss(d, sdesc(qs + t * L::QTERM + (kk >> 2) * (kRows * 128) + (kk & 3) * 32, 16),
+                                       sdesc(ks + (kk >> 2) * L::HALF + (kk & 3) * 32, 16), id_s, t < TERMS - 1 || kk);
+                        mma_commit(&s_full[i & 1]);
+                    }
+                    if (i > 0) {
+                        const int j = i - 1, w = j & 1, s = j % L::STAGES;
+                        if (!mbar_wait_bounded(&full_v[s], (uint32_t)((j / L::STAGES) & 1), a.err)) break;
+                        if (!mbar_wait_bounded(&p_full[w], (uint32_t)((j >> 1) & 1), a.err)) break;
+                        tc_fence_after();
+                        const uint32_t vs = smem_addr(smem + L::Q + s * 2 * L::KV + L::KV);
+                        const uint32_t p = tmem + L::S_COL + w * L::S_STEP, d = tmem + L::O_COL + w * kD;
+#pragma unroll
+                        for (int t = TERMS - 1; t >= 0; --t)
+#pragma unroll
+                            for (int kk = 0; kk < TILE / 16; ++kk)
+                                mma_ts(d, p + t * (TILE / 2) + kk * 8, sdesc(vs + kk * 2048, L::HALF), id_o,
+                                       j > 1 || t < TERMS - 1 || kk);
+                        mma_commit(&empty[s]);
+                        if (j + 2 >= n) mma_commit(&o_full[w]);
+                    }
+                }
             }
             __syncwarp();
-            if (lane < 2 * PER)
-                tma_box(smem_addr(ks + is_v * L::KV + half * L::HALF + blk * (kKvBlock * 128)), &kv_map,
-                        half * kHalfDims, y, is_v ? &full_v[s] : &full_k[s]);
         }
-    } else if (warp == 9) {
-        asm volatile("bar.sync 1, 288;" ::: "memory");  // Q is in shared memory
-        if (lane == 0) {
-            // ---------------- MMA issuer: S of tile i, then P V of tile i - 1.
-            // MMAs run in issue order, so S(i) overwrites the P of tile i - 2
-            // after it was read.
-            constexpr uint32_t id_s = idesc(TILE, false), id_o = idesc(kD, true);
-            const uint32_t qs = smem_addr(smem);
-            for (int i = 0; i <= n; ++i) {
-                if (i < n) {
-                    const int s = i % L::STAGES;
-                    if (!mbar_wait_bounded(&full_k[s], (uint32_t)((i / L::STAGES) & 1), a.err)) break;
-                    tc_fence_after();
-                    const uint32_t ks = smem_addr(smem + L::Q + s * 2 * L::KV);
-                    const uint32_t d = tmem + L::S_COL + (i & 1) * L::S_STEP;
-#pragma unroll
-                    for (int t = TERMS - 1; t >= 0; --t)  // the small terms first: fewer roundings at the sum's size
-#pragma unroll
-                        for (int kk = 0; kk < 8; ++kk)
-                            mma_ss(d, sdesc(qs + t * L::QTERM + (kk >> 2) * (kRows * 128) + (kk & 3) * 32, 16),
-                                   sdesc(ks + (kk >> 2) * L::HALF + (kk & 3) * 32, 16), id_s, t < TERMS - 1 || kk);
-                    mma_commit(&s_full[i & 1]);
-                }
-                if (i > 0) {
-                    const int j = i - 1, w = j & 1, s = j % L::STAGES;
-                    if (!mbar_wait_bounded(&full_v[s], (uint32_t)((j / L::STAGES) & 1), a.err)) break;
-                    if (!mbar_wait_bounded(&p_full[w], (uint32_t)((j >> 1) & 1), a.err)) break;
-                    tc_fence_after();
-                    const uint32_t vs = smem_addr(smem + L::Q + s * 2 * L::KV + L::KV);
-                    const uint32_t p = tmem + L::S_COL + w * L::S_STEP, d = tmem + L::O_COL + w * kD;
-#pragma unroll
-                    for (int t = TERMS - 1; t >= 0; --t)
-#pragma unroll
-                        for (int kk = 0; kk < TILE / 16; ++kk)
-                            mma_ts(d, p + t * (TILE / 2) + kk * 8, sdesc(vs + kk * 2048, L::HALF), id_o,
-                                   j > 1 || t < TERMS - 1 || kk);
-                    mma_commit(&empty[s]);
-                    if (j + 2 >= n) mma_commit(&o_full[w]);
-                }
-            }
-        }
-        __syncwarp();
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
         // ---------------- softmax: thread = one query row, warpgroup w takes tiles w, w + 2, ..
         const int w = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
         const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
@@ -387,10 +392,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (!((bits >> c) & 1u)) s[u * kKvBlock + c] = -INFINITY;
                 }
             }
-            float mt = s[0];
+            float mx[8];
 #pragma unroll
-            for (int c = 1; c < TILE; ++c) mt = fmaxf(mt, s[c]);
-            mt *= scale2;
+            for (int c = 0; c < 8; ++c) mx[c] = fmaxf(s[c], s[c + 8]);
+#pragma unroll
+            for (int c = 16; c < TILE; c += 16)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) mx[e] = fmaxf(mx[e], fmaxf(s[c + e], s[c + 8 + e]));
+            const float mt = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7]))) * scale2;
             const bool grow = mt > m_ref + kLag || (m_ref == -INFINITY && mt > -INFINITY);
             if (__any_sync(0xFFFFFFFFu, grow)) {
                 const float m_new = grow ? mt : m_ref;
@@ -410,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
             const float neg = m_ref == -INFINITY ? 0.0f : -m_ref;
-            float sum0 = 0.0f, sum1 = 0.0f;
+            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int c0 = 0; c0 < TILE; c0 += 64) {
                 uint32_t p[TERMS][32];
@@ -418,8 +427,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int e = 0; e < 32; ++e) {
                     const float x0 = exp2_fast(fmaf(s[c0 + 2 * e], scale2, neg));
                     const float x1 = exp2_fast(fmaf(s[c0 + 2 * e + 1], scale2, neg));
-                    sum0 += x0;
-                    sum1 += x1;
+                    sum[(2 * e) & 3] += x0;
+                    sum[(2 * e + 1) & 3] += x1;
                     uint32_t u[TERMS];
                     split_pair<TERMS>(x0, x1, u);
 #pragma unroll
@@ -428,7 +437,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                 for (int k = 0; k < TERMS; ++k) tmem_st32(s_at + k * (TILE / 2) + c0 / 2, p[k]);
             }
-            l += sum0 + sum1;
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             tmem_wait_st();
             tc_fence_before();
             mbar_arrive(&p_full[w]);
@@ -513,13 +522,29 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 void launch_attn_tile(const CUtensorMap& kv_map, const ServeRows& rows, const TileList& list, const ServeAttnArgs& a,
                       int items, cudaStream_t st) {
-    if (a.bf16) launch_pdl(attn_tile_kernel<1>, items, kThreads, Lay<1>::SMEM, st, kv_map, rows, list, a);
-    else launch_pdl(attn_tile_kernel<3>, items, kThreads, Lay<3>::SMEM, st, kv_map, rows, list, a);
+    if (a.batch <= kServeSmallBatch) {
+        TileListT<kServeSmallBatch> small;
+        small.n = list.n;
+        for (int e = 0; e < list.n; ++e) {
+            small.item0[e] = list.item0[e];
+            small.first[e] = list.first[e];
+            small.count[e] = list.count[e];
+            small.blocks[e] = list.blocks[e];
+        }
+        small.item0[list.n] = items;
+        if (a.bf16) launch_pdl(attn_tile_kernel<1, kServeSmallBatch>, items, kThreads, Lay<1>::SMEM, st, kv_map, small_rows(rows), small, a);
+        else launch_pdl(attn_tile_kernel<3, kServeSmallBatch>, items, kThreads, Lay<3>::SMEM, st, kv_map, small_rows(rows), small, a);
+    } else {
+        if (a.bf16) launch_pdl(attn_tile_kernel<1, kServeMaxBatch>, items, kThreads, Lay<1>::SMEM, st, kv_map, rows, list, a);
+        else launch_pdl(attn_tile_kernel<3, kServeMaxBatch>, items, kThreads, Lay<3>::SMEM, st, kv_map, rows, list, a);
+    }
 }
 
 void prepare_attn_tile_kernels() {
-    configure_kernel((const void*)attn_tile_kernel<1>, Lay<1>::SMEM);
-    configure_kernel((const void*)attn_tile_kernel<3>, Lay<3>::SMEM);
+    configure_kernel((const void*)attn_tile_kernel<1, kServeSmallBatch>, Lay<1>::SMEM);
+    configure_kernel((const void*)attn_tile_kernel<3, kServeSmallBatch>, Lay<3>::SMEM);
+    configure_kernel((const void*)attn_tile_kernel<1, kServeMaxBatch>, Lay<1>::SMEM);
+    configure_kernel((const void*)attn_tile_kernel<3, kServeMaxBatch>, Lay<3>::SMEM);
 }
 
 }  // namespace zc

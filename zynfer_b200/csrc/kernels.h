@@ -161,21 +161,27 @@ void launch_draw(const DrawArgs& a, cudaStream_t st);
 // nothing to the device.
 constexpr int kServeMaxBatch = 1024;
 constexpr int kServeRecord = 132;  // words of a partial result: m, l, -, -, acc[128]
-struct ServeRows {
-    int slot[kServeMaxBatch];  // sequence slot (block-table row)
-    int len[kServeMaxBatch];   // cached positions, the queries' own among them
-    int row[kServeMaxBatch];   // row of q and out (one query per sequence)
-    int skip[kServeMaxBatch];  // leading blocks that the row's tile takes
-    int nrec[kServeMaxBatch];  // partial results that the tile leaves
+// Kernel parameters cost about 0.1 us of the launch per KB, so the kernels are
+// built for small batches and for the largest (N rows).
+template <int N>
+struct ServeRowsT {
+    int slot[N];  // sequence slot (block-table row)
+    int len[N];   // cached positions, the queries' own among them
+    int row[N];   // row of q and out (one query per sequence)
+    int skip[N];  // leading blocks that the row's tile takes
+    int nrec[N];  // partial results that the tile leaves
 };
 // Rows that share leading blocks, in tiles of up to 64.
-constexpr int kServeMaxTiles = kServeMaxBatch / 2;
-struct TileList {
-    int n;                         // 0: tiles are chunks of sequences instead
-    int item0[kServeMaxTiles + 1]; // first work item; (item0[e + 1] - item0[e]) / n_kv splits of its blocks
-    short first[kServeMaxTiles], count[kServeMaxTiles];  // rows of ServeRows
-    int blocks[kServeMaxTiles];    // common leading blocks
+template <int N>
+struct TileListT {
+    int n;                               // 0: tiles are chunks of sequences instead
+    int item0[N / 2 + 1];                // first work item; (item0[e + 1] - item0[e]) / n_kv splits of its blocks
+    short first[N / 2], count[N / 2];    // rows of ServeRows
+    int blocks[N / 2];                   // common leading blocks
 };
+constexpr int kServeSmallBatch = 64;
+using ServeRows = ServeRowsT<kServeMaxBatch>;
+using TileList = TileListT<kServeMaxBatch>;
 struct ServeAttnArgs {
     const uint16_t* kv_layer;  // [n_kv][blocks][K, V][16][d], rows chunk-swizzled (kv_swizzle)
     const int* block_table;    // [seqs][max_blocks]
@@ -202,6 +208,18 @@ void prepare_attn_span_kernels();
 // blocks / (kSpanWarps min_per) + 2 CTAs.
 constexpr int kSpanWarps = 8;
 void launch_attn_span(const ServeRows& rows, const ServeAttnArgs& a, int ctas, cudaStream_t st);
+// The first rows of a batch of at most kServeSmallBatch.
+inline ServeRowsT<kServeSmallBatch> small_rows(const ServeRows& r) {
+    ServeRowsT<kServeSmallBatch> s;
+    for (int i = 0; i < kServeSmallBatch; ++i) {
+        s.slot[i] = r.slot[i];
+        s.len[i] = r.len[i];
+        s.row[i] = r.row[i];
+        s.skip[i] = r.skip[i];
+        s.nrec[i] = r.nrec[i];
+    }
+    return s;
+}
 // Cache blocks that a query at `pos` sees after the first `skip`.
 int serve_span_blocks(int pos, uint32_t window, int sinks, int skip);
 void launch_serve_merge(const ServeRows& rows, const ServeAttnArgs& a, cudaStream_t st);

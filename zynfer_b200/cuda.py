@@ -7,8 +7,8 @@ in-tree library and nothing else: there is no CPU path here.
 """
 from __future__ import annotations
 
+import array
 import atexit
-import contextlib
 import ctypes as C
 import os
 import weakref
@@ -178,12 +178,49 @@ def _ptr(a) -> C.c_void_p | None:
     return a.ctypes.data_as(C.c_void_p)
 
 
+_KINDS = {}  # dtype object -> its name ("float32"); a call looks up a dozen of them
+
+
+def _kind(t) -> str:
+    name = _KINDS.get(t.dtype)
+    if name is None:
+        name = _KINDS[t.dtype] = str(t.dtype).rsplit(".", 1)[-1]
+    return name
+
+
+_SERVE_DT = {"float32": DT_F32, "bfloat16": DT_BF16}
+
+
 def _dtype(t) -> int:
     """ZYNFER_CU_DT_* of a device tensor the serving calls take."""
-    name = str(t.dtype).rsplit(".", 1)[-1]
-    if name not in ("float32", "bfloat16"):
-        raise Unsupported(f"float32 or bfloat16 tensors, not {name}")
-    return DT_F32 if name == "float32" else DT_BF16
+    dt = _SERVE_DT.get(_kind(t))
+    if dt is None:
+        raise Unsupported(f"float32 or bfloat16 tensors, not {_kind(t)}")
+    return dt
+
+
+def _row_values(t, rows: int, kinds, name: str):
+    """Address of a dense tensor of one value per row (None: 0)."""
+    if t is None:
+        return None
+    if _kind(t) not in kinds or t.dim() != 1 or t.shape[0] != rows or not t.is_contiguous():
+        raise InvalidArgument(f"{name} must be a dense {kinds[0]} tensor of one value per row")
+    return t.data_ptr()
+
+
+_F32, _I32 = ("float32",), ("int32", "uint32")
+
+
+def _ids(seqs):
+    """Sequence ids as a C array: its address, its length, and the array to keep alive."""
+    if not isinstance(seqs, np.ndarray):
+        try:
+            a = array.array("I", seqs)
+        except OverflowError:
+            raise InvalidArgument("sequence id out of range") from None
+        return a.buffer_info()[0], len(a), a
+    a = np.ascontiguousarray(seqs, np.uint32)
+    return a.ctypes.data, a.size, a
 
 
 def _require(ok: bool, what: str):
@@ -261,6 +298,7 @@ class Gpu:
                 L.zynfer_cu_destroy(h)
             self.h = None
             raise _ERRORS.get(rc, CudaError)(msg)
+        self._rule = DrawRule()
         _LIVE.add(self)
 
     def check(self, rc: int):
@@ -314,21 +352,18 @@ class Gpu:
         random numbers uniforms [rows] into ids [rows] (32-bit) and, where given, logprobs [rows]; temperature,
         top_k (int32), top_p and min_p are device tensors [rows] or None (zynfer_cu_sample_rows). Asynchronous;
         `stream` (a torch stream) orders the call after its work and its later work after the call."""
-        _require(len(logits.shape) == 2 and logits.stride(1) == 1, "logits must be [rows, vocab] with unit inner stride")
+        if logits.dim() != 2 or logits.stride(1) != 1:
+            raise InvalidArgument("logits must be [rows, vocab] with unit inner stride")
         rows, vocab = logits.shape
-        per_row = [("uniforms", uniforms, "float32"), ("ids", ids, "int32"), ("logprobs", logprobs, "float32"),
-                   ("temperature", temperature, "float32"), ("top_k", top_k, "int32"), ("top_p", top_p, "float32"),
-                   ("min_p", min_p, "float32")]
-        for name, t, kind in per_row:
-            if t is not None:
-                got = str(t.dtype).rsplit(".", 1)[-1]
-                _require(got in (kind, "u" + kind) and tuple(t.shape) == (rows,) and (rows == 1 or t.stride(0) == 1),
-                         f"{name} must be a dense {kind} tensor of one value per row")
-        rule = DrawRule(*(None if t is None else t.data_ptr() for t in (temperature, top_k, top_p, min_p)))
-        stride = logits.stride(0) if rows > 1 else vocab
-        with self._ordered(stream):
-            self.check(lib().zynfer_cu_sample_rows(self.h, _ptr(logits), _dtype(logits), stride, rows, vocab,
-                                                   _ptr(uniforms), C.byref(rule), _ptr(ids), _ptr(logprobs)))
+        rule = self._rule
+        rule.temperature = _row_values(temperature, rows, _F32, "temperature")
+        rule.top_k = _row_values(top_k, rows, _I32, "top_k")
+        rule.top_p = _row_values(top_p, rows, _F32, "top_p")
+        rule.min_p = _row_values(min_p, rows, _F32, "min_p")
+        call = (self.h, logits.data_ptr(), _dtype(logits), logits.stride(0) if rows > 1 else vocab, rows, vocab,
+                _row_values(uniforms, rows, _F32, "uniforms"), C.byref(rule), _row_values(ids, rows, _I32, "ids"),
+                _row_values(logprobs, rows, _F32, "logprobs"))
+        self._enqueue(stream, lib().zynfer_cu_sample_rows, call)
 
     def wait_stream(self, stream):
         """Later work of this context waits for what `stream` (a torch stream or a cudaStream_t) holds now."""
@@ -338,11 +373,11 @@ class Gpu:
         """Later work of `stream` waits for what this context has enqueued so far."""
         self.check(lib().zynfer_cu_stream_wait(self.h, VP(int(getattr(stream, "cuda_stream", stream or 0)))))
 
-    @contextlib.contextmanager
-    def _ordered(self, stream):
+    def _enqueue(self, stream, fn, args):
+        """An asynchronous call; with a stream, after its work so far and before its later work."""
         if stream is not None:
             self.wait_stream(stream)
-        yield
+        self.check(fn(*args))
         if stream is not None:
             self.stream_wait(stream)
 
@@ -493,41 +528,45 @@ class Model:
         _require(len(k.shape) == 3 and k.shape == v.shape and k.shape[0] == a.n_kv and k.shape[2] == a.head_dim and
                  k.dtype == v.dtype and k.is_contiguous() and v.is_contiguous(),
                  "k and v must be dense [n_kv, n, head_dim] tensors of one type")
-        with self.gpu._ordered(stream):
-            self.gpu.check(lib().zynfer_cu_kv_write(self.gpu.h, seq, layer, pos, k.shape[1], _ptr(k), _ptr(v), _dtype(k)))
+        self.gpu._enqueue(stream, lib().zynfer_cu_kv_write,
+                          (self.gpu.h, seq, layer, pos, k.shape[1], k.data_ptr(), v.data_ptr(), _dtype(k)))
 
     def _serve_rows(self, t, lead):
         """Row stride of a [.., n_q, head_dim] tensor whose leading dimensions `lead` are rows at one stride."""
         a, shape, st = self.arch, tuple(t.shape), t.stride()
-        _require(shape == (*lead, a.n_q, a.head_dim), f"expected a tensor of shape {(*lead, a.n_q, a.head_dim)}, not {shape}")
-        _require(st[-1] == 1 and st[-2] == a.head_dim, "a row's heads must be dense")
-        rows = [(n, s) for n, s in zip(lead, st) if n > 1]
-        for (_, outer), (n, inner) in zip(rows, rows[1:]):
-            _require(outer == n * inner, "rows must lie at one stride")
-        return rows[-1][1] if rows else a.n_q * a.head_dim
+        if shape != (*lead, a.n_q, a.head_dim):
+            raise InvalidArgument(f"expected a tensor of shape {(*lead, a.n_q, a.head_dim)}, not {shape}")
+        if st[-1] != 1 or st[-2] != a.head_dim:
+            raise InvalidArgument("a row's heads must be dense")
+        if len(lead) == 2 and lead[1] > 1:
+            if lead[0] > 1 and st[0] != lead[1] * st[1]:
+                raise InvalidArgument("rows must lie at one stride")
+            return st[1]
+        return st[0] if lead[0] > 1 else a.n_q * a.head_dim
 
     def attn_shared(self, layer: int, seqs, q, out, stream=None):
         """Decode attention of one query per sequence (device q and out [B, n_q, head_dim], f32 or bf16, rows at
         any stride) over all cached positions; leading blocks that sequences share are read once. Asynchronous."""
-        s = np.ascontiguousarray(seqs, np.uint32)
-        _require(q.dtype == out.dtype, "q and out must have one type")
-        qs, os_ = self._serve_rows(q, (s.size,)), self._serve_rows(out, (s.size,))
-        with self.gpu._ordered(stream):
-            self.gpu.check(lib().zynfer_cu_attn_shared(self.gpu.h, layer, _ptr(s), s.size, _ptr(q), qs, _ptr(out), os_,
-                                                       _dtype(q)))
+        ids, n, keep = _ids(seqs)
+        if q.dtype != out.dtype:
+            raise InvalidArgument("q and out must have one type")
+        lead = (n,)
+        self.gpu._enqueue(stream, lib().zynfer_cu_attn_shared,
+                          (self.gpu.h, layer, ids, n, q.data_ptr(), self._serve_rows(q, lead), out.data_ptr(),
+                           self._serve_rows(out, lead), _dtype(q)))
 
     def attn_window(self, layer: int, seqs, q, out, window: int = WINDOW_ALL, sinks: int = 0, stream=None):
         """Attention of the last T cached positions of each sequence (device q and out [B, T, n_q, head_dim], or
         [B, n_q, head_dim] for T = 1) over the last `window` positions up to each and the first `sinks`. Asynchronous."""
-        s = np.ascontiguousarray(seqs, np.uint32)
-        _require(q.dtype == out.dtype, "q and out must have one type")
-        _require(len(q.shape) in (3, 4) and window >= 0 and sinks >= 0, "q must be [B, n_q, d] or [B, T, n_q, d]")
-        lead = (s.size,) if len(q.shape) == 3 else (s.size, q.shape[1])
-        qs, os_ = self._serve_rows(q, lead), self._serve_rows(out, lead)
-        with self.gpu._ordered(stream):
-            self.gpu.check(lib().zynfer_cu_attn_window(self.gpu.h, layer, _ptr(s), s.size, lead[1] if len(lead) > 1 else 1,
-                                                       min(window, WINDOW_ALL), min(sinks, WINDOW_ALL), _ptr(q), qs,
-                                                       _ptr(out), os_, _dtype(q)))
+        ids, n, keep = _ids(seqs)
+        dims = q.dim()
+        if q.dtype != out.dtype or dims not in (3, 4) or window < 0 or sinks < 0:
+            raise InvalidArgument("q and out must be [B, n_q, d] or [B, T, n_q, d] of one type; window and sinks not negative")
+        lead = (n,) if dims == 3 else (n, q.shape[1])
+        self.gpu._enqueue(stream, lib().zynfer_cu_attn_window,
+                          (self.gpu.h, layer, ids, n, q.shape[1] if dims == 4 else 1, min(window, WINDOW_ALL),
+                           min(sinks, WINDOW_ALL), q.data_ptr(), self._serve_rows(q, lead), out.data_ptr(),
+                           self._serve_rows(out, lead), _dtype(q)))
 
     def rmsnorm_qk_rope(self, qkv, rows: int, q_norm, k_norm, pos0: int, q_out, k_out):
         """Per-head q/k RMSNorm + RoPE of `rows` tokens (device pointers, heads-major outputs)."""
