@@ -366,3 +366,19 @@ def test_shared_prompt_nan_stays_in_its_dims(dtype):
         keep = torch.tensor([d for d in range(D) if d != 64], device="cuda")
         check(out[i:i + 1][..., keep], want[..., keep], clean, dtype)
         check(out[i:i + 1, 2:], want[:, 2:], clean, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("tokens,length,window,sinks", [(70, 2100, zc.WINDOW_ALL, 0), (1, 3000, 1500, 7), (2100, 2100, 900, 20)])
+def test_long_loops_over_tiles(tokens, length, window, sinks, dtype):
+    """Many tiles of keys per tile of queries: every ring and barrier wraps several times."""
+    m = make(n_kv=2, max_seq_len=3008)
+    k, v = normal(41, 2, length, D, dtype=torch.bfloat16), normal(42, 2, length, D, dtype=torch.bfloat16)
+    m.kv_write(2, 0, 0, k, v)
+    q = normal(43, 1, tokens, 4, D, dtype=DTYPES[dtype], scale=1.5)
+    out = torch.empty_like(q)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        m.attn_window(0, [2], q, out, window=window, sinks=sinks)
+    m.gpu.sync()
+    check(out[0], reference(q[0], k, v, window_seen(length, tokens, window, sinks)), v, dtype)

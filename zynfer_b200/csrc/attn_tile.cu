@@ -4,13 +4,14 @@
 // and sinks, and the common prompt of sequences that share it.
 //
 // A CTA takes 128 query rows of one kv head (64 queries x 2 query heads: the
-// MMA's M) and a range of the visible 16-token cache blocks, TILE tokens at a
+// MMA's M) and a range of the visible 16-token cache blocks, 64 tokens at a
 // time: S = Q K^T into TMEM, softmax in registers with one thread per row,
-// P back into TMEM as the next MMA's A operand, O += P V into TMEM.
-// Two warpgroups take the tiles in turn, each with an accumulator, a running
-// maximum and a sum of its own (joined at the end), so the tensor cores work
-// on one tile while the exponentials of the other are taken. Warp 8 loads
-// K and V, warp 9 issues the MMAs.
+// P back into TMEM over S as the next MMA's A operand, O += P V into TMEM.
+// S has two buffers: the tensor cores form tile i + 1 while the exponentials of
+// tile i are taken. Warps 0-3: softmax; 4, 5: loads of K and of V, each a ring
+// of its own (K's places are free again after S, V's after P V); 6: MMAs.
+// With bf16 queries two CTAs share an SM, so that the start and the end of one
+// (a third of its time at a window of 1024) run beside the middle of the other.
 //
 // The cache's layout is the MMA's: a block row is 256 bytes whose 16-byte
 // chunks are XOR-swizzled by token & 7 inside each 128-byte half, so 16-row
@@ -44,25 +45,26 @@ using namespace serve;
 
 constexpr int kRows = 128;       // MMA M: 64 queries x 2 query heads, row 2 m + h
 constexpr int kMembers = kRows / kG;
-constexpr int kThreads = 384;    // warps 0-3 and 4-7: softmax; 8: TMA; 9: MMA; 10, 11 fill the third warpgroup
-constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;  // 2 x 128 x 208 + 128 x 88 = 384 x 168, the launch's registers
-constexpr int kHalfDims = 64;    // dims of a 128-byte half row
+constexpr int kThreads = 256;    // warps 0-3: softmax; 4: K; 5: V; 6: MMA
+constexpr int TILE = 64, kTileBlocks = TILE / kKvBlock;  // tokens of a tile
+constexpr int kHalf = TILE * 128, kTileBytes = 2 * kHalf;  // a K or V tile: two 64-dim halves
+constexpr int kHalfDims = 64;
 constexpr float kLag = 8.0f;     // log2 of the growth of a row's maximum that is left to lag
+constexpr unsigned kAll = 0xFFFFFFFFu;
 
 template <int TERMS>
 struct Lay {
-    static constexpr int TILE = TERMS == 1 ? 128 : 64;  // tokens per tile
-    static constexpr int BLOCKS = TILE / kKvBlock;
-    static constexpr int STAGES = TERMS == 1 ? 3 : 4;
-    static constexpr int HALF = TILE * 128;             // bytes of one half (64 dims) of a K or V tile
-    static constexpr int KV = 2 * HALF;
+    static constexpr int CTAS = TERMS == 1 ? 2 : 1;      // per SM
+    static constexpr int KST = TERMS == 1 ? 2 : 3, VST = 3;
     static constexpr int QTERM = kRows * 256;
-    static constexpr int Q = TERMS * QTERM;
-    static constexpr int BARS = Q + STAGES * 2 * KV;
-    static constexpr int SMEM = BARS + 512 + 1024;      // 1024: alignment of the first atom
-    static_assert(SMEM <= 232448, "tile attention shared memory");
-    // TMEM columns: two accumulators, then per warpgroup S with P over it
-    static constexpr int O_COL = 0, S_COL = 256, S_STEP = 128;
+    static constexpr int K = TERMS * QTERM, V = K + KST * kTileBytes;
+    static constexpr int BARS = V + VST * kTileBytes;
+    static constexpr int SMEM = BARS + 512;
+    static_assert(CTAS * (SMEM + 1024) <= 233472, "tile attention shared memory");
+    static_assert(BARS >= kRows * kD * 4, "the results are staged over Q, K and V");
+    // TMEM columns: the accumulator, then two regions of S with P over it
+    static constexpr int S_COL = kD, S_STEP = TERMS == 1 ? 64 : 128;
+    static constexpr int COLS = TERMS == 1 ? 256 : 512;
 };
 
 __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
@@ -138,7 +140,7 @@ struct Job {
     int seg, nseg;     // its record among the tile's (nseg 1: the output itself)
 };
 
-template <int TILE_BLOCKS, int N>
+template <int N>
 __device__ __forceinline__ Job find_job(const ServeRowsT<N>& rows, const TileListT<N>& list, const ServeAttnArgs& a) {
     Job j;
     if (list.n == 0) {  // chunk: the tiles that see most first
@@ -173,7 +175,7 @@ __device__ __forceinline__ Job find_job(const ServeRowsT<N>& rows, const TileLis
         j.p0 = j.p1 = list.blocks[lo] * kKvBlock - 1;  // every row sees every position of the common blocks
         j.span = Span{0, 0, list.blocks[lo]};
     }
-    const int tiles = (j.span.total + TILE_BLOCKS - 1) / TILE_BLOCKS;
+    const int tiles = (j.span.total + kTileBlocks - 1) / kTileBlocks;
     j.t_lo = (int)((long long)j.seg * tiles / j.nseg);
     j.n = (int)((long long)(j.seg + 1) * tiles / j.nseg) - j.t_lo;
     return j;
@@ -194,43 +196,49 @@ __device__ __forceinline__ void split_pair(float x0, float x1, uint32_t (&t)[TER
 }
 
 template <int TERMS, int N>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads, Lay<TERMS>::CTAS)
     attn_tile_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_constant__ ServeRowsT<N> rows,
                      const __grid_constant__ TileListT<N> list, const __grid_constant__ ServeAttnArgs a) {
     using L = Lay<TERMS>;
-    constexpr int TILE = L::TILE;
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    extern __shared__ __align__(1024) uint8_t smem[];
     uint64_t* full_k = reinterpret_cast<uint64_t*>(smem + L::BARS);
-    uint64_t* full_v = full_k + L::STAGES;
-    uint64_t* empty = full_v + L::STAGES;
-    uint64_t* s_full = empty + L::STAGES;  // [2] S of warpgroup w is in TMEM
-    uint64_t* p_full = s_full + 2;         // [2] its P is
-    uint64_t* o_full = p_full + 2;         // [2] its last product is done
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2);
-    uint32_t* bad_rows = tmem_slot + 1;    // [4] bit per row: not finite
+    uint64_t* empty_k = full_k + L::KST;
+    uint64_t* full_v = empty_k + L::KST;
+    uint64_t* empty_v = full_v + L::VST;
+    uint64_t* s_full = empty_v + L::VST;  // [2] S of tile i (buffer i & 1) is in TMEM
+    uint64_t* p_full = s_full + 2;        // [2] its P is (a barrier per buffer: P of tile i + 1 may be there before
+                                          // the MMA warp has looked for that of tile i)
+    uint64_t* o_full = p_full + 2;        // P V of tile i is done
+    uint64_t* done = o_full + 1;          // that of the last one is
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+    uint32_t* bad_rows = tmem_slot + 1;   // [4] bit per row: not finite
 
     const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < L::STAGES; ++s) {
+        for (int s = 0; s < L::KST; ++s) {
             mbar_init(&full_k[s], 1);
+            mbar_init(&empty_k[s], 1);
+        }
+        for (int s = 0; s < L::VST; ++s) {
             mbar_init(&full_v[s], 1);
-            mbar_init(&empty[s], 1);
+            mbar_init(&empty_v[s], 1);
         }
-        for (int w = 0; w < 2; ++w) {
-            mbar_init(&s_full[w], 1);
-            mbar_init(&p_full[w], 128);
-            mbar_init(&o_full[w], 1);
-        }
+        mbar_init(&s_full[0], 1);
+        mbar_init(&s_full[1], 1);
+        mbar_init(&p_full[0], 128);
+        mbar_init(&p_full[1], 128);
+        mbar_init(o_full, 1);
+        mbar_init(done, 1);
         for (int w = 0; w < 4; ++w) bad_rows[w] = 0u;
         fence_barrier_init();
     }
-    if (warp == 9) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(tmem_slot))
+    if (warp == 6) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)),
+                     "n"(L::COLS)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    const Job job = find_job<L::BLOCKS>(rows, list, a);
+    const Job job = find_job(rows, list, a);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -239,151 +247,172 @@ __global__ void __launch_bounds__(kThreads, 1)
     pdl_launch_dependents();
     const int n = job.n;
 
-    if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-        if (warp == 8) {
-            // ---------------- K and V: one lane per half of a block of K or of V
-            constexpr int PER = 2 * L::BLOCKS;
-            const int* table = a.block_table + (size_t)job.slot * a.max_blocks;
-            const int is_v = lane / PER, blk = (lane % PER) >> 1, half = lane & 1;
-            for (int i = 0; i < n; ++i) {
-                const int s = i % L::STAGES, round = i / L::STAGES;
-                int y = a.kv_rows;  // past the end: zeros
-                const int v = (job.t_lo + i) * L::BLOCKS + blk;
-                if (lane < 2 * PER && v < job.span.total) {
-                    const int id = table[job.span.block(v)];
-                    if (id >= 0 && id < a.n_pool_blocks)
-                        y = a.kv_row0 + ((job.head * a.n_pool_blocks + id) * 2 + is_v) * kKvBlock;
-                    else if (a.err) atomicOr(a.err, kErrBadIndex);
-                }
-                bool ok = true;
-                if (round > 0) ok = mbar_wait_bounded(&empty[s], (uint32_t)((round - 1) & 1), a.err);
-                if (!__all_sync(0xFFFFFFFFu, ok)) {
-                    // the copies in flight land before the CTA ends
-                    for (int k = max(0, i - L::STAGES); k < i; ++k) {
-                        mbar_wait_bounded(&full_k[k % L::STAGES], (uint32_t)((k / L::STAGES) & 1), nullptr);
-                        mbar_wait_bounded(&full_v[k % L::STAGES], (uint32_t)((k / L::STAGES) & 1), nullptr);
-                    }
-                    break;
-                }
-                uint8_t* ks = smem + L::Q + s * 2 * L::KV;
-                if (lane == 0) {
-                    mbar_arrive_expect_tx(&full_k[s], L::KV);
-                    mbar_arrive_expect_tx(&full_v[s], L::KV);
-                }
-                __syncwarp();
-                if (lane < 2 * PER)
-                    tma_box(smem_addr(ks + is_v * L::KV + half * L::HALF + blk * (kKvBlock * 128)), &kv_map,
-                            half * kHalfDims, y, is_v ? &full_v[s] : &full_k[s]);
+    if (warp == 4 || warp == 5) {
+        // ---------------- K (warp 4) or V (warp 5): a lane per half of a block
+        const int is_v = warp - 4, stages = is_v ? L::VST : L::KST;
+        uint64_t* full = is_v ? full_v : full_k;
+        uint64_t* empty = is_v ? empty_v : empty_k;
+        uint8_t* ring = smem + (is_v ? L::V : L::K);
+        const int* table = a.block_table + (size_t)job.slot * a.max_blocks;
+        const int v0 = job.t_lo * kTileBlocks, row0 = a.kv_row0 + job.head * a.n_pool_blocks * 2 * kKvBlock + is_v * kKvBlock;
+        // rows of the pool of 32 blocks, a lane each (past the end: zeros), read a chunk ahead
+        auto rows_of = [&](int c) {
+            const int v = v0 + 32 * c + lane;
+            if (v >= job.span.total) return a.kv_rows;
+            const int id = table[job.span.block(v)];
+            if (id >= 0 && id < a.n_pool_blocks) return row0 + id * 2 * kKvBlock;
+            if (a.err) atomicOr(a.err, kErrBadIndex);
+            return a.kv_rows;
+        };
+        constexpr int kChunk = 32 / kTileBlocks;  // tiles of a chunk
+        int now = rows_of(0), next = n > kChunk ? rows_of(1) : 0;
+        const int blk = (lane >> 1) & (kTileBlocks - 1), half = lane & 1;
+        for (int i = 0, s = 0, round = 0; i < n; ++i) {
+            if (i > 0 && i % kChunk == 0) {
+                now = next;
+                if (i + kChunk < n) next = rows_of(i / kChunk + 1);
             }
-        } else if (warp == 9) {
-            asm volatile("bar.sync 1, 288;" ::: "memory");  // Q is in shared memory
-            if (lane == 0) {
-                // ---------------- MMA issuer: S of tile i, then P V of tile i - 1.
-                // MMAs run in issue order, so S(i) overwrites the P of tile i - 2
-                // after it was read.
-                constexpr uint32_t id_s = idesc(TILE, false), id_o = idesc(kD, true);
-                const uint32_t qs = smem_addr(smem);
-                for (int i = 0; i <= n; ++i) {
-                    if (i < n) {
-                        const int s = i % L::STAGES;
-                        if (!mbar_wait_bounded(&full_k[s], (uint32_t)((i / L::STAGES) & 1), a.err)) break;
-                        tc_fence_after();
-                        const uint32_t ks = smem_addr(smem + L::Q + s * 2 * L::KV);
-                        const uint32_t d = tmem + L::S_COL + (i & 1) * L::S_STEP;
-#pragma unroll
-                        for (int t = TERMS - 1; t >= 0; --t)  // the small terms first: fewer roundings at the sum's size
-#pragma unroll
-                            for (int kk = 0; kk < 8; ++kk)
-                                mma_ss(d, sdesc(qs + t * L::QTERM + (kk >> 2) * (kRows * 128) + (kk & 3) * 32, 16),
-                                       sdesc(ks + (kk >> 2) * L::HALF + (kk & 3) * 32, 16), id_s, t < TERMS - 1 || kk);
-                        mma_commit(&s_full[i & 1]);
-                    }
-                    if (i > 0) {
-                        const int j = i - 1, w = j & 1, s = j % L::STAGES;
-                        if (!mbar_wait_bounded(&full_v[s], (uint32_t)((j / L::STAGES) & 1), a.err)) break;
-                        if (!mbar_wait_bounded(&p_full[w], (uint32_t)((j >> 1) & 1), a.err)) break;
-                        tc_fence_after();
-                        const uint32_t vs = smem_addr(smem + L::Q + s * 2 * L::KV + L::KV);
-                        const uint32_t p = tmem + L::S_COL + w * L::S_STEP, d = tmem + L::O_COL + w * kD;
-#pragma unroll
-                        for (int t = TERMS - 1; t >= 0; --t)
-#pragma unroll
-                            for (int kk = 0; kk < TILE / 16; ++kk)
-                                mma_ts(d, p + t * (TILE / 2) + kk * 8, sdesc(vs + kk * 2048, L::HALF), id_o,
-                                       j > 1 || t < TERMS - 1 || kk);
-                        mma_commit(&empty[s]);
-                        if (j + 2 >= n) mma_commit(&o_full[w]);
-                    }
-                }
+            bool ok = true;
+            if (round > 0) ok = mbar_wait_bounded(&empty[s], (uint32_t)((round - 1) & 1), a.err);
+            if (!__all_sync(kAll, ok)) {
+                // the copies in flight land before the CTA ends
+                for (int k = max(0, i - stages); k < i; ++k)
+                    mbar_wait_bounded(&full[k % stages], (uint32_t)((k / stages) & 1), nullptr);
+                break;
             }
+            const int y = __shfl_sync(kAll, now, (i % kChunk) * kTileBlocks + blk);
+            if (lane == 0) mbar_arrive_expect_tx(&full[s], kTileBytes);
             __syncwarp();
+            if (lane < 2 * kTileBlocks)
+                tma_box(smem_addr(ring + s * kTileBytes + half * kHalf + blk * (kKvBlock * 128)), &kv_map, half * kHalfDims, y,
+                        &full[s]);
+            if (++s == stages) {
+                s = 0;
+                ++round;
+            }
         }
-    } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-        // ---------------- softmax: thread = one query row, warpgroup w takes tiles w, w + 2, ..
-        const int w = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
-        const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
-        {
-            // Q: two threads per row, 64 dims each, split into terms
-            const int qr = threadIdx.x >> 1, half = threadIdx.x & 1;
-            const int m = qr >> 1, hh = qr & 1;
-            const bool live = m < job.count;
-            size_t at = 0;
-            if (live) at = (size_t)(list.n ? rows.row[job.first + m] : job.first + m) * a.q_stride +
-                           (size_t)(job.head * kG + hh) * kD + half * kHalfDims;
+    } else if (warp == 6) {
+        asm volatile("bar.sync 1, 160;" ::: "memory");  // Q is in shared memory
+        if (lane == 0) {
+            // ---------------- MMA issuer: S of tile i, then P V of tile i - 1.
+            // MMAs run in issue order, so S(i) overwrites the P of tile i - 2
+            // after it was read.
+            constexpr uint32_t id_s = idesc(TILE, false), id_o = idesc(kD, true);
+            const uint32_t qs = smem_addr(smem);
+            int ks = 0, kround = 0, vs = 0, vround = 0;
+            for (int i = 0; i <= n; ++i) {
+                if (i < n) {
+                    if (!mbar_wait_bounded(&full_k[ks], (uint32_t)(kround & 1), a.err)) break;
+                    tc_fence_after();
+                    const uint32_t k = smem_addr(smem + L::K + ks * kTileBytes);
+                    const uint32_t d = tmem + L::S_COL + (i & 1) * L::S_STEP;
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                uint32_t t[TERMS][4];
-                if constexpr (TERMS == 1) {
-                    uint4 x = make_uint4(0, 0, 0, 0);
-                    if (live) x = __ldcg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + at + 8 * c));
-                    t[0][0] = x.x; t[0][1] = x.y; t[0][2] = x.z; t[0][3] = x.w;
-                } else {
-                    float4 x = make_float4(0, 0, 0, 0), y = x;
-                    if (live) {
-                        x = __ldcg(reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + at + 8 * c));
-                        y = __ldcg(reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + at + 8 * c + 4));
+                    for (int t = TERMS - 1; t >= 0; --t)  // the small terms first: fewer roundings at the sum's size
+#pragma unroll
+                        for (int kk = 0; kk < 8; ++kk)
+                            mma_ss(d, sdesc(qs + t * L::QTERM + (kk >> 2) * (kRows * 128) + (kk & 3) * 32, 16),
+                                   sdesc(k + (kk >> 2) * kHalf + (kk & 3) * 32, 16), id_s, t < TERMS - 1 || kk);
+                    mma_commit(&empty_k[ks]);
+                    mma_commit(&s_full[i & 1]);
+                    if (++ks == L::KST) {
+                        ks = 0;
+                        ++kround;
                     }
-                    const float f[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+                }
+                if (i > 0) {
+                    const int j = i - 1;
+                    if (!mbar_wait_bounded(&full_v[vs], (uint32_t)(vround & 1), a.err)) break;
+                    if (!mbar_wait_bounded(&p_full[j & 1], (uint32_t)((j >> 1) & 1), a.err)) break;
+                    tc_fence_after();
+                    const uint32_t v = smem_addr(smem + L::V + vs * kTileBytes);
+                    const uint32_t p = tmem + L::S_COL + (j & 1) * L::S_STEP;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        uint32_t u[TERMS];
-                        split_pair<TERMS>(f[2 * e], f[2 * e + 1], u);
+                    for (int t = TERMS - 1; t >= 0; --t)
 #pragma unroll
-                        for (int k = 0; k < TERMS; ++k) t[k][e] = u[k];
+                        for (int kk = 0; kk < TILE / 16; ++kk)
+                            mma_ts(tmem, p + t * (TILE / 2) + kk * 8, sdesc(v + kk * 2048, kHalf), id_o,
+                                   j > 0 || t < TERMS - 1 || kk);
+                    mma_commit(&empty_v[vs]);
+                    mma_commit(o_full);
+                    if (i == n) mma_commit(done);
+                    if (++vs == L::VST) {
+                        vs = 0;
+                        ++vround;
+                    }
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp < 4) {
+        // ---------------- softmax: thread = one query row
+        const int r = threadIdx.x;
+        const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
+        {
+            // Q, 16 lanes per row: 8 dims each, split into terms
+            const int c = lane & 15, half = c >> 3;
+            auto place = [&](int qr, int k) {
+                return reinterpret_cast<uint4*>(smem + k * L::QTERM + half * (kRows * 128) + qr * 128 + (((c & 7) ^ (qr & 7)) << 4));
+            };
+            constexpr int kAhead = TERMS == 1 ? 8 : 4;
+#pragma unroll 1
+            for (int g = 0; g < 16; g += kAhead) {
+                float4 x[kAhead][2];
+#pragma unroll
+                for (int e = 0; e < kAhead; ++e) {
+                    const int qr = 8 * (g + e) + 2 * warp + (lane >> 4), m = qr >> 1;
+                    x[e][0] = x[e][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (m < job.count) {
+                        const size_t at = (size_t)(list.n ? rows.row[job.first + m] : job.first + m) * a.q_stride +
+                                          (size_t)(job.head * kG + (qr & 1)) * kD + 8 * c;
+                        if constexpr (TERMS == 1) {
+                            x[e][0] = __ldcg(reinterpret_cast<const float4*>(static_cast<const uint16_t*>(a.q) + at));
+                        } else {
+                            x[e][0] = __ldcg(reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + at));
+                            x[e][1] = __ldcg(reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + at + 4));
+                        }
                     }
                 }
 #pragma unroll
-                for (int k = 0; k < TERMS; ++k)
-                    *reinterpret_cast<uint4*>(smem + k * L::QTERM + half * (kRows * 128) + qr * 128 + ((c ^ (qr & 7)) << 4)) =
-                        make_uint4(t[k][0], t[k][1], t[k][2], t[k][3]);
+                for (int e = 0; e < kAhead; ++e) {
+                    const int qr = 8 * (g + e) + 2 * warp + (lane >> 4);
+                    if constexpr (TERMS == 1) {
+                        *reinterpret_cast<float4*>(place(qr, 0)) = x[e][0];
+                    } else {
+                        uint32_t t[4][TERMS];
+                        split_pair<TERMS>(x[e][0].x, x[e][0].y, t[0]);
+                        split_pair<TERMS>(x[e][0].z, x[e][0].w, t[1]);
+                        split_pair<TERMS>(x[e][1].x, x[e][1].y, t[2]);
+                        split_pair<TERMS>(x[e][1].z, x[e][1].w, t[3]);
+#pragma unroll
+                        for (int k = 0; k < TERMS; ++k) *place(qr, k) = make_uint4(t[0][k], t[1][k], t[2][k], t[3][k]);
+                    }
+                }
             }
             fence_proxy_async_smem();
-            asm volatile("bar.sync 1, 288;" ::: "memory");
+            asm volatile("bar.sync 1, 160;" ::: "memory");
         }
         const int pos = min(job.p0 + (r >> 1), job.p1);  // this row's position (chunk)
-        const int low = window_low(pos, a.window);
+        const int low = window_low(pos, a.window), low1 = window_low(job.p1, a.window);
         const float scale2 = kLog2e / sqrtf((float)kD);
-        const uint32_t s_at = tmem + L::S_COL + w * L::S_STEP + lane_base;
-        const uint32_t o_at = tmem + L::O_COL + w * kD + lane_base;
         float m_ref = -INFINITY, l = 0.0f;  // reference point (log2 units) and sum of the exponentials
         bool alive = true;
-        for (int i = w; i < n; i += 2) {
-            alive = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&s_full[w], (uint32_t)((i >> 1) & 1), a.err));
+#pragma unroll 1
+        for (int i = 0; i < n; ++i) {
+            alive = __all_sync(kAll, mbar_wait_bounded(&s_full[i & 1], (uint32_t)((i >> 1) & 1), a.err));
             if (!alive) break;
             tc_fence_after();
+            const uint32_t s_at = tmem + L::S_COL + (i & 1) * L::S_STEP + lane_base;
             float s[TILE];
-#pragma unroll
-            for (int c = 0; c < TILE; c += 32) tmem_ld32(s_at + c, reinterpret_cast<uint32_t*>(s + c));
+            tmem_ld32(s_at, reinterpret_cast<uint32_t*>(s));
+            tmem_ld32(s_at + 32, reinterpret_cast<uint32_t*>(s + 32));
             tmem_wait_ld();
-            const int v0 = (job.t_lo + i) * L::BLOCKS;
-            const int b0 = job.span.block(v0), b1 = job.span.block(v0 + L::BLOCKS - 1);
-            const bool whole = v0 + L::BLOCKS <= job.span.total && v0 >= job.span.nsb && b1 * kKvBlock + kKvBlock - 1 <= job.p0 &&
-                               (list.n || b0 * kKvBlock >= window_low(job.p1, a.window));
+            const int v0 = (job.t_lo + i) * kTileBlocks;
+            const int b0 = job.span.block(v0), b1 = job.span.block(v0 + kTileBlocks - 1);
+            const bool whole = v0 + kTileBlocks <= job.span.total && v0 >= job.span.nsb &&
+                               b1 * kKvBlock + kKvBlock - 1 <= job.p0 && (list.n || b0 * kKvBlock >= low1);
             if (!whole) {
 #pragma unroll
-                for (int u = 0; u < L::BLOCKS; ++u) {
+                for (int u = 0; u < kTileBlocks; ++u) {
                     const uint32_t bits = v0 + u < job.span.total
                                               ? (list.n ? 0xFFFFu : seen_bits(job.span.block(v0 + u), pos, low, a.sinks))
                                               : 0u;
@@ -401,120 +430,137 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int e = 0; e < 8; ++e) mx[e] = fmaxf(mx[e], fmaxf(s[c + e], s[c + 8 + e]));
             const float mt = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7]))) * scale2;
             const bool grow = mt > m_ref + kLag || (m_ref == -INFINITY && mt > -INFINITY);
-            if (__any_sync(0xFFFFFFFFu, grow)) {
+            if (__any_sync(kAll, grow)) {
                 const float m_new = grow ? mt : m_ref;
                 const float c = grow ? exp2f(m_ref - m_new) : 1.0f;
                 l *= c;
                 m_ref = m_new;
-                if (i > 1) {  // the accumulator holds tiles up to i - 2, whose products are done (S(i) came after them)
-#pragma unroll
+                if (i > 0) {
+                    // the accumulator, once P V of the tile before is done. S(i) came
+                    // after P V of tile i - 2, and that of tile i waits for this warp: o_full
+                    // is in phase i - 1 or i, which its parity tells apart
+                    alive = __all_sync(kAll, mbar_wait_bounded(o_full, (uint32_t)((i - 1) & 1), a.err));
+                    if (!alive) break;
+                    tc_fence_after();
+#pragma unroll 1
                     for (int d = 0; d < kD; d += 32) {
                         uint32_t o[32];
-                        tmem_ld32(o_at + d, o);
+                        tmem_ld32(tmem + lane_base + d, o);
                         tmem_wait_ld();
 #pragma unroll
                         for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * c);
-                        tmem_st32(o_at + d, o);
+                        tmem_st32(tmem + lane_base + d, o);
                     }
                 }
             }
             const float neg = m_ref == -INFINITY ? 0.0f : -m_ref;
             float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            uint32_t p[TERMS][32];
 #pragma unroll
-            for (int c0 = 0; c0 < TILE; c0 += 64) {
-                uint32_t p[TERMS][32];
+            for (int e = 0; e < 32; ++e) {
+                const float x0 = exp2_fast(fmaf(s[2 * e], scale2, neg));
+                const float x1 = exp2_fast(fmaf(s[2 * e + 1], scale2, neg));
+                sum[(2 * e) & 3] += x0;
+                sum[(2 * e + 1) & 3] += x1;
+                uint32_t u[TERMS];
+                split_pair<TERMS>(x0, x1, u);
 #pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                    const float x0 = exp2_fast(fmaf(s[c0 + 2 * e], scale2, neg));
-                    const float x1 = exp2_fast(fmaf(s[c0 + 2 * e + 1], scale2, neg));
-                    sum[(2 * e) & 3] += x0;
-                    sum[(2 * e + 1) & 3] += x1;
-                    uint32_t u[TERMS];
-                    split_pair<TERMS>(x0, x1, u);
-#pragma unroll
-                    for (int k = 0; k < TERMS; ++k) p[k][e] = u[k];
-                }
-#pragma unroll
-                for (int k = 0; k < TERMS; ++k) tmem_st32(s_at + k * (TILE / 2) + c0 / 2, p[k]);
+                for (int k = 0; k < TERMS; ++k) p[k][e] = u[k];
             }
+#pragma unroll
+            for (int k = 0; k < TERMS; ++k) tmem_st32(s_at + k * (TILE / 2), p[k]);
             l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             tmem_wait_st();
             tc_fence_before();
-            mbar_arrive(&p_full[w]);
+            mbar_arrive(&p_full[i & 1]);
         }
-        // ---- join the two warpgroups' parts: maxima and sums through the Q
-        // buffer (its last reader is done), warpgroup w then takes dims 64 w ..
-        for (int k = 0; k < min(n, 2); ++k) alive = __all_sync(0xFFFFFFFFu, alive && mbar_wait_bounded(&o_full[k], 0u, a.err));
+        // ---- the result: through shared memory (Q, K and V are read), so that
+        // whole rows are stored together
+        // (a barrier of its own: o_full may be one or two phases on by now, which its
+        // parity does not tell apart)
+        if (n > 0) alive = __all_sync(kAll, alive && mbar_wait_bounded(done, 0u, a.err));
         tc_fence_after();
-        float2* ml = reinterpret_cast<float2*>(smem);
-        if (alive) ml[w * kRows + r] = make_float2(m_ref, l);
-        asm volatile("bar.sync 2, 256;" ::: "memory");
+        const bool direct = list.n == 0 && job.nseg == 1;
+        const int n_q = a.n_kv * kG;
         if (alive) {
-            const float2 x0 = ml[r], x1 = ml[kRows + r];
-            const float M = fmaxf(x0.x, x1.x);
-            const float c0 = x0.x == -INFINITY ? 0.0f : exp2f(x0.x - M), c1 = x1.x == -INFINITY ? 0.0f : exp2f(x1.x - M);
-            const float lsum = x0.y * c0 + x1.y * c1;
-            const bool live = (r >> 1) < job.count;
-            const bool direct = list.n == 0 && job.nseg == 1;
-            float inv = 1.0f;
-            if (direct) inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
-            bool finite = true;
-            const int member = job.first + (r >> 1), qrow = list.n ? rows.row[live ? member : job.first] : member;
-            const int hq = job.head * kG + (r & 1);
-            float* rec = a.part + (((size_t)member * (a.n_kv * kG) + hq) * a.max_segs + job.seg) * kRecord;
-            if (!direct && live && w == 0) *reinterpret_cast<float2*>(rec) = make_float2(M, lsum);
+            const float inv = !direct ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l);
+            bool finite = fabsf(l) < INFINITY;
+#pragma unroll 1
+            for (int d = 0; d < kD; d += 32) {
+                uint32_t u[32];
+                if (n > 0) tmem_ld32(tmem + lane_base + d, u);
+                else
 #pragma unroll
-            for (int d = 0; d < kHalfDims; d += 32) {
-                __syncwarp();
-                uint32_t u0[32], u1[32];
-                if (n > 0) tmem_ld32(tmem + L::O_COL + lane_base + w * kHalfDims + d, u0);
-                if (n > 1) tmem_ld32(tmem + L::O_COL + kD + lane_base + w * kHalfDims + d, u1);
+                    for (int e = 0; e < 32; ++e) u[e] = 0u;
                 tmem_wait_ld();
                 float o[32];
 #pragma unroll
                 for (int e = 0; e < 32; ++e) {
-                    o[e] = n > 0 ? __uint_as_float(u0[e]) * c0 : 0.0f;
-                    if (n > 1) o[e] += __uint_as_float(u1[e]) * c1;
+                    o[e] = __uint_as_float(u[e]);
                     finite = finite && fabsf(o[e]) < INFINITY;
                     o[e] *= inv;
                 }
-                if (!live) {
-                } else if (!direct) {
-#pragma unroll
-                    for (int e = 0; e < 32; e += 4)
-                        *reinterpret_cast<float4*>(rec + 4 + w * kHalfDims + d + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-                } else if (TERMS == 1) {
-                    uint16_t* op = static_cast<uint16_t*>(a.out) + (size_t)qrow * a.out_stride + (size_t)hq * kD + w * kHalfDims + d;
+                if (TERMS == 1 && direct) {
 #pragma unroll
                     for (int e = 0; e < 32; e += 8)
-                        *reinterpret_cast<uint4*>(op + e) = make_uint4(pack_bf16(o[e], o[e + 1]), pack_bf16(o[e + 2], o[e + 3]),
-                                                                       pack_bf16(o[e + 4], o[e + 5]), pack_bf16(o[e + 6], o[e + 7]));
+                        *reinterpret_cast<uint4*>(smem + r * 256 + ((((d + e) >> 3) ^ (r & 7)) << 4)) =
+                            make_uint4(pack_bf16(o[e], o[e + 1]), pack_bf16(o[e + 2], o[e + 3]), pack_bf16(o[e + 4], o[e + 5]),
+                                       pack_bf16(o[e + 6], o[e + 7]));
                 } else {
-                    float* op = static_cast<float*>(a.out) + (size_t)qrow * a.out_stride + (size_t)hq * kD + w * kHalfDims + d;
 #pragma unroll
                     for (int e = 0; e < 32; e += 4)
-                        *reinterpret_cast<float4*>(op + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                        *reinterpret_cast<float4*>(smem + r * 512 + ((((d + e) >> 2) ^ (r & 7)) << 4)) =
+                            make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
                 }
             }
-            if (live && !(finite && fabsf(lsum) < INFINITY)) atomicOr(&bad_rows[quarter], 1u << lane);
+            if ((r >> 1) < job.count) {
+                if (!finite) atomicOr(&bad_rows[warp], 1u << lane);
+                if (!direct) {
+                    float* rec = a.part + (((size_t)(job.first + (r >> 1)) * n_q + job.head * kG + (r & 1)) * a.max_segs + job.seg) * kRecord;
+                    *reinterpret_cast<float2*>(rec) = make_float2(m_ref, l);
+                }
+            }
+            __syncwarp();
+            // this warp's 32 rows
+            if (TERMS == 1 && direct) {
+#pragma unroll 4
+                for (int g = 0; g < 16; ++g) {
+                    const int qr = 32 * warp + 2 * g + (lane >> 4), c = lane & 15, m = job.first + (qr >> 1);
+                    if ((qr >> 1) < job.count)
+                        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + (size_t)m * a.out_stride +
+                                                  (size_t)(job.head * kG + (qr & 1)) * kD + 8 * c) =
+                            *reinterpret_cast<const uint4*>(smem + qr * 256 + ((c ^ (qr & 7)) << 4));
+                }
+            } else {
+#pragma unroll 4
+                for (int g = 0; g < 32; ++g) {
+                    const int qr = 32 * warp + g, m = job.first + (qr >> 1), hq = job.head * kG + (qr & 1);
+                    const float4 x = *reinterpret_cast<const float4*>(smem + qr * 512 + ((lane ^ (qr & 7)) << 4));
+                    if ((qr >> 1) < job.count) {
+                        float* to = direct ? static_cast<float*>(a.out) + (size_t)m * a.out_stride + (size_t)hq * kD + 4 * lane
+                                           : a.part + (((size_t)m * n_q + hq) * a.max_segs + job.seg) * kRecord + 4 + 4 * lane;
+                        *reinterpret_cast<float4*>(to) = x;
+                    }
+                }
+            }
         }
-        asm volatile("bar.sync 2, 256;" ::: "memory");
+        __syncwarp();
         // rows that are not finite, position by position over this CTA's blocks
-        for (int x = warp; x < kRows; x += 8) {
-            if (!((bad_rows[x >> 5] >> (x & 31)) & 1u)) continue;
+        for (uint32_t bad = bad_rows[warp]; bad; bad &= bad - 1) {
+            const int x = 32 * warp + __ffs(bad) - 1;
             const int m = job.first + (x >> 1), qrow = list.n ? rows.row[m] : m, hq = job.head * kG + (x & 1);
             const int p = list.n ? job.p1 : job.p0 + (x >> 1);
-            SlowRow row = slow_row(a, qrow, hq, job.slot, p, list.n ? 0 : window_low(p, a.window), list.n ? 0 : a.sinks, job.span,
-                                   job.t_lo * L::BLOCKS, min((job.t_lo + n) * L::BLOCKS, job.span.total));
-            if (list.n == 0 && job.nseg == 1) store_row(a, qrow, hq, row);
-            else store_record(a.part + (((size_t)m * (a.n_kv * kG) + hq) * a.max_segs + job.seg) * kRecord, row);
+            const SlowRow row = slow_row(a, qrow, hq, job.slot, p, list.n ? 0 : window_low(p, a.window), list.n ? 0 : a.sinks,
+                                         job.span, job.t_lo * kTileBlocks, min((job.t_lo + n) * kTileBlocks, job.span.total));
+            if (direct) store_row(a, qrow, hq, row);
+            else store_record(a.part + (((size_t)m * n_q + hq) * a.max_segs + job.seg) * kRecord, row);
         }
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 9) {
+    if (warp == 6) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(L::COLS) : "memory");
     }
 }
 

@@ -860,7 +860,7 @@ int plan_shared(ZynferCuCtx* c, uint32_t batch, bool bf16, int* max_segs) {
     for (uint32_t i = 0; i + 1 < batch; ++i)
         common[i] = group[order[i]] == group[order[i + 1]]
                         ? common_blocks(c->seq_blocks[rows.slot[i]], c->seq_blocks[rows.slot[i + 1]]) : 0;
-    const int tile_blocks = attn_tile_blocks(bf16);
+    const int tile_blocks = kAttnTileBlocks;
     long long work = 0;
     for (int g = 0; g < n; ++g)
         cut_runs(common, count[g], count[g + 1], true, [&](int r0, int r1, int d) {
@@ -873,7 +873,8 @@ int plan_shared(ZynferCuCtx* c, uint32_t batch, bool bf16, int* max_segs) {
             }
         });
     const int sms = c->caps.sm_count > 0 ? c->caps.sm_count : 148;
-    const int per = (int)std::max<long long>(2, (work + sms - 1) / sms);
+    const int slots = sms * attn_tile_ctas(bf16);
+    const int per = (int)std::max<long long>(2, (work + slots - 1) / slots);
     int items = 0;
     for (int e = 0; e < list.n; ++e) {
         const int tiles = (list.blocks[e] + tile_blocks - 1) / tile_blocks, split = (tiles + per - 1) / per;

@@ -52,8 +52,9 @@ bool make_tmap_k_major(CUtensorMap* map, const void* base, int wkind, uint64_t k
 // The KV pool as rows of 128 bf16, boxes of 16 rows x half a row, not swizzled
 // (the pool's own swizzle is the MMA's).
 bool make_tmap_kv(CUtensorMap* map, const void* pool, uint64_t rows);
-// attn_tile.cu: `items` = CTAs; cache blocks of a tile of keys
-inline int attn_tile_blocks(bool bf16) { return bf16 ? 8 : 4; }
+// attn_tile.cu: `items` = CTAs; cache blocks of a tile of keys; CTAs that an SM holds
+constexpr int kAttnTileBlocks = 4;
+inline int attn_tile_ctas(bool bf16) { return bf16 ? 2 : 1; }
 void launch_attn_tile(const CUtensorMap& kv_map, const ServeRows& rows, const TileList& list, const ServeAttnArgs& a,
                       int items, cudaStream_t st);
 void launch_prep_planes(const PlanesArgs& a, cudaStream_t st);
