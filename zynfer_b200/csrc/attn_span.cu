@@ -47,6 +47,7 @@ struct Smem {
     uint32_t kidx[kWarps][kIdRing];
     int rec_gid[2][kWarps];
     int pref[kServeMaxBatch + 1];
+    ServeRow info[kServeSmallBatch];  // the rows of a small batch
 };
 static_assert(sizeof(Smem) + 1024 <= 232448, "span attention shared memory");
 
@@ -62,32 +63,24 @@ __device__ __forceinline__ uint32_t term_of(float x0, float x1, int term) {
     return t;
 }
 
-// A merged piece: lane l holds dims 4 l .. 4 l + 3 of both heads.
-struct Piece {
-    float m[kG], l[kG], acc[kG][4];
-};
-__device__ __forceinline__ void clear(Piece& p) {
+// x joined with a record in shared memory.
+__device__ __forceinline__ void join_shared(Partial& x, const float* rec) {
+    const float m = rec[0], l = rec[1];
+    if (m == -INFINITY) return;
+    const float4 v = *reinterpret_cast<const float4*>(rec + 4 + 4 * (threadIdx.x % kWarp));
+    const float mn = fmaxf(x.m, m);
+    const float c0 = x.m == -INFINITY ? 0.0f : exp2_fast(x.m - mn), c1 = exp2_fast(m - mn);
+    x.m = mn;
+    x.l = x.l * c0 + l * c1;
+    const float f[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int h = 0; h < kG; ++h) {
-        p.m[h] = -INFINITY;
-        p.l[h] = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) p.acc[h][e] = 0.0f;
-    }
-}
-__device__ __forceinline__ void join(Piece& p, int h, float m, float l, const float4& x) {
-    const float mn = fmaxf(p.m[h], m);
-    const float c0 = p.m[h] == -INFINITY ? 0.0f : exp2f(p.m[h] - mn), c1 = m == -INFINITY ? 0.0f : exp2f(m - mn);
-    p.m[h] = mn;
-    p.l[h] = p.l[h] * c0 + l * c1;
-    const float f[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) p.acc[h][e] = (c0 == 0.0f ? 0.0f : p.acc[h][e] * c0) + (c1 == 0.0f ? 0.0f : f[e] * c1);
+    for (int e = 0; e < 4; ++e) x.acc[e] = (c0 == 0.0f ? 0.0f : x.acc[e] * c0) + f[e] * c1;
 }
 
 template <int N>
 __global__ void __launch_bounds__(kThreads, 1)
-    attn_span_kernel(const __grid_constant__ ServeRowsT<N> rows, const __grid_constant__ ServeAttnArgs a) {
+    attn_span_kernel(const __grid_constant__ ServeRowsT<N> rows_param, const __grid_constant__ ServeAttnArgs a) {
+    const ServeRowsT<N>& rows = as_memory(rows_param);
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
     const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
@@ -95,14 +88,24 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t* full = sm.full[warp];
     uint32_t* kidx = sm.kidx[warp];
     const int B = a.batch;
-    auto span_row = [&](int b) { return span_of(rows.len[b] - 1, rows.len[b] - 1, a.window, a.sinks, rows.skip[b]); };
+    auto info = [&](int b) {
+        const int4 x = *reinterpret_cast<const int4*>(N <= kServeSmallBatch ? &sm.info[b] : &rows.r[b]);
+        return ServeRow{x.x, x.y, x.z, (uint32_t)x.w};
+    };
+    auto span_row = [&](const ServeRow& r) { return span_of(r.len - 1, r.len - 1, a.window, a.sinks, r.skip()); };
 
     // prefix of the rows' block counts; a row that sees nothing here counts one
     if (warp == 0) {
         int carry = 0;
         for (int base = 0; base < B; base += kWarp) {
             const int b = base + lane;
-            int x = b < B ? max(1, span_row(b).total) : 0;
+            int x = 0;
+            if (b < B) {
+                const int4 w = *reinterpret_cast<const int4*>(&rows.r[b]);
+                const ServeRow r{w.x, w.y, w.z, (uint32_t)w.w};
+                if (N <= kServeSmallBatch) sm.info[b] = r;
+                x = max(1, span_row(r).total);
+            }
 #pragma unroll
             for (int o = 1; o < kWarp; o <<= 1) {
                 const int y = __shfl_up_sync(kAll, x, o);
@@ -158,10 +161,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (j < n) {
             Cursor x;
             locate(lo + j, x);
-            const Span span = span_row(x.b);
+            const ServeRow r = info(x.b);
+            const Span span = span_row(r);
             int id = 0;  // a row that sees nothing reads some block and weighs none of it
             if (x.blk < span.total) {
-                id = a.block_table[(size_t)rows.slot[x.b] * a.max_blocks + span.block(x.blk)];
+                id = a.block_table[(size_t)r.slot * a.max_blocks + span.block(x.blk)];
                 if (id < 0 || id >= a.n_pool_blocks) {
                     if (a.err) atomicOr(a.err, kErrBadIndex);
                     id = 0;
@@ -177,22 +181,42 @@ __global__ void __launch_bounds__(kThreads, 1)
                       l2_evict_first_policy());
     };
 
+    const int g = lane >> 2, t = lane & 3;
+    const int mi = lane >> 3, ri = lane & 7;
+    const int tok_a = ri + (mi & 1) * 8;             // row this lane addresses for ldmatrix
+    const int hsel = (g >> 1) & 1, term = (g & 4) ? ((g & 1) ? 3 : 2) : (g & 1);  // head and term of row / column g (3: none)
+    const float scale2 = kLog2e / sqrtf((float)kD);
+
+    // this lane's values of a row's query: dims 16 ks + 8 hf + 2 t, + 1 of head hsel
+    float2 qv[8][2];
+    auto load_q = [&](int row, int head) {
+        const size_t at = (size_t)row * a.q_stride + (size_t)(head * kG + hsel) * kD + 2 * t;
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks)
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+                const size_t x = at + 16 * ks + 8 * hf;
+                if (a.bf16) {
+                    const uint32_t two = __ldcg(reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(a.q) + x));
+                    qv[ks][hf] = make_float2(bf16lo(two), bf16hi(two));
+                } else {
+                    qv[ks][hf] = __ldcg(reinterpret_cast<const float2*>(static_cast<const float*>(a.q) + x));
+                }
+            }
+    };
+
     // The cache was written by earlier kernels. After a tile kernel (which
     // waited for those before it let this one start) it may be read at once;
     // the tile's records and the buffers are touched after the wait below.
     if (!a.early) pdl_wait();
     Cursor cc;
     locate(lo, cc);
+    ServeRow cur = info(cc.b);
+    if (n > 0) load_q(cur.row, cc.head);  // in front of the blocks, not behind them
     fill_chunk(0);
     if (lane == 0)
         for (int j = 0; j < min(kRing, n); ++j) issue(j, j);
     pdl_launch_dependents();
-
-    const int g = lane >> 2, t = lane & 3;
-    const int mi = lane >> 3, ri = lane & 7;
-    const int tok_a = ri + (mi & 1) * 8;             // row this lane addresses for ldmatrix
-    const int hsel = (g >> 1) & 1, term = (g & 4) ? ((g & 1) ? 3 : 2) : (g & 1);  // head and term of row / column g (3: none)
-    const float scale2 = kLog2e / sqrtf((float)kD);
 
     uint32_t qf[8][2];
     float acc[16][4];
@@ -201,22 +225,23 @@ __global__ void __launch_bounds__(kThreads, 1)
     Span span{};
     bool seg_start = true;
 
-    auto run_blocks = [&](int i, auto nb_c) -> bool {
-        constexpr int NB = decltype(nb_c)::value;
+    // blocks i and, if nb is 2, i + 1 of the share, both of one (row, kv head); a
+    // lone block is taken twice, the second time with no position seen
+    auto run_blocks = [&](int i, int nb) -> bool {
+        constexpr int NB = 2;
         bool ok = true;
-#pragma unroll
-        for (int u = 0; u < NB; ++u)
+        for (int u = 0; u < nb; ++u)
             ok = mbar_wait_bounded(&full[(i + u) % kRing], (uint32_t)(((i + u) / kRing) & 1), a.err) && ok;
         if (!__all_sync(kAll, ok)) return false;
         uint32_t kbase[NB], bits[NB];
         bool patched = false;
 #pragma unroll
         for (int u = 0; u < NB; ++u) {
-            unsigned char* kb = ring + ((i + u) % kRing) * kSlotBytes;
+            unsigned char* kb = ring + ((i + (u < nb ? u : 0)) % kRing) * kSlotBytes;
             kbase[u] = smem_addr(kb);
             const int v = cc.blk + u;
-            bits[u] = v < span.total ? seen_bits(span.block(v), pos, low, a.sinks) : 0u;
-            if (bits[u] != 0xFFFFu) {
+            bits[u] = u < nb && v < span.total ? seen_bits(span.block(v), pos, low, a.sinks) : 0u;
+            if (u < nb && bits[u] != 0xFFFFu) {
                 // positions that are not seen: p = 0 there, but 0 times a NaN that lies there is NaN
                 for (int x = lane; x < kKvBlock * (kD * 2 / 16); x += kWarp)
                     if (!((bits[u] >> (x / 16)) & 1u)) reinterpret_cast<uint4*>(kb + kBlockBytes)[x] = make_uint4(0, 0, 0, 0);
@@ -294,8 +319,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (patched) fence_proxy_async_smem();  // generic writes above, bulk copy next
         __syncwarp();
-#pragma unroll
-        for (int u = 0; u < NB; ++u) {
+        for (int u = 0; u < nb; ++u) {
             const int jn = i + u + kRing;
             if (jn < n && jn % kWarp == 0) fill_chunk(jn / kWarp);
             if (lane == 0 && jn < n) issue(jn, (i + u) % kRing);
@@ -303,49 +327,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         return true;
     };
 
-    // the first `cnt` global records of (row, kv head) into x, kAhead requested at a time
-    auto join_global = [&](Piece& x, int b, int head, int cnt) {
-        const float* base = a.part + ((size_t)b * (a.n_kv * kG) + head * kG) * a.max_segs * kRecord;
-        const size_t head_step = (size_t)a.max_segs * kRecord;
-        constexpr int kAhead = 4;
-        for (int j0 = 0; j0 < cnt; j0 += kAhead) {
-            float2 ml[kAhead][kG];
-            float4 v[kAhead][kG];
-#pragma unroll
-            for (int j = 0; j < kAhead; ++j)
-#pragma unroll
-                for (int h = 0; h < kG; ++h) {
-                    const float* r = base + h * head_step + (size_t)min(j0 + j, cnt - 1) * kRecord;
-                    ml[j][h] = __ldcg(reinterpret_cast<const float2*>(r));
-                    v[j][h] = __ldcg(reinterpret_cast<const float4*>(r + 4 + 4 * lane));
-                }
-#pragma unroll
-            for (int j = 0; j < kAhead; ++j)
-                if (j0 + j < cnt)
-#pragma unroll
-                    for (int h = 0; h < kG; ++h) join(x, h, ml[j][h].x, ml[j][h].y, v[j][h]);
-        }
-    };
     bool waited = !a.early;
     for (int i = 0; i < n;) {
         if (seg_start) {
             // this row's query as the B operand: column g holds term(g) of head hsel(g)
-            pos = rows.len[cc.b] - 1;
+            if (i > 0) {
+                cur = info(cc.b);
+                load_q(cur.row, cc.head);
+            }
+            pos = cur.len - 1;
             low = window_low(pos, a.window);
-            span = span_row(cc.b);
-            const size_t at = (size_t)rows.row[cc.b] * a.q_stride + (size_t)(cc.head * kG + hsel) * kD + 2 * t;
+            span = span_row(cur);
 #pragma unroll
             for (int ks = 0; ks < 8; ++ks)
 #pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    const size_t x = at + 16 * ks + 8 * hf;
-                    if (a.bf16) {
-                        qf[ks][hf] = term == 0 ? __ldcg(reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(a.q) + x)) : 0u;
-                    } else {
-                        const float2 q2 = __ldcg(reinterpret_cast<const float2*>(static_cast<const float*>(a.q) + x));
-                        qf[ks][hf] = term < 3 ? term_of(q2.x, q2.y, term) : 0u;
-                    }
-                }
+                for (int hf = 0; hf < 2; ++hf) qf[ks][hf] = term < 3 ? term_of(qv[ks][hf].x, qv[ks][hf].y, term) : 0u;
 #pragma unroll
             for (int nt = 0; nt < 16; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.0f;
             m_run = -INFINITY;
@@ -353,8 +349,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             seg_start = false;
         }
         const int nb = (i + 1 < n && cc.blk + 1 < cc.nblk) ? 2 : 1;
-        const bool ok = nb == 2 ? run_blocks(i, std::integral_constant<int, 2>{}) : run_blocks(i, std::integral_constant<int, 1>{});
-        if (!ok) {
+        if (!run_blocks(i, nb)) {
             // the copies in flight land before the warp stops; the error word reports the launch
             if (lane == 0)
                 for (int j = i; j < min(n, i + kRing); ++j)
@@ -382,14 +377,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool writer = (g & 5) == 0 && g < 4;
             const long long f0 = (long long)a.n_kv * pref[cc.b] + (long long)cc.head * cc.nblk;
             const bool whole = f0 >= lo && f0 + cc.nblk <= lo + n;
-            const int nrec = rows.nrec[cc.b];
+            const int nrec = cur.nrec();
             if (whole && !waited) {
                 pdl_wait();
                 waited = true;
             }
             if (whole && nrec == 0) {
                 if (writer) {
-                    const size_t at = (size_t)rows.row[cc.b] * a.out_stride + (size_t)(cc.head * kG + hsel) * kD + 2 * t;
+                    const size_t at = (size_t)cur.row * a.out_stride + (size_t)(cc.head * kG + hsel) * kD + 2 * t;
                     const float inv = Lh == 0.0f ? 0.0f : 1.0f / Lh;
 #pragma unroll
                     for (int nt = 0; nt < 16; ++nt) {
@@ -409,15 +404,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 if (whole) {  // all of the row's own part: with its prompt's records at once
                     __syncwarp();
-                    Piece x;
-                    clear(x);
-                    const float* r = sm.rec[1][warp];
-#pragma unroll
-                    for (int h = 0; h < kG; ++h)
-                        join(x, h, r[h * kRecord], r[h * kRecord + 1], *reinterpret_cast<const float4*>(r + h * kRecord + 4 + 4 * lane));
-                    join_global(x, cc.b, cc.head, nrec);
-#pragma unroll
-                    for (int h = 0; h < kG; ++h) store_out4(a, rows.row[cc.b], cc.head * kG + h, x.acc[h], x.l[h]);
+#pragma unroll 1
+                    for (int h = 0; h < kG; ++h) {
+                        const int hq = cc.head * kG + h;
+                        Partial x = no_partial();
+                        join_shared(x, sm.rec[1][warp] + h * kRecord);
+                        join_records(x, a.part + ((size_t)cc.b * (a.n_kv * kG) + hq) * a.max_segs * kRecord, nrec);
+                        store_out4(a, cur.row, hq, x.acc, x.l);
+                    }
                     __syncwarp();
                 } else if (lane == 0) {
                     sm.rec_gid[k][warp] = cc.b * a.n_kv + cc.head;
@@ -430,65 +424,52 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (!waited) pdl_wait();
 
     // ---- join the warps' records of each (row, kv head) of this CTA, in warp
-    // order; a row that goes on in other CTAs, or has a common prompt, through
-    // the global records
+    // order, a warp per query head; a row that goes on in other CTAs, or has a
+    // common prompt, through the global records
     __syncthreads();
     Cursor gc;
     locate(c_lo, gc);
     long long g0 = (long long)a.n_kv * pref[gc.b] + (long long)gc.head * gc.nblk;
+#pragma unroll 1
     for (int gi = 0; g0 < c_hi; ++gi) {
         const long long g1 = g0 + gc.nblk;
-        const int gb = gc.b, gh = gc.head, nrec = rows.nrec[gb];
-        if (gi % kWarps == warp) {
-            const int wa = (int)(max(0ll, g0 - c_lo) / per), wb = (int)min((long long)kWarps - 1, (g1 - 1 - c_lo) / per);
-            const long long lo_a = c_lo + (long long)wa * per;
-            if (!(wa == wb && g0 >= lo_a && g1 <= lo_a + per)) {  // else its warp stored it
-                Piece x;
-                clear(x);
-                for (int w = wa; w <= wb; ++w) {
-                    const int k = g0 >= c_lo + (long long)w * per ? 1 : 0;
-                    if (sm.rec_gid[k][w] != gb * a.n_kv + gh) continue;  // a warp that stopped early
-                    const float* r = sm.rec[k][w];
-#pragma unroll
-                    for (int h = 0; h < kG; ++h)
-                        join(x, h, r[h * kRecord], r[h * kRecord + 1], *reinterpret_cast<const float4*>(r + h * kRecord + 4 + 4 * lane));
+        const int gb = gc.b, gh = gc.head;
+        const int wa = (int)(max(0ll, g0 - c_lo) / per), wb = (int)min((long long)kWarps - 1, (g1 - 1 - c_lo) / per);
+        const long long lo_a = c_lo + (long long)wa * per;
+        const int h = (warp - 2 * gi) & (kWarps - 1);  // warps 2 gi, 2 gi + 1 (mod 8) take the two heads
+        if (h < kG && !(wa == wb && g0 >= lo_a && g1 <= lo_a + per)) {  // (else its warp stored it)
+            const ServeRow r = info(gb);
+            const int nrec = r.nrec(), hq = gh * kG + h;
+            Partial x = no_partial();
+            for (int w = wa; w <= wb; ++w) {
+                const int k = g0 >= c_lo + (long long)w * per ? 1 : 0;
+                if (sm.rec_gid[k][w] == gb * a.n_kv + gh) join_shared(x, sm.rec[k][w] + h * kRecord);  // (else it stopped early)
+            }
+            const long long reach = (long long)kWarps * per;
+            const int first = (int)(g0 / reach), nown = (int)((g1 - 1) / reach) - first + 1, seg = (int)blockIdx.x - first;
+            float* base = a.part + ((size_t)gb * (a.n_kv * kG) + hq) * a.max_segs * kRecord;
+            bool last = true;
+            if (nrec + nown > a.max_segs) {
+                if (lane == 0 && a.err) atomicOr(a.err, kErrBadIndex);
+                last = false;
+            } else if (nown > 1) {
+                store_record(base + (size_t)(nrec + seg) * kRecord, x);
+                __threadfence();
+                __syncwarp();
+                unsigned prev = 0;
+                unsigned* counter = a.counters + (size_t)gb * (a.n_kv * kG) + hq;
+                if (lane == 0) {
+                    prev = atomicAdd(counter, 1u);
+                    if (prev == (unsigned)(nown - 1)) *counter = 0u;
                 }
-                const long long reach = (long long)kWarps * per;
-                const int first = (int)(g0 / reach), nown = (int)((g1 - 1) / reach) - first + 1, seg = (int)blockIdx.x - first;
-                bool store = nown == 1 && nrec == 0;
-                if (!store && nrec + nown <= a.max_segs) {
-                    float* base = a.part + ((size_t)gb * (a.n_kv * kG) + gh * kG) * a.max_segs * kRecord;
-                    const size_t head_step = (size_t)a.max_segs * kRecord;
-                    bool last = true;
-                    if (nown > 1) {
-#pragma unroll
-                        for (int h = 0; h < kG; ++h) {
-                            float* r = base + h * head_step + (size_t)(nrec + seg) * kRecord;
-                            if (lane == 0) *reinterpret_cast<float2*>(r) = make_float2(x.m[h], x.l[h]);
-                            *reinterpret_cast<float4*>(r + 4 + 4 * lane) = make_float4(x.acc[h][0], x.acc[h][1], x.acc[h][2], x.acc[h][3]);
-                        }
-                        __threadfence();
-                        __syncwarp();
-                        unsigned prev = 0;
-                        unsigned* counter = a.counters + (size_t)gb * a.n_kv + gh;
-                        if (lane == 0) prev = atomicAdd(counter, 1u);
-                        prev = __shfl_sync(kAll, prev, 0);
-                        last = prev == (unsigned)(nown - 1);
-                        if (last && lane == 0) *counter = 0u;
-                        __threadfence();
-                        if (last) clear(x);
-                    }
-                    if (last) {
-                        // every record: the prompt's, then (if this row crosses CTAs) the CTAs' in order
-                        join_global(x, gb, gh, nown > 1 ? nrec + nown : nrec);
-                        store = true;
-                    }
-                } else if (!store && lane == 0 && a.err) {
-                    atomicOr(a.err, kErrBadIndex);
-                }
-                if (store)
-#pragma unroll
-                    for (int h = 0; h < kG; ++h) store_out4(a, rows.row[gb], gh * kG + h, x.acc[h], x.l[h]);
+                last = __shfl_sync(kAll, prev, 0) == (unsigned)(nown - 1);
+                __threadfence();
+                x = no_partial();
+            }
+            if (last) {
+                // every record: the prompt's, then (if this row crosses CTAs) the CTAs' in order
+                join_records(x, base, nown > 1 ? nrec + nown : nrec);
+                store_out4(a, r.row, hq, x.acc, x.l);
             }
         }
         g0 = g1;

@@ -154,8 +154,8 @@ __device__ __forceinline__ Job find_job(const ServeRowsT<N>& rows, const TileLis
         const int b = x % a.batch, ti = per_seq - 1 - x / a.batch;
         j.first = b * a.tokens + ti * kMembers;
         j.count = min(kMembers, a.tokens - ti * kMembers);
-        j.slot = rows.slot[b];
-        j.p0 = rows.len[b] - a.tokens + ti * kMembers;
+        j.slot = rows.r[b].slot;
+        j.p0 = rows.r[b].len - a.tokens + ti * kMembers;
         j.p1 = j.p0 + j.count - 1;
         j.span = span_of(j.p0, j.p1, a.window, a.sinks, 0);
     } else {
@@ -171,7 +171,7 @@ __device__ __forceinline__ Job find_job(const ServeRowsT<N>& rows, const TileLis
         j.nseg = (list.item0[lo + 1] - list.item0[lo]) / a.n_kv;
         j.first = list.first[lo];
         j.count = list.count[lo];
-        j.slot = rows.slot[j.first];
+        j.slot = rows.r[j.first].slot;
         j.p0 = j.p1 = list.blocks[lo] * kKvBlock - 1;  // every row sees every position of the common blocks
         j.span = Span{0, 0, list.blocks[lo]};
     }
@@ -362,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, Lay<TERMS>::CTAS)
                     const int qr = 8 * (g + e) + 2 * warp + (lane >> 4), m = qr >> 1;
                     x[e][0] = x[e][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                     if (m < job.count) {
-                        const size_t at = (size_t)(list.n ? rows.row[job.first + m] : job.first + m) * a.q_stride +
+                        const size_t at = (size_t)(list.n ? rows.r[job.first + m].row : job.first + m) * a.q_stride +
                                           (size_t)(job.head * kG + (qr & 1)) * kD + 8 * c;
                         if constexpr (TERMS == 1) {
                             x[e][0] = __ldcg(reinterpret_cast<const float4*>(static_cast<const uint16_t*>(a.q) + at));
@@ -548,7 +548,7 @@ __global__ void __launch_bounds__(kThreads, Lay<TERMS>::CTAS)
         // rows that are not finite, position by position over this CTA's blocks
         for (uint32_t bad = bad_rows[warp]; bad; bad &= bad - 1) {
             const int x = 32 * warp + __ffs(bad) - 1;
-            const int m = job.first + (x >> 1), qrow = list.n ? rows.row[m] : m, hq = job.head * kG + (x & 1);
+            const int m = job.first + (x >> 1), qrow = list.n ? rows.r[m].row : m, hq = job.head * kG + (x & 1);
             const int p = list.n ? job.p1 : job.p0 + (x >> 1);
             const SlowRow row = slow_row(a, qrow, hq, job.slot, p, list.n ? 0 : window_low(p, a.window), list.n ? 0 : a.sinks,
                                          job.span, job.t_lo * kTileBlocks, min((job.t_lo + n) * kTileBlocks, job.span.total));

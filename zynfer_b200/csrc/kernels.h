@@ -163,13 +163,23 @@ constexpr int kServeMaxBatch = 1024;
 constexpr int kServeRecord = 132;  // words of a partial result: m, l, -, -, acc[128]
 // Kernel parameters cost about 0.1 us of the launch per KB, so the kernels are
 // built for small batches and for the largest (N rows).
+struct alignas(16) ServeRow {
+    int slot;      // sequence slot (block-table row)
+    int len;       // cached positions, the queries' own among them
+    int row;       // row of q and out (one query per sequence)
+    uint32_t own;  // leading blocks that the row's tile takes << 10 | partial results that it leaves
+#ifdef __CUDACC__
+    __host__ __device__
+#endif
+    int skip() const { return (int)(own >> 10); }
+#ifdef __CUDACC__
+    __host__ __device__
+#endif
+    int nrec() const { return (int)(own & 1023u); }
+};
 template <int N>
 struct ServeRowsT {
-    int slot[N];  // sequence slot (block-table row)
-    int len[N];   // cached positions, the queries' own among them
-    int row[N];   // row of q and out (one query per sequence)
-    int skip[N];  // leading blocks that the row's tile takes
-    int nrec[N];  // partial results that the tile leaves
+    ServeRow r[N];
 };
 // Rows that share leading blocks, in tiles of up to 64.
 template <int N>
@@ -197,7 +207,7 @@ struct ServeAttnArgs {
     int nsplit;                // chunk: CTAs that share a tile's blocks
     float* part;               // [row][n_q][max_segs][kServeRecord]
     int max_segs;
-    unsigned* counters;        // [row][n_kv], zero between launches
+    unsigned* counters;        // [row][n_q], zero between launches
     int min_per;               // span kernel: blocks a warp takes at least
     int early;                 // span kernel: launched behind a tile kernel
     uint32_t* err;
@@ -211,18 +221,12 @@ void launch_attn_span(const ServeRows& rows, const ServeAttnArgs& a, int ctas, c
 // The first rows of a batch of at most kServeSmallBatch.
 inline ServeRowsT<kServeSmallBatch> small_rows(const ServeRows& r) {
     ServeRowsT<kServeSmallBatch> s;
-    for (int i = 0; i < kServeSmallBatch; ++i) {
-        s.slot[i] = r.slot[i];
-        s.len[i] = r.len[i];
-        s.row[i] = r.row[i];
-        s.skip[i] = r.skip[i];
-        s.nrec[i] = r.nrec[i];
-    }
+    for (int i = 0; i < kServeSmallBatch; ++i) s.r[i] = r.r[i];
     return s;
 }
 // Cache blocks that a query at `pos` sees after the first `skip`.
 int serve_span_blocks(int pos, uint32_t window, int sinks, int skip);
-void launch_serve_merge(const ServeRows& rows, const ServeAttnArgs& a, cudaStream_t st);
+void launch_serve_merge(const ServeAttnArgs& a, cudaStream_t st);
 struct KvWriteArgs {
     uint16_t* kv_layer;
     const int* table_row;      // the sequence's device block-table row

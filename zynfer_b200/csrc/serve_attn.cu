@@ -16,41 +16,17 @@ namespace {
 
 using namespace serve;
 
-// The records of a (row, query head) joined: o = sum acc 2^(m - M) / sum l 2^(m - M).
-// A warp per (row, query head); rows with one partial result wrote the output.
-__global__ void __launch_bounds__(128) serve_merge_kernel(const __grid_constant__ ServeRows rows,
-                                                          const __grid_constant__ ServeAttnArgs a) {
+// The records of a chunk's (row, query head) joined: a warp each.
+__global__ void __launch_bounds__(128) serve_merge_kernel(const __grid_constant__ ServeAttnArgs a) {
     pdl_wait();
     pdl_launch_dependents();
-    const int n_q = a.n_kv * kG, lane = threadIdx.x % kWarp;
+    const int n_q = a.n_kv * kG;
     const long long w = ((long long)blockIdx.x * blockDim.x + threadIdx.x) / kWarp;
     if (w >= (long long)a.batch * a.tokens * n_q) return;
-    const int hq = (int)(w % n_q);
-    const int qi = (int)(w / n_q);
-    int n = a.nsplit, qrow = qi;
-    if (a.tokens == 1) {
-        qrow = rows.row[qi];
-        if (a.nsplit <= 1) n = rows.nrec[qi] + 1;
-    }
-    if (n == 1) return;
-    const float* rec = a.part + ((size_t)qi * n_q + hq) * a.max_segs * kRecord;
-    float M = -INFINITY;
-    for (int i = lane; i < n; i += kWarp) M = fmaxf(M, __ldcg(rec + (size_t)i * kRecord));
-    M = warp_max(M);
-    float l = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-        const float2 ml = __ldcg(reinterpret_cast<const float2*>(rec + (size_t)i * kRecord));
-        const float4 x = __ldcg(reinterpret_cast<const float4*>(rec + (size_t)i * kRecord + 4 + 4 * lane));
-        if (ml.x == -INFINITY) continue;
-        const float c = exp2f(ml.x - M);
-        l += ml.y * c;
-        acc[0] += x.x * c;
-        acc[1] += x.y * c;
-        acc[2] += x.z * c;
-        acc[3] += x.w * c;
-    }
-    store_out4(a, qrow, hq, acc, l);
+    const int hq = (int)(w % n_q), row = (int)(w / n_q);
+    Partial x = no_partial();
+    join_records(x, a.part + ((size_t)row * n_q + hq) * a.max_segs * kRecord, a.nsplit);
+    store_out4(a, row, hq, x.acc, x.l);
 }
 
 // K and V rows [n_kv][n][128] (f32 rounded to nearest even, or bf16) into
@@ -91,9 +67,9 @@ __global__ void __launch_bounds__(256) kv_write_kernel(KvWriteArgs a) {
 
 int serve_span_blocks(int pos, uint32_t window, int sinks, int skip) { return span_of(pos, pos, window, sinks, skip).total; }
 
-void launch_serve_merge(const ServeRows& rows, const ServeAttnArgs& a, cudaStream_t st) {
+void launch_serve_merge(const ServeAttnArgs& a, cudaStream_t st) {
     const long long warps = (long long)a.batch * a.tokens * a.n_kv * kG;
-    launch_pdl(serve_merge_kernel, (unsigned)((warps + 3) / 4), 128, 0, st, rows, a);
+    launch_pdl(serve_merge_kernel, (unsigned)((warps + 3) / 4), 128, 0, st, a);
 }
 
 void launch_kv_write(const KvWriteArgs& a, cudaStream_t st) {

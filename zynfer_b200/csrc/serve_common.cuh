@@ -17,6 +17,15 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kRecord = kServeRecord;
 static_assert(kRecord == kD + 4, "record: m, l, -, -, acc");
 
+// A kernel parameter as ordinary memory: indexed by lane, constant-bank loads
+// would be taken one index after another.
+template <typename T>
+__device__ __forceinline__ const T& as_memory(const T& param) {
+    const T* p = &param;
+    asm volatile("" : "+l"(p));
+    return *p;
+}
+
 // First position inside the window of a query at `pos` (pos + 1: none).
 __host__ __device__ __forceinline__ int window_low(int pos, uint32_t window) {
     const long long low = (long long)pos - (long long)window + 1;
@@ -60,11 +69,58 @@ __device__ __forceinline__ uint32_t pack_bf16(float x0, float x1) {
 }
 __device__ __forceinline__ void fence_proxy_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// One query head over blocks [v0, v1) of its span, a warp together: lane l
-// holds dims 4 l .. 4 l + 3. Positions that are not seen are not read.
-struct SlowRow {
+// A partial result of one query head held by a warp: lane l has dims 4 l ..
+// 4 l + 3.
+struct Partial {
     float m, l, acc[4];
 };
+using SlowRow = Partial;
+__device__ __forceinline__ Partial no_partial() { return Partial{-INFINITY, 0.0f, {0.0f, 0.0f, 0.0f, 0.0f}}; }
+
+// x joined with `cnt` records in global memory, in order: 2^(m - M) weighs each.
+// Lane j reads the (m, l) of record j and weighs it, so a batch of up to 32
+// costs one exponential and, with kAhead accumulators requested before any is
+// used, about cnt / kAhead round trips.
+__device__ __forceinline__ void join_records(Partial& x, const float* base, int cnt) {
+    const int lane = threadIdx.x % kWarp;
+    constexpr int kAhead = 8;
+    for (int j0 = 0; j0 < cnt; j0 += kWarp) {
+        const int some = min(kWarp, cnt - j0);
+        const float* rec = base + (size_t)j0 * kRecord;
+        float2 ml = make_float2(-INFINITY, 0.0f);
+        if (lane < some) ml = __ldcg(reinterpret_cast<const float2*>(rec + (size_t)lane * kRecord));
+        float c = 0.0f;
+#pragma unroll 1
+        for (int i = 0; i < some; i += kAhead) {
+            float4 v[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k)
+                v[k] = __ldcg(reinterpret_cast<const float4*>(rec + (size_t)min(i + k, some - 1) * kRecord + 4 + 4 * lane));
+            if (i == 0) {
+                const float M = fmaxf(x.m, warp_max(ml.x));
+                c = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - M);
+                const float cx = x.m == -INFINITY ? 0.0f : exp2_fast(x.m - M);
+                x.m = M;
+                x.l = (cx == 0.0f ? 0.0f : x.l * cx) + warp_sum(c == 0.0f ? 0.0f : ml.y * c);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x.acc[e] = cx == 0.0f ? 0.0f : x.acc[e] * cx;
+            }
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                const float ck = __shfl_sync(0xFFFFFFFFu, c, (i + k) & (kWarp - 1));
+                if (i + k < some && ck != 0.0f) {
+                    x.acc[0] += v[k].x * ck;
+                    x.acc[1] += v[k].y * ck;
+                    x.acc[2] += v[k].z * ck;
+                    x.acc[3] += v[k].w * ck;
+                }
+            }
+        }
+    }
+}
+
+// One query head over blocks [v0, v1) of its span, a warp together: lane l
+// holds dims 4 l .. 4 l + 3. Positions that are not seen are not read.
 __device__ __forceinline__ SlowRow slow_row(const ServeAttnArgs& a, int qrow, int hq, int slot, int pos, int low,
                                             int sinks, const Span& span, int v0, int v1) {
     const int lane = threadIdx.x % kWarp, head = hq / kG;

@@ -145,6 +145,7 @@ struct ZynferCuCtx {
     CUtensorMap tm_kv;                  // the KV pool (serving attention)
     float* serve_part = nullptr;        // its partial results
     size_t serve_part_words = 0;
+    unsigned* serve_cnt = nullptr;      // [max_batch][n_q] arrival counters, zero between launches
     std::vector<int> serve_mark;        // [pool blocks] scratch of plan_shared: group of a first block, -1
     ServeRows serve_rows;               // the batch of the call (host)
     TileList serve_tiles;
@@ -348,6 +349,7 @@ int check_device_error(ZynferCuCtx* c) {
     if (!e) return ZYNFER_CU_OK;
     cudaMemsetAsync(c->derr, 0, 4, c->stream);
     cudaMemsetAsync(c->dcnt, 0, (size_t)c->d.max_batch * c->d.n_kv * 4, c->stream);
+    cudaMemsetAsync(c->serve_cnt, 0, (size_t)c->d.max_batch * c->d.n_q * 4, c->stream);
     if (c->psync) cudaMemsetAsync(c->psync, 0, 3 * sizeof(unsigned), c->stream);
     cudaMemsetAsync(c->dkeys, 0, (size_t)c->d.max_batch * 8, c->stream);
     cudaStreamSynchronize(c->stream);
@@ -767,10 +769,7 @@ int serve_batch(ZynferCuCtx* c, const uint32_t* seqs, uint32_t batch, uint32_t t
         if (seqs[i] >= c->d.max_seqs) return fail(c, ZYNFER_CU_INVALID, "sequence id out of range");
         if (c->seq_len[seqs[i]] + extra < tokens)
             return fail(c, ZYNFER_CU_INVALID, "a sequence is shorter than the queries' positions");
-        rows.slot[i] = (int)seqs[i];
-        rows.len[i] = (int)(c->seq_len[seqs[i]] + extra);
-        rows.row[i] = (int)i;
-        rows.skip[i] = rows.nrec[i] = 0;
+        rows.r[i] = ServeRow{(int)seqs[i], (int)(c->seq_len[seqs[i]] + extra), (int)i, 0u};
     }
     return ZYNFER_CU_OK;
 }
@@ -838,28 +837,23 @@ int plan_shared(ZynferCuCtx* c, uint32_t batch, bool bf16, int* max_segs) {
     // counting sort by first block
     int group[kServeMaxBatch], count[kServeMaxBatch + 1] = {0}, at[kServeMaxBatch], n = 0;
     for (uint32_t i = 0; i < batch; ++i) {
-        int& mark = c->serve_mark[c->seq_blocks[rows.slot[i]][0]];
+        int& mark = c->serve_mark[c->seq_blocks[rows.r[i].slot][0]];
         if (mark < 0) mark = n++;
         group[i] = mark;
         count[mark + 1] += 1;
     }
-    for (uint32_t i = 0; i < batch; ++i) c->serve_mark[c->seq_blocks[rows.slot[i]][0]] = -1;
+    for (uint32_t i = 0; i < batch; ++i) c->serve_mark[c->seq_blocks[rows.r[i].slot][0]] = -1;
     if (n == (int)batch) return 0;
     for (int g = 0; g < n; ++g) count[g + 1] += count[g];
     int order[kServeMaxBatch], common[kServeMaxBatch];
     for (int g = 0; g < n; ++g) at[g] = count[g];
     for (uint32_t i = 0; i < batch; ++i) order[at[group[i]]++] = (int)i;
-    int slot[kServeMaxBatch], len[kServeMaxBatch];
-    std::copy(rows.slot, rows.slot + batch, slot);
-    std::copy(rows.len, rows.len + batch, len);
-    for (uint32_t i = 0; i < batch; ++i) {
-        rows.slot[i] = slot[order[i]];
-        rows.len[i] = len[order[i]];
-        rows.row[i] = order[i];
-    }
+    ServeRow given[kServeMaxBatch];
+    std::copy(rows.r, rows.r + batch, given);
+    for (uint32_t i = 0; i < batch; ++i) rows.r[i] = given[order[i]];
     for (uint32_t i = 0; i + 1 < batch; ++i)
         common[i] = group[order[i]] == group[order[i + 1]]
-                        ? common_blocks(c->seq_blocks[rows.slot[i]], c->seq_blocks[rows.slot[i + 1]]) : 0;
+                        ? common_blocks(c->seq_blocks[rows.r[i].slot], c->seq_blocks[rows.r[i + 1].slot]) : 0;
     const int tile_blocks = kAttnTileBlocks;
     long long work = 0;
     for (int g = 0; g < n; ++g)
@@ -873,7 +867,7 @@ int plan_shared(ZynferCuCtx* c, uint32_t batch, bool bf16, int* max_segs) {
             }
         });
     const int sms = c->caps.sm_count > 0 ? c->caps.sm_count : 148;
-    const int slots = sms * attn_tile_ctas(bf16);
+    const int slots = sms * attn_tile_ctas(bf16);  // (a split count stays below 1024)
     const int per = (int)std::max<long long>(2, (work + slots - 1) / slots);
     int items = 0;
     for (int e = 0; e < list.n; ++e) {
@@ -882,8 +876,7 @@ int plan_shared(ZynferCuCtx* c, uint32_t batch, bool bf16, int* max_segs) {
         items += split * (int)c->d.n_kv;
         *max_segs = std::max(*max_segs, split + 1);
         for (int r = list.first[e]; r < list.first[e] + list.count[e]; ++r) {
-            rows.skip[r] = list.blocks[e];
-            rows.nrec[r] = split;
+            rows.r[r].own = (uint32_t)list.blocks[e] << 10 | (uint32_t)split;
         }
     }
     list.item0[list.n] = items;
@@ -925,8 +918,8 @@ int plan_serve(ZynferCuCtx* c, uint32_t batch, uint32_t tokens, uint32_t window,
     long long blocks = 0;
     int longest = 1;
     for (uint32_t i = 0; i < batch; ++i) {
-        const int pos = rows.len[i] - 1;
-        const int n = std::max(1, serve_span_blocks(pos, window, (int)std::min<uint32_t>(sinks, c->d.max_seq_len), rows.skip[i]));
+        const int n = std::max(1, serve_span_blocks(rows.r[i].len - 1, window, (int)std::min<uint32_t>(sinks, c->d.max_seq_len),
+                                                    rows.r[i].skip()));
         blocks += n;
         longest = std::max(longest, n);
     }
@@ -941,12 +934,12 @@ void enqueue_serve(ZynferCuCtx* c, const ServePlan& p, ServeAttnArgs a) {
     a.nsplit = p.nsplit;
     a.max_segs = p.max_segs;
     a.part = c->serve_part;
-    a.counters = c->dcnt;
+    a.counters = c->serve_cnt;
     a.min_per = p.min_per;
     a.early = p.items > 0 ? 1 : 0;
     if (p.items) launch_attn_tile(c->tm_kv, c->serve_rows, c->serve_tiles, a, p.items, c->stream);
     if (!p.chunk) launch_attn_span(c->serve_rows, a, p.ctas, c->stream);
-    else if (p.nsplit > 1) launch_serve_merge(c->serve_rows, a, c->stream);
+    else if (p.nsplit > 1) launch_serve_merge(a, c->stream);
 }
 
 // Changed block-table rows to the device; the pinned copy may be rewritten by
@@ -1208,6 +1201,7 @@ int zynfer_cu_model_init(ZynferCuCtx* c, const ZynferCuModelDesc* desc) {
     ALLOC(c->dkeys, B);
     ALLOC(c->dids, B);
     ALLOC(c->dcnt, B * m.n_kv);
+    ALLOC(c->serve_cnt, B * m.n_q);
     ALLOC(c->dpart, B * m.n_kv * (size_t)decode_max_segs(c->max_blocks) * 2 * (hd + 4));
     c->hist_cap = std::max<size_t>(B * 4096, 1 << 16);
     ALLOC(c->dhist, c->hist_cap);
@@ -1273,6 +1267,7 @@ int zynfer_cu_model_init(ZynferCuCtx* c, const ZynferCuModelDesc* desc) {
     if ((rc = halloc(c, &c->hids, B)) != ZYNFER_CU_OK) return rc;
     cudaMemset(c->dkeys, 0, B * 8);
     cudaMemset(c->dcnt, 0, B * m.n_kv * 4);
+    cudaMemset(c->serve_cnt, 0, B * m.n_q * 4);
     cudaMemset(c->derr, 0, 4);
     cudaMemset(c->dstep, 0, 4);
     ZC_CHECK(c, cudaDeviceSynchronize(), "model init");
