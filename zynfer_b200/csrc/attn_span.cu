@@ -15,9 +15,9 @@
 //   O[8 rows][128] += P . V with P's rows the three terms of each head's p.
 // Maximum, sum and accumulators are f32, exponentials in powers of two.
 // The pieces of a (row, kv head) that meet in one CTA are joined in shared
-// memory; what crosses CTAs, and a common prompt's partial results, meet in
-// global records that the last CTA of the row joins in a fixed order (an
-// atomic counter tells which is last; nothing waits).
+// memory; what crosses CTAs meets in global records that the last CTA of the
+// row joins in a fixed order (an atomic counter tells which is last; nothing
+// waits). A row with a common prompt leaves its records to serve_attn.cu's join.
 #include <algorithm>
 #include <type_traits>
 
@@ -47,7 +47,7 @@ struct Smem {
     uint32_t kidx[kWarps][kIdRing];
     int rec_gid[2][kWarps];
     int pref[kServeMaxBatch + 1];
-    ServeRow info[kServeSmallBatch];  // the rows of a small batch
+    ServeRow info[kServeMidBatch];  // the rows, where they fit
 };
 static_assert(sizeof(Smem) + 1024 <= 232448, "span attention shared memory");
 
@@ -89,7 +89,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t* kidx = sm.kidx[warp];
     const int B = a.batch;
     auto info = [&](int b) {
-        const int4 x = *reinterpret_cast<const int4*>(N <= kServeSmallBatch ? &sm.info[b] : &rows.r[b]);
+        const int4 x = *reinterpret_cast<const int4*>(N <= kServeMidBatch ? &sm.info[b] : &rows.r[b]);
         return ServeRow{x.x, x.y, x.z, (uint32_t)x.w};
     };
     auto span_row = [&](const ServeRow& r) { return span_of(r.len - 1, r.len - 1, a.window, a.sinks, r.skip()); };
@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (b < B) {
                 const int4 w = *reinterpret_cast<const int4*>(&rows.r[b]);
                 const ServeRow r{w.x, w.y, w.z, (uint32_t)w.w};
-                if (N <= kServeSmallBatch) sm.info[b] = r;
+                if (N <= kServeMidBatch) sm.info[b] = r;
                 x = max(1, span_row(r).total);
             }
 #pragma unroll
@@ -378,8 +378,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             const long long f0 = (long long)a.n_kv * pref[cc.b] + (long long)cc.head * cc.nblk;
             const bool whole = f0 >= lo && f0 + cc.nblk <= lo + n;
             const int nrec = cur.nrec();
-            if (whole && !waited) {
-                pdl_wait();
+            if (whole && nrec == 0 && !waited) {
+                pdl_wait();  // (the output may still be read)
                 waited = true;
             }
             if (whole && nrec == 0) {
@@ -395,27 +395,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
             } else {
+                // (the records of the call before were joined before the tile kernel started)
                 const int k = f0 < lo ? 0 : 1;
-                float* rec = sm.rec[k][warp] + hsel * kRecord;
+                float* rec = whole ? a.part + (((size_t)cc.b * (a.n_kv * kG) + cc.head * kG + hsel) * a.max_segs + nrec) * kRecord
+                                   : sm.rec[k][warp] + hsel * kRecord;
                 if (writer) {
-                    if (t == 0) *reinterpret_cast<float2*>(rec) = make_float2(Mh, Lh);
+                    if (t == 0) *reinterpret_cast<float4*>(rec) = make_float4(Mh, Lh, __int_as_float(1), 0.0f);
 #pragma unroll
                     for (int nt = 0; nt < 16; ++nt) *reinterpret_cast<float2*>(rec + 4 + 8 * nt + 2 * t) = make_float2(acc[nt][0], acc[nt][1]);
                 }
-                if (whole) {  // all of the row's own part: with its prompt's records at once
-                    __syncwarp();
-#pragma unroll 1
-                    for (int h = 0; h < kG; ++h) {
-                        const int hq = cc.head * kG + h;
-                        Partial x = no_partial();
-                        join_shared(x, sm.rec[1][warp] + h * kRecord);
-                        join_records(x, a.part + ((size_t)cc.b * (a.n_kv * kG) + hq) * a.max_segs * kRecord, nrec);
-                        store_out4(a, cur.row, hq, x.acc, x.l);
-                    }
-                    __syncwarp();
-                } else if (lane == 0) {
-                    sm.rec_gid[k][warp] = cc.b * a.n_kv + cc.head;
-                }
+                if (!whole && lane == 0) sm.rec_gid[k][warp] = cc.b * a.n_kv + cc.head;
             }
             seg_start = true;
         }
@@ -424,8 +413,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (!waited) pdl_wait();
 
     // ---- join the warps' records of each (row, kv head) of this CTA, in warp
-    // order, a warp per query head; a row that goes on in other CTAs, or has a
-    // common prompt, through the global records
+    // order, a warp per query head; a row that goes on in other CTAs through the
+    // global records
     __syncthreads();
     Cursor gc;
     locate(c_lo, gc);
@@ -452,8 +441,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (nrec + nown > a.max_segs) {
                 if (lane == 0 && a.err) atomicOr(a.err, kErrBadIndex);
                 last = false;
+            } else if (nrec > 0) {
+                store_record(base + (size_t)(nrec + seg) * kRecord, x, nown);
+                last = false;
             } else if (nown > 1) {
-                store_record(base + (size_t)(nrec + seg) * kRecord, x);
+                store_record(base + (size_t)seg * kRecord, x);
                 __threadfence();
                 __syncwarp();
                 unsigned prev = 0;
@@ -467,8 +459,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 x = no_partial();
             }
             if (last) {
-                // every record: the prompt's, then (if this row crosses CTAs) the CTAs' in order
-                join_records(x, base, nown > 1 ? nrec + nown : nrec);
+                if (nown > 1) join_records(x, base, nown);  // the CTAs', in order
                 store_out4(a, r.row, hq, x.acc, x.l);
             }
         }
@@ -485,13 +476,19 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 void launch_attn_span(const ServeRows& rows, const ServeAttnArgs& a, int ctas, cudaStream_t st) {
     if (a.batch <= kServeSmallBatch)
-        launch_pdl(attn_span_kernel<kServeSmallBatch>, ctas, kThreads, sizeof(Smem), st, small_rows(rows), a);
-    else
-        launch_pdl(attn_span_kernel<kServeMaxBatch>, ctas, kThreads, sizeof(Smem), st, rows, a);
+        with_rows<kServeSmallBatch>(rows, [&](const ServeRowsT<kServeSmallBatch>& r) {
+            launch_pdl(attn_span_kernel<kServeSmallBatch>, ctas, kThreads, sizeof(Smem), st, r, a);
+        });
+    else if (a.batch <= kServeMidBatch)
+        with_rows<kServeMidBatch>(rows, [&](const ServeRowsT<kServeMidBatch>& r) {
+            launch_pdl(attn_span_kernel<kServeMidBatch>, ctas, kThreads, sizeof(Smem), st, r, a);
+        });
+    else launch_pdl(attn_span_kernel<kServeMaxBatch>, ctas, kThreads, sizeof(Smem), st, rows, a);
 }
 
 void prepare_attn_span_kernels() {
     configure_kernel((const void*)attn_span_kernel<kServeSmallBatch>, sizeof(Smem));
+    configure_kernel((const void*)attn_span_kernel<kServeMidBatch>, sizeof(Smem));
     configure_kernel((const void*)attn_span_kernel<kServeMaxBatch>, sizeof(Smem));
 }
 

@@ -8,7 +8,7 @@
 // time: S = Q K^T into TMEM, softmax in registers with one thread per row,
 // P back into TMEM over S as the next MMA's A operand, O += P V into TMEM.
 // S has two buffers: the tensor cores form tile i + 1 while the exponentials of
-// tile i are taken. Warps 0-3: softmax; 4, 5: loads of K and of V, each a ring
+// tile i are taken. Warps 0-3: softmax; 4, 7 and 5: loads of K and of V, each a ring
 // of its own (K's places are free again after S, V's after P V); 6: MMAs.
 // With bf16 queries two CTAs share an SM, so that the start and the end of one
 // (a third of its time at a window of 1024) run beside the middle of the other.
@@ -45,7 +45,7 @@ using namespace serve;
 
 constexpr int kRows = 128;       // MMA M: 64 queries x 2 query heads, row 2 m + h
 constexpr int kMembers = kRows / kG;
-constexpr int kThreads = 256;    // warps 0-3: softmax; 4: K; 5: V; 6: MMA
+constexpr int kThreads = 256;    // warps 0-3: softmax; 4, 7: K; 5: V; 6: MMA
 constexpr int TILE = 64, kTileBlocks = TILE / kKvBlock;  // tokens of a tile
 constexpr int kHalf = TILE * 128, kTileBytes = 2 * kHalf;  // a K or V tile: two 64-dim halves
 constexpr int kHalfDims = 64;
@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(kThreads, Lay<TERMS>::CTAS)
     const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
     if (threadIdx.x == 0) {
         for (int s = 0; s < L::KST; ++s) {
-            mbar_init(&full_k[s], 1);
+            mbar_init(&full_k[s], 2);
             mbar_init(&empty_k[s], 1);
         }
         for (int s = 0; s < L::VST; ++s) {
@@ -247,9 +247,11 @@ __global__ void __launch_bounds__(kThreads, Lay<TERMS>::CTAS)
     pdl_launch_dependents();
     const int n = job.n;
 
-    if (warp == 4 || warp == 5) {
-        // ---------------- K (warp 4) or V (warp 5): a lane per half of a block
-        const int is_v = warp - 4, stages = is_v ? L::VST : L::KST;
+    if (warp == 4 || warp == 5 || warp == 7) {
+        // ---------------- K (warps 4 and 7, a half of the dims each) or V (warp 5):
+        // a lane per half of a block. A copy costs its warp about 100 cycles, so the
+        // eight of a K tile, which S waits for, are shared.
+        const int is_v = warp == 5, stages = is_v ? L::VST : L::KST;
         uint64_t* full = is_v ? full_v : full_k;
         uint64_t* empty = is_v ? empty_v : empty_k;
         uint8_t* ring = smem + (is_v ? L::V : L::K);
@@ -266,7 +268,8 @@ __global__ void __launch_bounds__(kThreads, Lay<TERMS>::CTAS)
         };
         constexpr int kChunk = 32 / kTileBlocks;  // tiles of a chunk
         int now = rows_of(0), next = n > kChunk ? rows_of(1) : 0;
-        const int blk = (lane >> 1) & (kTileBlocks - 1), half = lane & 1;
+        const int copies = is_v ? 2 * kTileBlocks : kTileBlocks;
+        const int blk = lane & (kTileBlocks - 1), half = is_v ? (lane / kTileBlocks) & 1 : (warp == 7);
         for (int i = 0, s = 0, round = 0; i < n; ++i) {
             if (i > 0 && i % kChunk == 0) {
                 now = next;
@@ -281,9 +284,9 @@ __global__ void __launch_bounds__(kThreads, Lay<TERMS>::CTAS)
                 break;
             }
             const int y = __shfl_sync(kAll, now, (i % kChunk) * kTileBlocks + blk);
-            if (lane == 0) mbar_arrive_expect_tx(&full[s], kTileBytes);
+            if (lane == 0) mbar_arrive_expect_tx(&full[s], copies * (kTileBytes / (2 * kTileBlocks)));
             __syncwarp();
-            if (lane < 2 * kTileBlocks)
+            if (lane < copies)
                 tma_box(smem_addr(ring + s * kTileBytes + half * kHalf + blk * (kKvBlock * 128)), &kv_map, half * kHalfDims, y,
                         &full[s]);
             if (++s == stages) {
@@ -566,29 +569,31 @@ __global__ void __launch_bounds__(kThreads, Lay<TERMS>::CTAS)
 
 }  // namespace
 
+template <int N>
+void launch_sized(const CUtensorMap& kv_map, const ServeRowsT<N>& rows, const TileListT<N>& list, const ServeAttnArgs& a,
+                  int items, cudaStream_t st) {
+    if (a.bf16) launch_pdl(attn_tile_kernel<1, N>, items, kThreads, Lay<1>::SMEM, st, kv_map, rows, list, a);
+    else launch_pdl(attn_tile_kernel<3, N>, items, kThreads, Lay<3>::SMEM, st, kv_map, rows, list, a);
+}
+
 void launch_attn_tile(const CUtensorMap& kv_map, const ServeRows& rows, const TileList& list, const ServeAttnArgs& a,
                       int items, cudaStream_t st) {
-    if (a.batch <= kServeSmallBatch) {
-        TileListT<kServeSmallBatch> small;
-        small.n = list.n;
-        for (int e = 0; e < list.n; ++e) {
-            small.item0[e] = list.item0[e];
-            small.first[e] = list.first[e];
-            small.count[e] = list.count[e];
-            small.blocks[e] = list.blocks[e];
-        }
-        small.item0[list.n] = items;
-        if (a.bf16) launch_pdl(attn_tile_kernel<1, kServeSmallBatch>, items, kThreads, Lay<1>::SMEM, st, kv_map, small_rows(rows), small, a);
-        else launch_pdl(attn_tile_kernel<3, kServeSmallBatch>, items, kThreads, Lay<3>::SMEM, st, kv_map, small_rows(rows), small, a);
-    } else {
-        if (a.bf16) launch_pdl(attn_tile_kernel<1, kServeMaxBatch>, items, kThreads, Lay<1>::SMEM, st, kv_map, rows, list, a);
-        else launch_pdl(attn_tile_kernel<3, kServeMaxBatch>, items, kThreads, Lay<3>::SMEM, st, kv_map, rows, list, a);
-    }
+    if (a.batch <= kServeSmallBatch)
+        with_rows<kServeSmallBatch>(rows, [&](const ServeRowsT<kServeSmallBatch>& r) {
+            launch_sized(kv_map, r, first_tiles<kServeSmallBatch>(list, items), a, items, st);
+        });
+    else if (a.batch <= kServeMidBatch)
+        with_rows<kServeMidBatch>(rows, [&](const ServeRowsT<kServeMidBatch>& r) {
+            launch_sized(kv_map, r, first_tiles<kServeMidBatch>(list, items), a, items, st);
+        });
+    else launch_sized(kv_map, rows, list, a, items, st);
 }
 
 void prepare_attn_tile_kernels() {
     configure_kernel((const void*)attn_tile_kernel<1, kServeSmallBatch>, Lay<1>::SMEM);
     configure_kernel((const void*)attn_tile_kernel<3, kServeSmallBatch>, Lay<3>::SMEM);
+    configure_kernel((const void*)attn_tile_kernel<1, kServeMidBatch>, Lay<1>::SMEM);
+    configure_kernel((const void*)attn_tile_kernel<3, kServeMidBatch>, Lay<3>::SMEM);
     configure_kernel((const void*)attn_tile_kernel<1, kServeMaxBatch>, Lay<1>::SMEM);
     configure_kernel((const void*)attn_tile_kernel<3, kServeMaxBatch>, Lay<3>::SMEM);
 }

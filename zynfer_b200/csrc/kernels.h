@@ -189,7 +189,7 @@ struct TileListT {
     short first[N / 2], count[N / 2];    // rows of ServeRows
     int blocks[N / 2];                   // common leading blocks
 };
-constexpr int kServeSmallBatch = 64;
+constexpr int kServeSmallBatch = 64, kServeMidBatch = 256;
 using ServeRows = ServeRowsT<kServeMaxBatch>;
 using TileList = TileListT<kServeMaxBatch>;
 struct ServeAttnArgs {
@@ -218,15 +218,30 @@ void prepare_attn_span_kernels();
 // blocks / (kSpanWarps min_per) + 2 CTAs.
 constexpr int kSpanWarps = 8;
 void launch_attn_span(const ServeRows& rows, const ServeAttnArgs& a, int ctas, cudaStream_t st);
-// The first rows of a batch of at most kServeSmallBatch.
-inline ServeRowsT<kServeSmallBatch> small_rows(const ServeRows& r) {
-    ServeRowsT<kServeSmallBatch> s;
-    for (int i = 0; i < kServeSmallBatch; ++i) s.r[i] = r.r[i];
+// Calls f with the first rows (and tiles) of a batch in the smallest parameter
+// type that holds them.
+template <int N, typename F>
+inline void with_rows(const ServeRows& r, F&& f) {
+    ServeRowsT<N> s;
+    for (int i = 0; i < N; ++i) s.r[i] = r.r[i];
+    f(s);
+}
+template <int N>
+inline TileListT<N> first_tiles(const TileList& l, int items) {
+    TileListT<N> s;
+    s.n = l.n;
+    for (int e = 0; e < l.n; ++e) {
+        s.item0[e] = l.item0[e];
+        s.first[e] = l.first[e];
+        s.count[e] = l.count[e];
+        s.blocks[e] = l.blocks[e];
+    }
+    s.item0[l.n] = items;
     return s;
 }
 // Cache blocks that a query at `pos` sees after the first `skip`.
 int serve_span_blocks(int pos, uint32_t window, int sinks, int skip);
-void launch_serve_merge(const ServeAttnArgs& a, cudaStream_t st);
+void launch_serve_merge(const ServeRows& rows, const ServeAttnArgs& a, cudaStream_t st);
 struct KvWriteArgs {
     uint16_t* kv_layer;
     const int* table_row;      // the sequence's device block-table row

@@ -16,17 +16,36 @@ namespace {
 
 using namespace serve;
 
-// The records of a chunk's (row, query head) joined: a warp each.
-__global__ void __launch_bounds__(128) serve_merge_kernel(const __grid_constant__ ServeAttnArgs a) {
-    pdl_wait();
-    pdl_launch_dependents();
+// The records of a (row, query head) joined, a warp each: a chunk's (rows.n
+// == 0), or those of the rows that share a prompt: the prompt's, then the row's
+// own, whose first says how many they are. A launch of its own because a row's
+// join is a chain of round trips: inside the kernel that streams the rows' own
+// blocks it held up the warps that have many short rows (64 rows sharing 4096
+// positions: 31 us a call there, LATER here).
+template <int N>
+__global__ void __launch_bounds__(128) serve_merge_kernel(const __grid_constant__ ServeRowsT<N> rows_param,
+                                                          const __grid_constant__ ServeAttnArgs a) {
+    const ServeRowsT<N>& rows = as_memory(rows_param);
     const int n_q = a.n_kv * kG;
     const long long w = ((long long)blockIdx.x * blockDim.x + threadIdx.x) / kWarp;
     if (w >= (long long)a.batch * a.tokens * n_q) return;
-    const int hq = (int)(w % n_q), row = (int)(w / n_q);
+    const int hq = (int)(w % n_q), i = (int)(w / n_q);
+    const float* base = a.part + ((size_t)i * n_q + hq) * a.max_segs * kRecord;
     Partial x = no_partial();
-    join_records(x, a.part + ((size_t)row * n_q + hq) * a.max_segs * kRecord, a.nsplit);
-    store_out4(a, row, hq, x.acc, x.l);
+    if (a.nsplit > 1) {
+        pdl_wait();
+        pdl_launch_dependents();
+        join_records(x, base, a.nsplit);
+        store_out4(a, i, hq, x.acc, x.l);
+    } else {
+        const int4 r = *reinterpret_cast<const int4*>(&rows.r[i]);
+        const int nrec = (int)((uint32_t)r.w & 1023u);
+        pdl_wait();
+        pdl_launch_dependents();
+        if (nrec == 0) return;
+        join_records(x, base, 0, nrec);
+        store_out4(a, r.z, hq, x.acc, x.l);
+    }
 }
 
 // K and V rows [n_kv][n][128] (f32 rounded to nearest even, or bf16) into
@@ -67,9 +86,18 @@ __global__ void __launch_bounds__(256) kv_write_kernel(KvWriteArgs a) {
 
 int serve_span_blocks(int pos, uint32_t window, int sinks, int skip) { return span_of(pos, pos, window, sinks, skip).total; }
 
-void launch_serve_merge(const ServeAttnArgs& a, cudaStream_t st) {
+void launch_serve_merge(const ServeRows& rows, const ServeAttnArgs& a, cudaStream_t st) {
     const long long warps = (long long)a.batch * a.tokens * a.n_kv * kG;
-    launch_pdl(serve_merge_kernel, (unsigned)((warps + 3) / 4), 128, 0, st, a);
+    const unsigned ctas = (unsigned)((warps + 3) / 4);
+    if (a.batch <= kServeSmallBatch)
+        with_rows<kServeSmallBatch>(rows, [&](const ServeRowsT<kServeSmallBatch>& r) {
+            launch_pdl(serve_merge_kernel<kServeSmallBatch>, ctas, 128, 0, st, r, a);
+        });
+    else if (a.batch <= kServeMidBatch)
+        with_rows<kServeMidBatch>(rows, [&](const ServeRowsT<kServeMidBatch>& r) {
+            launch_pdl(serve_merge_kernel<kServeMidBatch>, ctas, 128, 0, st, r, a);
+        });
+    else launch_pdl(serve_merge_kernel<kServeMaxBatch>, ctas, 128, 0, st, rows, a);
 }
 
 void launch_kv_write(const KvWriteArgs& a, cudaStream_t st) {
@@ -79,7 +107,9 @@ void launch_kv_write(const KvWriteArgs& a, cudaStream_t st) {
 }
 
 void prepare_serve_attn_kernels() {
-    configure_kernel((const void*)serve_merge_kernel, 0);
+    configure_kernel((const void*)serve_merge_kernel<kServeSmallBatch>, 0);
+    configure_kernel((const void*)serve_merge_kernel<kServeMidBatch>, 0);
+    configure_kernel((const void*)serve_merge_kernel<kServeMaxBatch>, 0);
     configure_kernel((const void*)kv_write_kernel, 0);
 }
 

@@ -13,7 +13,7 @@ constexpr int kD = 128, kG = 2;  // head dim, query heads per kv head
 constexpr int kBlockElems = kKvBlock * kD;
 constexpr float kLog2e = 1.4426950408889634f;
 // A partial result of one query head: reference point (log2 units) and sum of
-// its exponentials, two words of padding, the weighted sum of V.
+// its exponentials, a count (below) and a word of padding, the weighted sum of V.
 constexpr int kRecord = kServeRecord;
 static_assert(kRecord == kD + 4, "record: m, l, -, -, acc");
 
@@ -81,8 +81,10 @@ __device__ __forceinline__ Partial no_partial() { return Partial{-INFINITY, 0.0f
 // Lane j reads the (m, l) of record j and weighs it, so a batch of up to 32
 // costs one exponential and, with kAhead accumulators requested before any is
 // used, about cnt / kAhead round trips.
-__device__ __forceinline__ void join_records(Partial& x, const float* base, int cnt) {
+// counted >= 0: record `counted` says how many there are from it on.
+__device__ __forceinline__ void join_records(Partial& x, const float* base, int cnt, int counted = -1) {
     const int lane = threadIdx.x % kWarp;
+    if (counted >= 0) cnt = counted + __ldcg(reinterpret_cast<const int*>(base + (size_t)counted * kRecord + 2));
     constexpr int kAhead = 8;
     for (int j0 = 0; j0 < cnt; j0 += kWarp) {
         const int some = min(kWarp, cnt - j0);
@@ -173,9 +175,9 @@ __device__ __forceinline__ void store_out4(const ServeAttnArgs& a, int qrow, int
 __device__ __forceinline__ void store_row(const ServeAttnArgs& a, int qrow, int hq, const SlowRow& r) {
     store_out4(a, qrow, hq, r.acc, r.l);
 }
-__device__ __forceinline__ void store_record(float* rec, const SlowRow& r) {
+__device__ __forceinline__ void store_record(float* rec, const Partial& r, int count = 0) {
     const int lane = threadIdx.x % kWarp;
-    if (lane == 0) *reinterpret_cast<float2*>(rec) = make_float2(r.m, r.l);
+    if (lane == 0) *reinterpret_cast<float4*>(rec) = make_float4(r.m, r.l, __int_as_float(count), 0.0f);
     *reinterpret_cast<float4*>(rec + 4 + 4 * lane) = make_float4(r.acc[0], r.acc[1], r.acc[2], r.acc[3]);
 }
 

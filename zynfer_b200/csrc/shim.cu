@@ -868,7 +868,16 @@ int plan_shared(ZynferCuCtx* c, uint32_t batch, bool bf16, int* max_segs) {
         });
     const int sms = c->caps.sm_count > 0 ? c->caps.sm_count : 148;
     const int slots = sms * attn_tile_ctas(bf16);  // (a split count stays below 1024)
-    const int per = (int)std::max<long long>(2, (work + slots - 1) / slots);
+    // tiles of keys per work item: the least, 2 or more, with which all items run at once
+    int per = (int)std::max<long long>(2, (work + slots - 1) / slots);
+    for (;; ++per) {
+        long long n_items = 0;
+        for (int e = 0; e < list.n; ++e) {
+            const int tiles = (list.blocks[e] + tile_blocks - 1) / tile_blocks;
+            n_items += (long long)((tiles + per - 1) / per) * c->d.n_kv;
+        }
+        if (n_items <= slots || n_items == (long long)list.n * c->d.n_kv) break;
+    }
     int items = 0;
     for (int e = 0; e < list.n; ++e) {
         const int tiles = (list.blocks[e] + tile_blocks - 1) / tile_blocks, split = (tiles + per - 1) / per;
@@ -939,7 +948,7 @@ void enqueue_serve(ZynferCuCtx* c, const ServePlan& p, ServeAttnArgs a) {
     a.early = p.items > 0 ? 1 : 0;
     if (p.items) launch_attn_tile(c->tm_kv, c->serve_rows, c->serve_tiles, a, p.items, c->stream);
     if (!p.chunk) launch_attn_span(c->serve_rows, a, p.ctas, c->stream);
-    else if (p.nsplit > 1) launch_serve_merge(a, c->stream);
+    if (p.chunk ? p.nsplit > 1 : p.items > 0) launch_serve_merge(c->serve_rows, a, c->stream);
 }
 
 // Changed block-table rows to the device; the pinned copy may be rewritten by
