@@ -4,8 +4,10 @@
 //
 // Bound by the bytes of K and V, so built to stream: persistent and
 // warp-granular. The work is the list of (row, kv head, visible 16-token
-// block), row-major; every warp of the grid takes an equal contiguous share,
-// whatever the rows' lengths, through a private ring of kRing 8 KB slots (K
+// block), row-major; every warp of the grid takes a contiguous share of equal
+// cost, whatever the rows' lengths (a (row, kv head) costs kSpanLead blocks beside its
+// own: its query's way in and its result's way out; without them warps with many
+// short rows finished last, 36 against 13 us), through a private ring of kRing 8 KB slots (K
 // then V of one block and head are contiguous) filled by cp.async.bulk. Two
 // blocks of one (row, kv head) are taken per step, on the tensor cores
 // (mma.sync m16n8k16, bf16 in, f32 out; a query's 2 heads are too few rows for
@@ -46,6 +48,7 @@ struct Smem {
     uint64_t full[kWarps][kRing];
     uint32_t kidx[kWarps][kIdRing];
     int rec_gid[2][kWarps];
+    long long bound[kWarps + 1];  // first block of each warp's share
     int pref[kServeMaxBatch + 1];
     ServeRow info[kServeMidBatch];  // the rows, where they fit
 };
@@ -97,22 +100,29 @@ __global__ void __launch_bounds__(kThreads, 1)
     // prefix of the rows' block counts; a row that sees nothing here counts one
     if (warp == 0) {
         int carry = 0;
-        for (int base = 0; base < B; base += kWarp) {
-            const int b = base + lane;
-            int x = 0;
-            if (b < B) {
-                const int4 w = *reinterpret_cast<const int4*>(&rows.r[b]);
-                const ServeRow r{w.x, w.y, w.z, (uint32_t)w.w};
-                if (N <= kServeMidBatch) sm.info[b] = r;
-                x = max(1, span_row(r).total);
-            }
+        constexpr int kAhead = N < 256 ? N / kWarp : 8;
+        for (int base0 = 0; base0 < B; base0 += kAhead * kWarp) {
+            int4 w[kAhead];
 #pragma unroll
-            for (int o = 1; o < kWarp; o <<= 1) {
-                const int y = __shfl_up_sync(kAll, x, o);
-                if (lane >= o) x += y;
+            for (int k = 0; k < kAhead; ++k)
+                if (base0 + k * kWarp + lane < B) w[k] = *reinterpret_cast<const int4*>(&rows.r[base0 + k * kWarp + lane]);
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                const int b = base0 + k * kWarp + lane;
+                int x = 0;
+                if (b < B) {
+                    const ServeRow r{w[k].x, w[k].y, w[k].z, (uint32_t)w[k].w};
+                    if (N <= kServeMidBatch) sm.info[b] = r;
+                    x = max(1, span_row(r).total);
+                }
+#pragma unroll
+                for (int o = 1; o < kWarp; o <<= 1) {
+                    const int y = __shfl_up_sync(kAll, x, o);
+                    if (lane >= o) x += y;
+                }
+                if (b < B) sm.pref[b + 1] = carry + x;
+                carry += __shfl_sync(kAll, x, kWarp - 1);
             }
-            if (b < B) sm.pref[b + 1] = carry + x;
-            carry += __shfl_sync(kAll, x, kWarp - 1);
         }
         if (lane == 0) sm.pref[0] = 0;
     }
@@ -123,13 +133,30 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane < 2) sm.rec_gid[lane][warp] = -1;
     __syncthreads();
     const int* pref = sm.pref;
-    const long long total = (long long)pref[B] * a.n_kv;
+    // cost units: kSpanLead of every (row, kv head), then its blocks. Block f of row b
+    // is unit f + kSpanLead (b n_kv + head + 1); first_block(u) is the first block at
+    // or after unit u.
+    const long long total = (long long)pref[B] * a.n_kv, units = total + (long long)kSpanLead * B * a.n_kv;
+    auto first_block = [&](long long u) -> long long {
+        if (u >= units) return total;
+        int l = 0, h = B - 1;
+        while (l < h) {
+            const int mid = (l + h + 1) / 2;
+            if ((long long)a.n_kv * (pref[mid] + kSpanLead * mid) <= u) l = mid;
+            else h = mid - 1;
+        }
+        const int nblk = pref[l + 1] - pref[l], r = (int)(u - (long long)a.n_kv * (pref[l] + kSpanLead * l));
+        return (long long)a.n_kv * pref[l] + (long long)(r / (nblk + kSpanLead)) * nblk + max(0, r % (nblk + kSpanLead) - kSpanLead);
+    };
     const int nwarps = gridDim.x * kWarps;
-    const int per = (int)max((total + nwarps - 1) / nwarps, (long long)a.min_per);
-    const long long c_lo = (long long)blockIdx.x * kWarps * per, c_hi = min(total, c_lo + (long long)kWarps * per);
-    if (c_lo >= total) return;
-    const long long lo = c_lo + (long long)warp * per;
-    const int n = (int)max(0ll, min(c_hi, lo + per) - lo);
+    const int per = (int)max((units + nwarps - 1) / nwarps, (long long)a.min_per);
+    const long long reach = (long long)kWarps * per;  // units of a CTA
+    if (warp == 0 && lane <= kWarps) sm.bound[lane] = first_block(blockIdx.x * reach + (long long)lane * per);
+    __syncthreads();
+    const long long* bound = sm.bound;
+    const long long c_lo = bound[0], c_hi = bound[kWarps];
+    const long long lo = bound[warp];
+    const int n = (int)(bound[warp + 1] - lo);
 
     struct Cursor {
         int b, head, blk, nblk;
@@ -210,7 +237,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // the tile's records and the buffers are touched after the wait below.
     if (!a.early) pdl_wait();
     Cursor cc;
-    locate(lo, cc);
+    locate(min(lo, total - 1), cc);
     ServeRow cur = info(cc.b);
     if (n > 0) load_q(cur.row, cc.head);  // in front of the blocks, not behind them
     fill_chunk(0);
@@ -417,25 +444,30 @@ __global__ void __launch_bounds__(kThreads, 1)
     // global records
     __syncthreads();
     Cursor gc;
-    locate(c_lo, gc);
+    locate(min(c_lo, total - 1), gc);
     long long g0 = (long long)a.n_kv * pref[gc.b] + (long long)gc.head * gc.nblk;
 #pragma unroll 1
     for (int gi = 0; g0 < c_hi; ++gi) {
         const long long g1 = g0 + gc.nblk;
         const int gb = gc.b, gh = gc.head;
-        const int wa = (int)(max(0ll, g0 - c_lo) / per), wb = (int)min((long long)kWarps - 1, (g1 - 1 - c_lo) / per);
-        const long long lo_a = c_lo + (long long)wa * per;
+        int wa = kWarps, wb = -1;  // warps with blocks of it
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w)
+            if (max(bound[w], g0) < min(bound[w + 1], g1)) {
+                wa = min(wa, w);
+                wb = w;
+            }
         const int h = (warp - 2 * gi) & (kWarps - 1);  // warps 2 gi, 2 gi + 1 (mod 8) take the two heads
-        if (h < kG && !(wa == wb && g0 >= lo_a && g1 <= lo_a + per)) {  // (else its warp stored it)
+        if (h < kG && wb >= 0 && !(wa == wb && g0 >= bound[wa] && g1 <= bound[wa + 1])) {  // (else its warp stored it)
             const ServeRow r = info(gb);
             const int nrec = r.nrec(), hq = gh * kG + h;
             Partial x = no_partial();
             for (int w = wa; w <= wb; ++w) {
-                const int k = g0 >= c_lo + (long long)w * per ? 1 : 0;
+                const int k = g0 >= bound[w] ? 1 : 0;
                 if (sm.rec_gid[k][w] == gb * a.n_kv + gh) join_shared(x, sm.rec[k][w] + h * kRecord);  // (else it stopped early)
             }
-            const long long reach = (long long)kWarps * per;
-            const int first = (int)(g0 / reach), nown = (int)((g1 - 1) / reach) - first + 1, seg = (int)blockIdx.x - first;
+            const long long lead = (long long)kSpanLead * ((long long)gb * a.n_kv + gh + 1);
+            const int first = (int)((g0 + lead) / reach), nown = (int)((g1 - 1 + lead) / reach) - first + 1, seg = (int)blockIdx.x - first;
             float* base = a.part + ((size_t)gb * (a.n_kv * kG) + hq) * a.max_segs * kRecord;
             bool last = true;
             if (nrec + nown > a.max_segs) {

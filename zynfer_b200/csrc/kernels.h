@@ -208,15 +208,16 @@ struct ServeAttnArgs {
     float* part;               // [row][n_q][max_segs][kServeRecord]
     int max_segs;
     unsigned* counters;        // [row][n_q], zero between launches
-    int min_per;               // span kernel: blocks a warp takes at least
+    int min_per;               // span kernel: units a warp takes at least
     int early;                 // span kernel: launched behind a tile kernel
     uint32_t* err;
 };
 void prepare_attn_tile_kernels();
 void prepare_attn_span_kernels();
-// attn_span.cu: single tokens. A (row, kv head) meets at most
-// blocks / (kSpanWarps min_per) + 2 CTAs.
-constexpr int kSpanWarps = 8;
+// attn_span.cu: single tokens. A (row, kv head) counts kSpanLead blocks more than
+// it has; at `per` of these units a warp it meets at most blocks / (kSpanWarps per)
+// + 2 CTAs.
+constexpr int kSpanWarps = 8, kSpanLead = 3;
 void launch_attn_span(const ServeRows& rows, const ServeAttnArgs& a, int ctas, cudaStream_t st);
 // Calls f with the first rows (and tiles) of a batch in the smallest parameter
 // type that holds them.

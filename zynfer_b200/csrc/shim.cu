@@ -932,7 +932,7 @@ int plan_serve(ZynferCuCtx* c, uint32_t batch, uint32_t tokens, uint32_t window,
         blocks += n;
         longest = std::max(longest, n);
     }
-    const long long total = blocks * c->d.n_kv, share = (long long)kSpanWarps * p->min_per;
+    const long long total = (blocks + (long long)kSpanLead * batch) * c->d.n_kv, share = (long long)kSpanWarps * p->min_per;
     p->ctas = (int)std::min<long long>(sms, (total + share - 1) / share);
     const long long per = std::max<long long>(p->min_per, (total + (long long)p->ctas * kSpanWarps - 1) / ((long long)p->ctas * kSpanWarps));
     p->max_segs = tile_segs + (int)((longest - 1) / (per * kSpanWarps) + 2);
