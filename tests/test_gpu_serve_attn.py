@@ -382,3 +382,73 @@ def test_long_loops_over_tiles(tokens, length, window, sinks, dtype):
         m.attn_window(0, [2], q, out, window=window, sinks=sinks)
     m.gpu.sync()
     check(out[0], reference(q[0], k, v, window_seen(length, tokens, window, sinks)), v, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("plen,rows", [([1000], [60]), ([700, 1000, 16, 333], [40, 30, 5, 7]), ([1015], [64])])
+def test_attn_shared_prompts_worth_sharing(plen, rows, dtype):
+    """Large groups (their prompts are read once) and small ones in one batch, the rows interleaved."""
+    total = sum(rows)
+    m = make(n_kv=4, max_batch=total, max_seqs=total, max_seq_len=1100, kv_blocks=sum(p // 16 + 1 for p in plen) + 6 * total)
+    own = [[(7 * i) % 50 if g else 1 + (11 * i) % 60 for i in range(n)] for g, n in enumerate(rows)]
+    kv = share(m, len(plen), plen, own)
+    seqs = [(37 * i + 11) % total for i in range(total)] if total % 37 else list(range(total))
+    assert sorted(seqs) == list(range(total))
+    q = normal(9, total, 8, D, dtype=DTYPES[dtype], scale=1.5)
+    out = torch.full_like(q, float("nan"))
+    torch.cuda.synchronize()
+    for _ in range(2):
+        m.attn_shared(0, seqs, q, out)
+    m.gpu.sync()
+    for i, s in enumerate(seqs):
+        k, v = kv[s]
+        check(out[i:i + 1], reference(q[i:i + 1], k, v, torch.ones(1, k.shape[1], dtype=torch.bool, device="cuda")), v, dtype)
+
+
+def test_attn_shared_forks_of_forks():
+    """A common start, two longer prompts on top of it, and their samples: each run at its own depth."""
+    m = make(n_kv=4, max_batch=80, max_seqs=80, max_seq_len=1400, kv_blocks=700)
+    k, v = normal(51, 4, 1300, D, dtype=torch.bfloat16), normal(52, 4, 1300, D, dtype=torch.bfloat16)
+    k2, v2 = normal(53, 4, 1300, D, dtype=torch.bfloat16), normal(54, 4, 1300, D, dtype=torch.bfloat16)
+    kv = {}
+    m.kv_write(0, 0, 0, k[:, :400].contiguous(), v[:, :400].contiguous())
+    for first, kk, vv in ((1, k, v), (40, k2, v2)):
+        m.seq_fork(first, 0, 400)
+        m.kv_write(first, 0, 400, kk[:, 400:1290].contiguous(), vv[:, 400:1290].contiguous())
+        full = (torch.cat([k[:, :400], kk[:, 400:1290]], 1), torch.cat([v[:, :400], vv[:, 400:1290]], 1))
+        kv[first] = full
+        for s in range(first + 1, first + 39):
+            m.seq_fork(s, first, 1290)
+            e = normal(100 + s, 4, s % 5, D, dtype=torch.bfloat16)
+            m.kv_write(s, 0, 1290, e, e)
+            kv[s] = (torch.cat([full[0], e], 1), torch.cat([full[1], e], 1))
+    kv[0] = (k[:, :400], v[:, :400])
+    seqs = sorted(kv)
+    q = normal(9, len(seqs), 8, D, scale=1.5)
+    out = torch.empty_like(q)
+    torch.cuda.synchronize()
+    m.attn_shared(0, seqs, q, out)
+    m.gpu.sync()
+    for i, s in enumerate(seqs):
+        kk, vv = kv[s]
+        check(out[i:i + 1], reference(q[i:i + 1], kk, vv, torch.ones(1, kk.shape[1], dtype=torch.bool, device="cuda")), vv, "f32")
+
+
+def test_shared_tiles_keep_nan_in_its_dims():
+    m = make(n_kv=4, max_batch=64, max_seqs=64, max_seq_len=1100, kv_blocks=300)
+    k, v = normal(61, 4, 1000, D, dtype=torch.bfloat16), normal(62, 4, 1000, D, dtype=torch.bfloat16)
+    clean = v.clone()
+    v[1, 500, 7] = float("nan")
+    m.kv_write(0, 0, 0, k, v)
+    for s in range(1, 64):
+        m.seq_fork(s, 0, 1000)
+    q = normal(63, 64, 8, D)
+    out = torch.empty_like(q)
+    torch.cuda.synchronize()
+    m.attn_shared(0, range(64), q, out)
+    m.gpu.sync()
+    want = torch.cat([reference(q[i:i + 1], k, clean, torch.ones(1, 1000, dtype=torch.bool, device="cuda")) for i in range(64)])
+    assert torch.isnan(out[:, 2:4, 7]).all()
+    keep = torch.tensor([d for d in range(D) if d != 7], device="cuda")
+    check(out[..., keep], want[..., keep], clean, "f32")
+    assert torch.isfinite(out[:, [0, 1, 4, 5, 6, 7]]).all()

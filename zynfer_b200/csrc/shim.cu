@@ -823,6 +823,13 @@ long long cut_runs(const int* common, int r0, int r1, bool emit, Leaf&& leaf) {
     return std::max(whole, parts);
 }
 
+// Reading a prompt once takes two launches more (tiles, join), about 10 us, the
+// time of 64 MB: below that many saved block reads (of 8 KB) each row reads its own
+// way. Measured, shared / not, one call after another: 8 rows x 1024 positions
+// (3584 blocks saved) 16 / 13 us, 8 x 4096 (14336) 25 / 25 (bf16 20 / 25),
+// 64 x 512 (16128) 26 / 29, 8 x 16384 (57344) 45 / 68.
+constexpr long long kShareBlocks = 8192;
+
 // Common leading blocks of the rows of c->serve_rows (one query each): the
 // rows reordered so that rows with the same first block are neighbours, in the
 // caller's order otherwise; the runs that share blocks as tiles of 64 rows,
@@ -855,7 +862,9 @@ int plan_shared(ZynferCuCtx* c, uint32_t batch, bool bf16, int* max_segs) {
         common[i] = group[order[i]] == group[order[i + 1]]
                         ? common_blocks(c->seq_blocks[rows.r[i].slot], c->seq_blocks[rows.r[i + 1].slot]) : 0;
     const int tile_blocks = kAttnTileBlocks;
-    long long work = 0;
+    long long work = 0, saved = 0;
+    for (int g = 0; g < n; ++g) saved += cut_runs(common, count[g], count[g + 1], false, [](int, int, int) {});
+    if (saved * c->d.n_kv < kShareBlocks) return 0;
     for (int g = 0; g < n; ++g)
         cut_runs(common, count[g], count[g + 1], true, [&](int r0, int r1, int d) {
             for (int r = r0; r < r1; r += 64) {
