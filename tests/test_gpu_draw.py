@@ -198,3 +198,33 @@ def test_one_row_at_any_offset(gpu):
             ids, lp = draw(gpu, x, u, p=0.9)
             for r in range(5):
                 check_row(x[r], float(u[r]), 1.0, 0, float(np.float32(0.9)), 0.0, int(ids[r]), float(lp[r]))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows", [60, 130, 300])
+def test_many_rows(gpu, rows, dtype):
+    """Fewer CTAs take a row the more rows there are; every split follows the definition."""
+    vocab = 50257  # odd: bf16 rows start off 4-byte boundaries in turn
+    g = torch.Generator().manual_seed(rows)
+    x = (3.0 * torch.randn(rows, vocab, generator=g)).to(dtype)
+    x[::4, ::3] = float("-inf")
+    x[5, 7] = float("nan")
+    x = x.cuda()
+    u = torch.rand(rows, generator=g).numpy().astype(np.float32)
+    t, k, p, mp = (np.array([RULES[i % len(RULES)][j] for i in range(rows)]) for j in range(4))
+    ids, lp = draw(gpu, x, u, t.astype(np.float32), k.astype(np.int32), p.astype(np.float32), mp.astype(np.float32))
+    for r in range(rows):
+        check_row(x[r], float(u[r]), float(np.float32(t[r])), int(k[r]), float(np.float32(p[r])), float(np.float32(mp[r])),
+                  int(ids[r]), float(lp[r]))
+
+
+@pytest.mark.parametrize("rows", [30, 60, 130, 300])
+def test_equal_logits_in_every_split(gpu, rows):
+    """One bin holds every token: it is divided down to the index, and its sums pass 32 bits."""
+    vocab = 151936
+    l = torch.full((rows, vocab), 1.5, device="cuda")
+    u = ((np.arange(rows) + 0.5) / rows).astype(np.float32)
+    ids, _ = draw(gpu, l, u)
+    assert np.array_equal(ids, (u.astype(np.float64) * vocab).astype(np.int64))
+    ids, _ = draw(gpu, l, u, k=100000, p=0.25)
+    assert np.array_equal(ids, (u.astype(np.float64) * 25000).astype(np.int64))

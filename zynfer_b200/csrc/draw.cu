@@ -17,8 +17,8 @@
 // weight of 2^-34 of the largest apart from 0 and the sum of 2^18 of them
 // below 2^53, so products with top_p and u are single f64 roundings.
 //
-// One pass over HBM: a cluster of C CTAs holds a row in shared memory and
-// selects by sums.
+// One pass over HBM: a cluster of C CTAs takes a row, each CTA its C-th part,
+// and selects by sums.
 //   1. the largest and smallest logit of the row (one exchange over distributed
 //      shared memory);
 //   2. every CTA adds its tokens' weights (and counts) into NB bins even in
@@ -29,10 +29,14 @@
 //      that bin, which all CTAs send to the first, where they are sorted and
 //      their weights scanned. A bin of more tokens than that list holds (many
 //      equal logits) is divided again, by (logit, index) itself, until it fits.
-// A few rows are bound by the chain of exchanges and barriers, many rows by
-// the instructions per logit (about 60, an accurate exponential among them),
-// not by the bytes: so weights are split into two 32-bit words without integer
-// conversions, and two CTAs share an SM so that one works while the other waits.
+// A few rows are bound by the chain of loads, exchanges and barriers (25 us for
+// one row of 151936), many rows by the instructions per logit (about 50, an
+// accurate exponential among them), not by the bytes. So C is the more CTAs the
+// fewer rows there are: 8 for up to 37 rows, then 4, 2 and 1 (256 rows: LATER us
+// with one CTA a row, 206 with eight, whose barriers left the SMs idle); weights
+// are split into two 32-bit words without integer conversions; and two CTAs
+// share an SM. Eight CTAs hold their parts of a row in shared memory, fewer
+// read them again from L2.
 #include <type_traits>
 
 #include "common.cuh"
@@ -103,23 +107,36 @@ struct Note {
     uint32_t c, d;
 };
 
-template <int C>
-struct Shared {
-    static constexpr int NB = C == 1 ? 512 : 2048;  // bins
-    static constexpr int NB_LOG = C == 1 ? 9 : 11;
+// HOLD: the row's part stays in shared memory (of at most kBatch tokens);
+// otherwise it is read again, and the bins' 32-bit sums are carried over into
+// 64-bit ones every kBatch tokens.
+constexpr int kBatch = 1 << 15;
+template <int NB, bool HOLD>
+struct Bins {
     uint32_t count[NB], hi[NB];  // tokens, and their weights' parts
     int lo[NB];
+};
+template <int NB>
+struct Bins<NB, false> {
+    uint32_t count[NB], hi[NB];
+    int lo[NB];
+    u64 mass[NB];
+};
+template <int C, bool HOLD>
+struct Shared {
+    static constexpr int NB_LOG = C == 1 && HOLD ? 9 : 11, NB = 1 << NB_LOG;  // bins
+    Bins<NB, HOLD> bins;
     u64 list[kList];
     Note note[2][C];
     uint32_t list_n;  // of rank 0
     u64 scan_m[kWarps], scan_x[kWarps], res[3];
     uint32_t scan_c[kWarps];
     float red_a[kWarps], red_b[kWarps];
-    alignas(16) float row[1];  // this CTA's logits
+    alignas(16) float row[1];  // HOLD: this CTA's logits
 };
-template <int C>
+template <int C, bool HOLD>
 constexpr size_t smem_bytes(int chunk) {
-    return sizeof(Shared<C>) + (size_t)chunk * sizeof(float);
+    return sizeof(Shared<C, HOLD>) + (HOLD ? (size_t)chunk * sizeof(float) : 0);
 }
 
 __device__ __forceinline__ uint32_t at_rank(const void* p, uint32_t rank) {
@@ -130,6 +147,11 @@ __device__ __forceinline__ uint32_t at_rank(const void* p, uint32_t rank) {
 __device__ __forceinline__ uint32_t ld_rank(uint32_t addr) {
     uint32_t v;
     asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ u64 ld_rank64(uint32_t addr) {
+    u64 v;
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
     return v;
 }
 __device__ __forceinline__ void st_rank(uint32_t addr, u64 v) {
@@ -149,11 +171,11 @@ __device__ __forceinline__ u64 warp_scan(u64 v) {
     return v;
 }
 
-template <int C>
+template <int C, bool HOLD>
 __global__ void __launch_bounds__(kThreads, 2) draw_kernel(const __grid_constant__ DrawArgs a) {
-    using Sh = Shared<C>;
-    constexpr int NB = Sh::NB, SLICE = NB / C;
-    static_assert(SLICE <= kThreads, "a thread per bin of a slice");
+    using Sh = Shared<C, HOLD>;
+    constexpr int NB = Sh::NB, SLICE = NB / C, PER = SLICE > kThreads ? SLICE / kThreads : 1;  // bins: of a CTA, of a thread
+    static_assert(PER * kThreads == SLICE || PER == 1, "bins of a slice");
     extern __shared__ __align__(16) unsigned char smem_raw[];
     Sh& sh = *reinterpret_cast<Sh*>(smem_raw);
     const int tid = threadIdx.x, warp = tid / kWarp, lane = tid % kWarp;
@@ -191,8 +213,9 @@ __global__ void __launch_bounds__(kThreads, 2) draw_kernel(const __grid_constant
     };
     auto clear_bins = [&]() {
         for (int i = tid; i < NB; i += kThreads) {
-            sh.count[i] = sh.hi[i] = 0u;
-            sh.lo[i] = 0;
+            sh.bins.count[i] = sh.bins.hi[i] = 0u;
+            sh.bins.lo[i] = 0;
+            if constexpr (!HOLD) sh.bins.mass[i] = 0ull;
         }
     };
 
@@ -218,46 +241,56 @@ __global__ void __launch_bounds__(kThreads, 2) draw_kernel(const __grid_constant
 
     // ---- the row: this CTA holds tokens i0 .. i0 + n - 1 (chunk is even)
     const int i0 = min(a.vocab, rank * a.chunk), n = min(a.vocab, i0 + a.chunk) - i0;
-    float top = -INFINITY, least = INFINITY;
-    auto take = [&](float l, int i) {
-        l = fmaxf(l + 0.0f, -INFINITY);  // NaN becomes -inf, -0 becomes 0
-        sh.row[i] = l;
-        top = fmaxf(top, l);
-        least = fminf(least, l == -INFINITY ? INFINITY : l);
-    };
     const size_t base = (size_t)r * a.stride + i0;
-    if (a.bf16) {
-        const uint16_t* src = static_cast<const uint16_t*>(a.logits) + base;
-        if (reinterpret_cast<uintptr_t>(src) % 4 == 0) {
-            const uint32_t* two = reinterpret_cast<const uint32_t*>(src);
+    // f(logit, i) for this CTA's tokens i0 + i, i in [from, to): NaN as -inf, -0 as 0
+    auto from_memory = [&](int from, int to, auto f) {
+        auto clean = [&](float l, int i) { f(fmaxf(l + 0.0f, -INFINITY), i); };
+        const uint16_t* half = static_cast<const uint16_t*>(a.logits) + base;
+        if (a.bf16 && reinterpret_cast<uintptr_t>(half) % 4 == 0) {
+            const uint32_t* two = reinterpret_cast<const uint32_t*>(half);
             constexpr int kAhead = 8;
-            for (int j = tid; j < n / 2; j += kAhead * kThreads) {
+            const int end = to / 2;  // (from is even)
+            for (int j = from / 2 + tid; j < end; j += kAhead * kThreads) {
                 uint32_t x[kAhead];
 #pragma unroll
-                for (int v = 0; v < kAhead; ++v) x[v] = j + v * kThreads < n / 2 ? __ldg(two + j + v * kThreads) : 0u;
+                for (int v = 0; v < kAhead; ++v) x[v] = j + v * kThreads < end ? __ldg(two + j + v * kThreads) : 0u;
 #pragma unroll
                 for (int v = 0; v < kAhead; ++v)
-                    if (j + v * kThreads < n / 2) {
-                        take(bf16lo(x[v]), 2 * (j + v * kThreads));
-                        take(bf16hi(x[v]), 2 * (j + v * kThreads) + 1);
+                    if (j + v * kThreads < end) {
+                        clean(bf16lo(x[v]), 2 * (j + v * kThreads));
+                        clean(bf16hi(x[v]), 2 * (j + v * kThreads) + 1);
                     }
             }
-            if ((n & 1) && tid == 0) take(bf16lo(__ldg(src + n - 1)), n - 1);
+            if ((to & 1) && tid == 0) clean(bf16lo(__ldg(half + to - 1)), to - 1);
+        } else if (a.bf16) {
+            for (int i = from + tid; i < to; i += kThreads) clean(bf16lo(__ldg(half + i)), i);
         } else {
-            for (int i = tid; i < n; i += kThreads) take(bf16lo(__ldg(src + i)), i);
-        }
-    } else {
-        const float* src = static_cast<const float*>(a.logits) + base;
-        constexpr int kAhead = 16;
-        for (int j = tid; j < n; j += kAhead * kThreads) {
-            float x[kAhead];
+            const float* src = static_cast<const float*>(a.logits) + base;
+            constexpr int kAhead = 8;
+            for (int j = from + tid; j < to; j += kAhead * kThreads) {
+                float x[kAhead];
 #pragma unroll
-            for (int v = 0; v < kAhead; ++v) x[v] = j + v * kThreads < n ? __ldg(src + j + v * kThreads) : 0.0f;
+                for (int v = 0; v < kAhead; ++v) x[v] = j + v * kThreads < to ? __ldg(src + j + v * kThreads) : 0.0f;
 #pragma unroll
-            for (int v = 0; v < kAhead; ++v)
-                if (j + v * kThreads < n) take(x[v], j + v * kThreads);
+                for (int v = 0; v < kAhead; ++v)
+                    if (j + v * kThreads < to) clean(x[v], j + v * kThreads);
+            }
         }
-    }
+    };
+    auto each = [&](int from, int to, auto f) {
+        if constexpr (HOLD) {
+#pragma unroll 4
+            for (int i = from + tid; i < to; i += kThreads) f(sh.row[i], i);
+        } else {
+            from_memory(from, to, f);
+        }
+    };
+    float top = -INFINITY, least = INFINITY;
+    from_memory(0, n, [&](float l, int i) {
+        if constexpr (HOLD) sh.row[i] = l;
+        top = fmaxf(top, l);
+        least = fminf(least, l == -INFINITY ? INFINITY : l);
+    });
     auto warp_range = [&]() {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
@@ -290,8 +323,9 @@ __global__ void __launch_bounds__(kThreads, 2) draw_kernel(const __grid_constant
     }
     if (k == 1) {  // the first of the largest
         uint32_t first = 0xFFFFFFFFu;
-        for (int i = tid; i < n; i += kThreads)
-            if (sh.row[i] == top) first = min(first, (uint32_t)(i0 + i));
+        each(0, n, [&](float l, int i) {
+            if (l == top) first = min(first, (uint32_t)(i0 + i));
+        });
         first = __reduce_min_sync(kAll, first);
         if (lane == 0) sh.scan_c[warp] = first;
         __syncthreads();
@@ -314,50 +348,71 @@ __global__ void __launch_bounds__(kThreads, 2) draw_kernel(const __grid_constant
     const bool counts = k > 0;
 
     // Adds this CTA's tokens into the bins (bin0 >= 0: those of that bin between
-    // c_hi and c_lo, into bins of 2^shift places) and scans the sums: thread
-    // t < SLICE has bin rank SLICE + t.
-    u64 mass_ex, mass, all_mass, c_hi = ~0ull, c_lo = 0ull;
-    uint32_t count_ex, count, all_count;
+    // c_hi and c_lo, into bins of 2^shift places) and scans the sums: thread t has
+    // bins rank SLICE + PER t .. of the whole row.
+    u64 mass_ex = 0ull, mass[PER], all_mass, c_hi = ~0ull, c_lo = 0ull;
+    uint32_t count_ex = 0u, count[PER], all_count;
     int bin0 = -1, shift = 0;
     auto histogram = [&]() {
         const bool counted = counts || bin0 >= 0;
-#pragma unroll 4
-        for (int i = tid; i < n; i += kThreads) {
-            const float l = sh.row[i], x = rule.exponent(l);
-            int b = rule.bin(x);
-            if (bin0 >= 0) {
-                if (b != bin0) continue;
-                const u64 c = composite(l, i0 + i);
-                if (c < c_lo || c > c_hi) continue;
-                b = (int)((c_hi - c) >> shift);
-            }
-            const Weight w = rule.weight(l, x);
-            if (w.any()) {
-                atomicAdd(&sh.hi[b], w.hi);
-                atomicAdd(&sh.lo[b], w.lo);
-                if (counted) atomicAdd(&sh.count[b], 1u);
+        for (int from = 0; from < n; from += kBatch) {
+            each(from, min(n, from + kBatch), [&](float l, int i) {
+                const float x = rule.exponent(l);
+                int b = rule.bin(x);
+                if (bin0 >= 0) {
+                    if (b != bin0) return;
+                    const u64 c = composite(l, i0 + i);
+                    if (c < c_lo || c > c_hi) return;
+                    b = (int)((c_hi - c) >> shift);
+                }
+                const Weight w = rule.weight(l, x);
+                if (w.any()) {
+                    atomicAdd(&sh.bins.hi[b], w.hi);
+                    atomicAdd(&sh.bins.lo[b], w.lo);
+                    if (counted) atomicAdd(&sh.bins.count[b], 1u);
+                }
+            });
+            if constexpr (!HOLD) {
+                __syncthreads();
+                for (int i = tid; i < NB; i += kThreads) {
+                    sh.bins.mass[i] += ((u64)sh.bins.hi[i] << 17) + (u64)(long long)sh.bins.lo[i];
+                    sh.bins.hi[i] = 0u;
+                    sh.bins.lo[i] = 0;
+                }
+                __syncthreads();
             }
         }
         barrier();
-        mass = 0ull;
-        count = 0u;
-        if (tid < SLICE) {
-            const int b = rank * SLICE + tid;
-            uint32_t x[C], y[C], z[C];
+        u64 own_mass = 0ull;
+        uint32_t own_count = 0u;
 #pragma unroll
-            for (int c = 0; c < C; ++c) {
-                const uint32_t at = at_rank(&sh.count[b], c);
-                x[c] = ld_rank(at);
-                y[c] = ld_rank(at + NB * 4);
-                z[c] = ld_rank(at + 2 * NB * 4);
-            }
+        for (int k2 = 0; k2 < PER; ++k2) {
+            mass[k2] = 0ull;
+            count[k2] = 0u;
+            if (PER * tid < SLICE) {
+                const int b = rank * SLICE + PER * tid + k2;
+                uint32_t x[C], y[C], z[C];
+                u64 s[C];
 #pragma unroll
-            for (int c = 0; c < C; ++c) {
-                count += x[c];
-                mass += ((u64)y[c] << 17) + (u64)(long long)(int)z[c];
+                for (int c = 0; c < C; ++c) {
+                    x[c] = ld_rank(at_rank(&sh.bins.count[b], c));
+                    if constexpr (HOLD) {
+                        y[c] = ld_rank(at_rank(&sh.bins.hi[b], c));
+                        z[c] = ld_rank(at_rank(&sh.bins.lo[b], c));
+                    } else {
+                        s[c] = ld_rank64(at_rank(&sh.bins.mass[b], c));
+                    }
+                }
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    count[k2] += x[c];
+                    mass[k2] += HOLD ? ((u64)y[c] << 17) + (u64)(long long)(int)z[c] : s[c];
+                }
             }
+            own_mass += mass[k2];
+            own_count += count[k2];
         }
-        const u64 m = warp_scan(mass), nn = warp_scan(count);
+        const u64 m = warp_scan(own_mass), nn = warp_scan(own_count);
         if (lane == kWarp - 1) {
             sh.scan_m[warp] = m;
             sh.scan_c[warp] = (uint32_t)nn;
@@ -378,8 +433,8 @@ __global__ void __launch_bounds__(kThreads, 2) draw_kernel(const __grid_constant
             all_mass += t[c].a;
             all_count += (uint32_t)t[c].b;
         }
-        mass_ex = before_m + m - mass;
-        count_ex = (uint32_t)(before_n + nn) - count;
+        mass_ex = before_m + m - own_mass;
+        count_ex = (uint32_t)(before_n + nn) - own_count;
     };
 
     // ---- the questions: where the running count (of top_k) or weight sum (of
@@ -414,12 +469,22 @@ __global__ void __launch_bounds__(kThreads, 2) draw_kernel(const __grid_constant
                 }
             }
             // the bin that holds it: only its thread speaks up
-            const bool mine = tid < SLICE && (by_mass ? before_m + mass_ex < want && want <= before_m + mass_ex + mass
-                                                      : before_n + count_ex < want && want <= before_n + count_ex + count);
-            if (mine) {
-                sh.res[0] = mass_ex;
-                sh.res[1] = ((u64)(uint32_t)(rank * SLICE + tid + 1) << 32) | count;
-                sh.res[2] = count_ex;
+            bool mine = false;
+            {
+                u64 m_ex = mass_ex;
+                uint32_t n_ex = count_ex;
+#pragma unroll
+                for (int k2 = 0; k2 < PER; ++k2) {
+                    if (by_mass ? before_m + m_ex < want && want <= before_m + m_ex + mass[k2]
+                                : before_n + n_ex < want && want <= before_n + n_ex + count[k2]) {
+                        mine = true;
+                        sh.res[0] = m_ex;
+                        sh.res[1] = ((u64)(uint32_t)(rank * SLICE + PER * tid + k2 + 1) << 32) | count[k2];
+                        sh.res[2] = n_ex;
+                    }
+                    m_ex += mass[k2];
+                    n_ex += count[k2];
+                }
             }
             const bool here = __syncthreads_or(mine);
             Note note{0ull, 0ull, 0u, 0u};
@@ -451,12 +516,11 @@ __global__ void __launch_bounds__(kThreads, 2) draw_kernel(const __grid_constant
             const bool fits = counted && (uint32_t)bc <= kList;
             if (!counted || fits) {
                 // to the first CTA's list, as far as it goes
-#pragma unroll 4
-                for (int i = tid; i < n; i += kThreads) {
-                    const float l = sh.row[i], x = rule.exponent(l);
-                    if (rule.bin(x) != bin0) continue;
+                each(0, n, [&](float l, int i) {
+                    const float x = rule.exponent(l);
+                    if (rule.bin(x) != bin0) return;
                     const u64 c = composite(l, i0 + i);
-                    if (c < c_lo || c > c_hi || !rule.weight(l, x).any()) continue;
+                    if (c < c_lo || c > c_hi || !rule.weight(l, x).any()) return;
                     if constexpr (C == 1) {
                         const uint32_t s = atomicAdd(&sh.list_n, 1u);
                         if (s < kList) sh.list[s] = c;
@@ -464,7 +528,7 @@ __global__ void __launch_bounds__(kThreads, 2) draw_kernel(const __grid_constant
                         const uint32_t s = add_rank(counter, 1u);
                         if (s < kList) st_rank(list + 8 * s, c);
                     }
-                }
+                });
                 barrier();
                 sent = C == 1 ? sh.list_n : ld_rank(counter);
             }
@@ -512,14 +576,14 @@ __global__ void __launch_bounds__(kThreads, 2) draw_kernel(const __grid_constant
                 break;
             }
             // too many: divide the bin by (logit, index) between its extremes
-            for (int i = tid; i < n; i += kThreads) {
-                const float l = sh.row[i], x = rule.exponent(l);
-                if (rule.bin(x) != bin0) continue;
+            each(0, n, [&](float l, int i) {
+                const float x = rule.exponent(l);
+                if (rule.bin(x) != bin0) return;
                 const u64 c = composite(l, i0 + i);
-                if (c < c_lo || c > c_hi || !rule.weight(l, x).any()) continue;
+                if (c < c_lo || c > c_hi || !rule.weight(l, x).any()) return;
                 mx = max(mx, c);
                 mn = min(mn, c);
-            }
+            });
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) {
                 mx = max(mx, __shfl_xor_sync(kAll, mx, o));
@@ -556,13 +620,13 @@ __global__ void __launch_bounds__(kThreads, 2) draw_kernel(const __grid_constant
     }
 }
 
-template <int C>
+template <int C, bool HOLD>
 void launch(DrawArgs a, cudaStream_t st) {
     a.chunk = (((a.vocab + C - 1) / C) + 1) & ~1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)a.rows * C);
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem_bytes<C>(a.chunk);
+    cfg.dynamicSmemBytes = smem_bytes<C, HOLD>(a.chunk);
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -572,21 +636,30 @@ void launch(DrawArgs a, cudaStream_t st) {
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = C == 1 ? 1 : 2;
-    cudaLaunchKernelEx(&cfg, draw_kernel<C>, a);
+    cudaLaunchKernelEx(&cfg, draw_kernel<C, HOLD>, a);
 }
 
-constexpr int kOneCta = 16384;  // largest vocabulary that one CTA takes
+constexpr int kOneCta = 16384;  // largest vocabulary that one CTA holds
 
 }  // namespace
 
+// Two CTAs fit an SM: with the largest C whose CTAs run all at once, every SM
+// has work and a row's barriers are few.
 void launch_draw(const DrawArgs& a, cudaStream_t st) {
-    if (a.vocab <= kOneCta) launch<1>(a, st);
-    else launch<8>(a, st);
+    const int slots = 2 * device_sm_count();
+    if (a.vocab <= kOneCta) launch<1, true>(a, st);
+    else if (8 * a.rows <= slots) launch<8, true>(a, st);
+    else if (4 * a.rows <= slots) launch<4, false>(a, st);
+    else if (2 * a.rows <= slots) launch<2, false>(a, st);
+    else launch<1, false>(a, st);
 }
 
 void prepare_draw_kernels() {
-    configure_kernel((const void*)draw_kernel<1>, smem_bytes<1>(kOneCta));
-    configure_kernel((const void*)draw_kernel<8>, smem_bytes<8>(kDrawMaxVocab / 8));
+    configure_kernel((const void*)draw_kernel<1, true>, smem_bytes<1, true>(kOneCta));
+    configure_kernel((const void*)draw_kernel<8, true>, smem_bytes<8, true>(kDrawMaxVocab / 8));
+    configure_kernel((const void*)draw_kernel<4, false>, smem_bytes<4, false>(0));
+    configure_kernel((const void*)draw_kernel<2, false>, smem_bytes<2, false>(0));
+    configure_kernel((const void*)draw_kernel<1, false>, smem_bytes<1, false>(0));
 }
 
 }  // namespace zc
