@@ -59,45 +59,40 @@ static_assert(kDrawMaxVocab == 1 << kIndexBits, "composite keys");
 
 // The place of a token in the order as one number: larger = earlier.
 __device__ __forceinline__ u64 composite(float l, int idx) {
-    return ((argmax_key(l, 0u) >> 32) << kIndexBits) | (u64)((1 << kIndexBits) - 1 - idx);
+    return ((argmax_key(l + 0.0f, 0u) >> 32) << kIndexBits) | (u64)((1 << kIndexBits) - 1 - idx);  // (-0 is 0)
 }
 __device__ __forceinline__ float composite_logit(u64 c) {
     const uint32_t k = (uint32_t)(c >> kIndexBits);
     return __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k);
 }
 
-// rint(e 2^33) = hi 2^17 + lo, lo in [-2^16, 2^16): both parts by adding 2^23
+// rint(e 2^33) = hi 2^17 + lo, lo in [-2^16, 2^16]: both parts by adding 2^23
 // (1.5 2^23 for the signed one). e 2^16 and the remainder are exact, and hi 2^17
 // is even, so rounding the remainder alone rounds the whole the same way. The
-// sums of 2^15 such words fit 32 bits.
+// sums of kBatch such words fit 32 bits.
 struct Weight {
     uint32_t hi;
     int lo;
-    __device__ __forceinline__ bool any() const { return (hi | (uint32_t)lo) != 0u; }
     __device__ __forceinline__ u64 whole() const { return ((u64)hi << 17) + (u64)(long long)lo; }
 };
 
 struct RowRule {
-    float m, inv_t, min_p, end, bin_scale;
-    __device__ __forceinline__ float exponent(float l) const { return l == m ? 0.0f : (l - m) * inv_t; }
+    float m, inv_t, end, bin_scale;
+    float least;  // the smallest exponential with weight: min_p, or the float after 2^-34 (which rounds to 0)
+    bool odd;     // m is infinite: l - m is not 0 where l is m
+    __device__ __forceinline__ float exponent(float l) const {
+        const float d = l - m;
+        return (odd && l == m ? 0.0f : d) * inv_t;
+    }
     __device__ __forceinline__ int bin(float x) const {
         return __float_as_int(__fmaf_rn(fminf(-x, end), bin_scale, kMagic)) - 0x4B000000;
     }
-    // (a logit of -inf has exponent -inf, or NaN where 1 / T is 0: no weight)
-    __device__ __forceinline__ Weight weight(float l, float x) const {
-        const float e = expf(x);
-        Weight w{0u, 0};
-        if (e >= min_p && l != -INFINITY) {
-            const float s = e * 65536.0f, t = s + kMagic;
-            const float rem = (s - (t - kMagic)) * 131072.0f;
-            w.hi = (uint32_t)(__float_as_int(t) - 0x4B000000);
-            w.lo = __float_as_int(rem + 12582912.0f) - 0x4B400000;
-            if (w.lo == 65536) {
-                w.lo = -65536;
-                w.hi += 1u;
-            }
-        }
-        return w;
+    // does a token of exponential e weigh anything? (NaN does not)
+    __device__ __forceinline__ bool weighs(float e) const { return e >= least; }
+    __device__ __forceinline__ Weight weight(float e) const {
+        const float s = e * 65536.0f, t = s + kMagic;
+        return Weight{(uint32_t)(__float_as_int(t) - 0x4B000000),
+                      __float_as_int(__fmaf_rn(s - (t - kMagic), 131072.0f, 12582912.0f)) - 0x4B400000};
     }
 };
 
@@ -110,7 +105,7 @@ struct Note {
 // HOLD: the row's part stays in shared memory (of at most kBatch tokens);
 // otherwise it is read again, and the bins' 32-bit sums are carried over into
 // 64-bit ones every kBatch tokens.
-constexpr int kBatch = 1 << 15;
+constexpr int kBatch = (1 << 15) - 2;
 template <int NB, bool HOLD>
 struct Bins {
     uint32_t count[NB], hi[NB];  // tokens, and their weights' parts
@@ -242,39 +237,46 @@ __global__ void __launch_bounds__(kThreads, 2) draw_kernel(const __grid_constant
     // ---- the row: this CTA holds tokens i0 .. i0 + n - 1 (chunk is even)
     const int i0 = min(a.vocab, rank * a.chunk), n = min(a.vocab, i0 + a.chunk) - i0;
     const size_t base = (size_t)r * a.stride + i0;
-    // f(logit, i) for this CTA's tokens i0 + i, i in [from, to): NaN as -inf, -0 as 0
+    // f(logit, i) for this CTA's tokens i0 + i, i in [from, to), kAhead loads before any is used
     auto from_memory = [&](int from, int to, auto f) {
-        auto clean = [&](float l, int i) { f(fmaxf(l + 0.0f, -INFINITY), i); };
+        constexpr int kAhead = 8;
         const uint16_t* half = static_cast<const uint16_t*>(a.logits) + base;
         if (a.bf16 && reinterpret_cast<uintptr_t>(half) % 4 == 0) {
             const uint32_t* two = reinterpret_cast<const uint32_t*>(half);
-            constexpr int kAhead = 8;
             const int end = to / 2;  // (from is even)
-            for (int j = from / 2 + tid; j < end; j += kAhead * kThreads) {
+            int j = from / 2 + tid;
+            for (; j + (kAhead - 1) * kThreads < end; j += kAhead * kThreads) {
                 uint32_t x[kAhead];
 #pragma unroll
-                for (int v = 0; v < kAhead; ++v) x[v] = j + v * kThreads < end ? __ldg(two + j + v * kThreads) : 0u;
+                for (int v = 0; v < kAhead; ++v) x[v] = __ldg(two + j + v * kThreads);
 #pragma unroll
-                for (int v = 0; v < kAhead; ++v)
-                    if (j + v * kThreads < end) {
-                        clean(bf16lo(x[v]), 2 * (j + v * kThreads));
-                        clean(bf16hi(x[v]), 2 * (j + v * kThreads) + 1);
-                    }
+                for (int v = 0; v < kAhead; ++v) {
+                    f(bf16lo(x[v]), 2 * (j + v * kThreads));
+                    f(bf16hi(x[v]), 2 * (j + v * kThreads) + 1);
+                }
             }
-            if ((to & 1) && tid == 0) clean(bf16lo(__ldg(half + to - 1)), to - 1);
+#pragma unroll 1
+            for (; j < end; j += kThreads) {
+                const uint32_t x = __ldg(two + j);
+                f(bf16lo(x), 2 * j);
+                f(bf16hi(x), 2 * j + 1);
+            }
+            if ((to & 1) && tid == 0) f(bf16lo(__ldg(half + to - 1)), to - 1);
         } else if (a.bf16) {
-            for (int i = from + tid; i < to; i += kThreads) clean(bf16lo(__ldg(half + i)), i);
+#pragma unroll 4
+            for (int i = from + tid; i < to; i += kThreads) f(bf16lo(__ldg(half + i)), i);
         } else {
             const float* src = static_cast<const float*>(a.logits) + base;
-            constexpr int kAhead = 8;
-            for (int j = from + tid; j < to; j += kAhead * kThreads) {
+            int j = from + tid;
+            for (; j + (kAhead - 1) * kThreads < to; j += kAhead * kThreads) {
                 float x[kAhead];
 #pragma unroll
-                for (int v = 0; v < kAhead; ++v) x[v] = j + v * kThreads < to ? __ldg(src + j + v * kThreads) : 0.0f;
+                for (int v = 0; v < kAhead; ++v) x[v] = __ldg(src + j + v * kThreads);
 #pragma unroll
-                for (int v = 0; v < kAhead; ++v)
-                    if (j + v * kThreads < to) clean(x[v], j + v * kThreads);
+                for (int v = 0; v < kAhead; ++v) f(x[v], j + v * kThreads);
             }
+#pragma unroll 4
+            for (; j < to; j += kThreads) f(__ldg(src + j), j);
         }
     };
     auto each = [&](int from, int to, auto f) {
@@ -288,8 +290,8 @@ __global__ void __launch_bounds__(kThreads, 2) draw_kernel(const __grid_constant
     float top = -INFINITY, least = INFINITY;
     from_memory(0, n, [&](float l, int i) {
         if constexpr (HOLD) sh.row[i] = l;
-        top = fmaxf(top, l);
-        least = fminf(least, l == -INFINITY ? INFINITY : l);
+        top = fmaxf(top, l);  // (NaN is passed over)
+        least = fminf(least, l);
     });
     auto warp_range = [&]() {
 #pragma unroll
@@ -340,8 +342,9 @@ __global__ void __launch_bounds__(kThreads, 2) draw_kernel(const __grid_constant
     }
 
     // ---- bins even in (m - l) / T, up to the last weight
-    RowRule rule{top, 1.0f / T, min_p, 0.0f, 0.0f};
-    rule.end = fminf(-rule.exponent(least), kEnd);
+    // (1 / T beyond the floats: the largest of them gives the same zeros)
+    RowRule rule{top, fminf(1.0f / T, 3.402823466e38f), 0.0f, 0.0f, fmaxf(min_p, 5.8207667e-11f), top == INFINITY};
+    rule.end = fminf(-rule.exponent(least), kEnd);  // (with a logit of -inf in the row: where weights end)
     if (!(rule.end >= 0.0f)) rule.end = kEnd;
     if (min_p > 0.0f) rule.end = fminf(rule.end, 0.01f - logf(min_p));
     rule.bin_scale = rule.end > 0.0f ? (float)(NB - 1) / rule.end : 0.0f;
@@ -357,7 +360,7 @@ __global__ void __launch_bounds__(kThreads, 2) draw_kernel(const __grid_constant
         const bool counted = counts || bin0 >= 0;
         for (int from = 0; from < n; from += kBatch) {
             each(from, min(n, from + kBatch), [&](float l, int i) {
-                const float x = rule.exponent(l);
+                const float x = rule.exponent(l), e = expf(x);
                 int b = rule.bin(x);
                 if (bin0 >= 0) {
                     if (b != bin0) return;
@@ -365,8 +368,8 @@ __global__ void __launch_bounds__(kThreads, 2) draw_kernel(const __grid_constant
                     if (c < c_lo || c > c_hi) return;
                     b = (int)((c_hi - c) >> shift);
                 }
-                const Weight w = rule.weight(l, x);
-                if (w.any()) {
+                if (rule.weighs(e)) {
+                    const Weight w = rule.weight(e);
                     atomicAdd(&sh.bins.hi[b], w.hi);
                     atomicAdd(&sh.bins.lo[b], w.lo);
                     if (counted) atomicAdd(&sh.bins.count[b], 1u);
@@ -509,18 +512,29 @@ __global__ void __launch_bounds__(kThreads, 2) draw_kernel(const __grid_constant
                 c_lo = max(c_lo, hi - ((1ull << shift) - 1ull));
                 c_hi = hi;
             }
+            // the bin's logits lie between these (a bin's width and a few roundings of
+            // slack): a comparison leaves few tokens to look at closely
+            const float width = rule.bin_scale > 0.0f ? T / rule.bin_scale : INFINITY, slack = width + 1e-6f * fabsf(top);
+            const float l_hi = bin0 < 2 ? INFINITY : top - ((float)bin0 * width - slack) * (1.0f - 1e-6f);
+            const float l_lo = bin0 >= NB - 2 ? -INFINITY : top - ((float)bin0 * width + slack) * (1.0f + 1e-6f);
             u64 mx = 0ull, mn = ~0ull;
             uint32_t sent = 0u;
+            // f(place, its logit) of each of this CTA's tokens in the bin
+            auto chosen = [&](auto f) {
+                each(0, n, [&](float l, int i) {
+                    if (!(l <= l_hi) || l < l_lo) return;
+                    const float x = rule.exponent(l);
+                    if (rule.bin(x) != bin0 || !rule.weighs(expf(x))) return;
+                    const u64 c = composite(l, i0 + i);
+                    if (c >= c_lo && c <= c_hi) f(c);
+                });
+            };
             const bool counted = counts || held == 2;
             const uint32_t counter = C == 1 ? 0u : at_rank(&sh.list_n, 0), list = C == 1 ? 0u : at_rank(sh.list, 0);
             const bool fits = counted && (uint32_t)bc <= kList;
             if (!counted || fits) {
                 // to the first CTA's list, as far as it goes
-                each(0, n, [&](float l, int i) {
-                    const float x = rule.exponent(l);
-                    if (rule.bin(x) != bin0) return;
-                    const u64 c = composite(l, i0 + i);
-                    if (c < c_lo || c > c_hi || !rule.weight(l, x).any()) return;
+                chosen([&](u64 c) {
                     if constexpr (C == 1) {
                         const uint32_t s = atomicAdd(&sh.list_n, 1u);
                         if (s < kList) sh.list[s] = c;
@@ -554,7 +568,7 @@ __global__ void __launch_bounds__(kThreads, 2) draw_kernel(const __grid_constant
                             c = larger ? max(c, other) : min(c, other);
                         }
                     const float l = composite_logit(c);
-                    const u64 w = c ? rule.weight(l, rule.exponent(l)).whole() : 0ull;
+                    const u64 w = c ? rule.weight(expf(rule.exponent(l))).whole() : 0ull;
                     const u64 m = warp_scan(w);
                     if (lane == kWarp - 1) sh.scan_x[warp] = m;
                     __syncthreads();
@@ -576,11 +590,7 @@ __global__ void __launch_bounds__(kThreads, 2) draw_kernel(const __grid_constant
                 break;
             }
             // too many: divide the bin by (logit, index) between its extremes
-            each(0, n, [&](float l, int i) {
-                const float x = rule.exponent(l);
-                if (rule.bin(x) != bin0) return;
-                const u64 c = composite(l, i0 + i);
-                if (c < c_lo || c > c_hi || !rule.weight(l, x).any()) return;
+            chosen([&](u64 c) {
                 mx = max(mx, c);
                 mn = min(mn, c);
             });
@@ -648,7 +658,7 @@ constexpr int kOneCta = 16384;  // largest vocabulary that one CTA holds
 void launch_draw(const DrawArgs& a, cudaStream_t st) {
     const int slots = 2 * device_sm_count();
     if (a.vocab <= kOneCta) launch<1, true>(a, st);
-    else if (8 * a.rows <= slots) launch<8, true>(a, st);
+    else if (8 * a.rows <= slots && a.vocab <= 8 * kBatch) launch<8, true>(a, st);
     else if (4 * a.rows <= slots) launch<4, false>(a, st);
     else if (2 * a.rows <= slots) launch<2, false>(a, st);
     else launch<1, false>(a, st);
@@ -656,7 +666,7 @@ void launch_draw(const DrawArgs& a, cudaStream_t st) {
 
 void prepare_draw_kernels() {
     configure_kernel((const void*)draw_kernel<1, true>, smem_bytes<1, true>(kOneCta));
-    configure_kernel((const void*)draw_kernel<8, true>, smem_bytes<8, true>(kDrawMaxVocab / 8));
+    configure_kernel((const void*)draw_kernel<8, true>, smem_bytes<8, true>(kBatch));
     configure_kernel((const void*)draw_kernel<4, false>, smem_bytes<4, false>(0));
     configure_kernel((const void*)draw_kernel<2, false>, smem_bytes<2, false>(0));
     configure_kernel((const void*)draw_kernel<1, false>, smem_bytes<1, false>(0));
