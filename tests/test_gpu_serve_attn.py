@@ -452,3 +452,22 @@ def test_shared_tiles_keep_nan_in_its_dims():
     keep = torch.tensor([d for d in range(D) if d != 7], device="cuda")
     check(out[..., keep], want[..., keep], clean, "f32")
     assert torch.isfinite(out[:, [0, 1, 4, 5, 6, 7]]).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("lens,tokens,window,sinks", [([2900], 2, zc.WINDOW_ALL, 0), ([2900, 700], 33, 2000, 5), ([3000, 64, 1500], 64, 1024, 70)])
+def test_few_queries_with_many_keys(lens, tokens, window, sinks, dtype):
+    """A tile's keys shared by several CTAs, rows of one batch with very different ranges."""
+    m = make(n_kv=2, max_seq_len=3008)
+    k = [normal(70 + i, 2, n, D, dtype=torch.bfloat16) for i, n in enumerate(lens)]
+    v = [normal(80 + i, 2, n, D, dtype=torch.bfloat16) for i, n in enumerate(lens)]
+    for s, (a, b) in enumerate(zip(k, v)):
+        m.kv_write(s, 0, 0, a, b)
+    q = normal(90, len(lens), tokens, 4, D, dtype=DTYPES[dtype], scale=1.5)
+    out = torch.full_like(q, float("nan"))
+    torch.cuda.synchronize()
+    for _ in range(2):
+        m.attn_window(0, range(len(lens)), q, out, window=window, sinks=sinks)
+    m.gpu.sync()
+    for i, n in enumerate(lens):
+        check(out[i], reference(q[i], k[i], v[i], window_seen(n, tokens, window, sinks)), v[i], dtype)

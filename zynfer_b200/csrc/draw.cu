@@ -29,14 +29,15 @@
 //      that bin, which all CTAs send to the first, where they are sorted and
 //      their weights scanned. A bin of more tokens than that list holds (many
 //      equal logits) is divided again, by (logit, index) itself, until it fits.
-// A few rows are bound by the chain of loads, exchanges and barriers (25 us for
-// one row of 151936), many rows by the instructions per logit (about 50, an
-// accurate exponential among them), not by the bytes. So C is the more CTAs the
-// fewer rows there are: 8 for up to 37 rows, then 4, 2 and 1 (256 rows: LATER us
-// with one CTA a row, 206 with eight, whose barriers left the SMs idle); weights
-// are split into two 32-bit words without integer conversions; and two CTAs
-// share an SM. Eight CTAs hold their parts of a row in shared memory, fewer
-// read them again from L2.
+// A few rows are bound by the chain of loads, exchanges and barriers (20 us for
+// one row of 151936), many rows by the instructions per logit (about 40, an
+// accurate exponential among them), not by the bytes. So a row has the more CTAs
+// the fewer rows there are: 16 for up to 4, 8 for up to 37, then 4, 2 and 1 (256
+// rows of bf16: 123 us a call with one CTA a row against 206 with eight, whose
+// barriers left the SMs idle; 88 with half the instructions since); weights are
+// split into two 32-bit words without integer conversions; and two CTAs share an
+// SM. Eight CTAs or more hold their parts of a row in shared memory, fewer read
+// them again from L2.
 #include <type_traits>
 
 #include "common.cuh"
@@ -631,14 +632,12 @@ __global__ void __launch_bounds__(kThreads, 2) draw_kernel(const __grid_constant
 }
 
 template <int C, bool HOLD>
-void launch(DrawArgs a, cudaStream_t st) {
-    a.chunk = (((a.vocab + C - 1) / C) + 1) & ~1;
+cudaLaunchConfig_t config(const DrawArgs& a, cudaLaunchAttribute* attr, cudaStream_t st) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)a.rows * C);
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = smem_bytes<C, HOLD>(a.chunk);
     cfg.stream = st;
-    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
@@ -646,10 +645,40 @@ void launch(DrawArgs a, cudaStream_t st) {
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = C == 1 ? 1 : 2;
+    return cfg;
+}
+
+template <int C, bool HOLD>
+void launch(DrawArgs a, cudaStream_t st) {
+    a.chunk = (((a.vocab + C - 1) / C) + 1) & ~1;
+    cudaLaunchAttribute attr[2];
+    const cudaLaunchConfig_t cfg = config<C, HOLD>(a, attr, st);
     cudaLaunchKernelEx(&cfg, draw_kernel<C, HOLD>, a);
 }
 
 constexpr int kOneCta = 16384;  // largest vocabulary that one CTA holds
+// A few rows of a large vocabulary take 16 CTAs each (one row of 151936: 19.8 us
+// against 22.1 with 8; 4 rows 24.9 / 27.8; but 8 rows 30.7 / 27.9, and one row of
+// 32000 17.0 / 16.6). Clusters of 16 are more than every GPU must offer.
+constexpr int kWideRows = 4, kWideVocab = 65536;
+bool wide_clusters_fit() {
+    static int fit[64] = {0};  // by device: 0 not asked, 1 yes, 2 no
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64) return false;
+    if (!fit[dev]) {
+        DrawArgs a{};
+        a.rows = 1;
+        a.chunk = kDrawMaxVocab / 16;
+        cudaLaunchAttribute attr[2];
+        const cudaLaunchConfig_t cfg = config<16, true>(a, attr, nullptr);
+        int n = 0;
+        const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, draw_kernel<16, true>, &cfg);
+        if (e != cudaSuccess) cudaGetLastError();
+        fit[dev] = e == cudaSuccess && n >= kWideRows ? 1 : 2;
+    }
+    return fit[dev] == 1;
+}
 
 }  // namespace
 
@@ -658,6 +687,7 @@ constexpr int kOneCta = 16384;  // largest vocabulary that one CTA holds
 void launch_draw(const DrawArgs& a, cudaStream_t st) {
     const int slots = 2 * device_sm_count();
     if (a.vocab <= kOneCta) launch<1, true>(a, st);
+    else if (a.rows <= kWideRows && a.vocab > kWideVocab && wide_clusters_fit()) launch<16, true>(a, st);
     else if (8 * a.rows <= slots && a.vocab <= 8 * kBatch) launch<8, true>(a, st);
     else if (4 * a.rows <= slots) launch<4, false>(a, st);
     else if (2 * a.rows <= slots) launch<2, false>(a, st);
@@ -666,6 +696,9 @@ void launch_draw(const DrawArgs& a, cudaStream_t st) {
 
 void prepare_draw_kernels() {
     configure_kernel((const void*)draw_kernel<1, true>, smem_bytes<1, true>(kOneCta));
+    configure_kernel((const void*)draw_kernel<16, true>, smem_bytes<16, true>(kDrawMaxVocab / 16));
+    cudaFuncSetAttribute(draw_kernel<16, true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    wide_clusters_fit();  // (asked now, never during a graph capture)
     configure_kernel((const void*)draw_kernel<8, true>, smem_bytes<8, true>(kBatch));
     configure_kernel((const void*)draw_kernel<4, false>, smem_bytes<4, false>(0));
     configure_kernel((const void*)draw_kernel<2, false>, smem_bytes<2, false>(0));

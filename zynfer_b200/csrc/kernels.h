@@ -242,6 +242,8 @@ inline TileListT<N> first_tiles(const TileList& l, int items) {
 }
 // Cache blocks that a query at `pos` sees after the first `skip`.
 int serve_span_blocks(int pos, uint32_t window, int sinks, int skip);
+// Those that a tile of queries at p0 .. p1 sees.
+int serve_tile_blocks(int p0, int p1, uint32_t window, int sinks);
 void launch_serve_merge(const ServeRows& rows, const ServeAttnArgs& a, cudaStream_t st);
 struct KvWriteArgs {
     uint16_t* kv_layer;

@@ -926,8 +926,26 @@ int plan_serve(ZynferCuCtx* c, uint32_t batch, uint32_t tokens, uint32_t window,
     if (tokens > 1) {
         p->chunk = true;
         c->serve_tiles.n = 0;
-        p->items = (int)((long long)batch * ((tokens + 63) / 64) * c->d.n_kv);
-        return ZYNFER_CU_OK;
+        const uint32_t per_seq = (tokens + 63) / 64;
+        p->items = (int)((long long)batch * per_seq * c->d.n_kv);
+        // few tiles of queries with many tiles of keys: several CTAs share one's keys, at
+        // least kSplitTiles each, if all then run at once
+        int longest = 0;
+        for (uint32_t i = 0; i < batch; ++i) {
+            const int p1 = rows.r[i].len - 1, p0 = std::max(rows.r[i].len - (int)tokens, p1 - 63);
+            longest = std::max(longest, serve_tile_blocks(p0, p1, window, (int)std::min<uint32_t>(sinks, c->d.max_seq_len)));
+        }
+        constexpr int kSplitTiles = 4;
+        const int tiles = (longest + kAttnTileBlocks - 1) / kAttnTileBlocks;
+        p->nsplit = std::max(1, std::min(sms * attn_tile_ctas(bf16) / p->items, tiles / kSplitTiles));
+        // (a split in two gains a third of one call's time, 43 -> 32 us for 512 f32 queries with
+        // a window of 1024, and loses as much where other streams fill the GPU; 16
+        // queries over 8000 keys, split in sixteen: 245 -> 26 us)
+        if (p->nsplit < 3) p->nsplit = 1;
+        if (p->nsplit == 1) return ZYNFER_CU_OK;
+        p->items *= p->nsplit;
+        p->max_segs = p->nsplit;
+        return serve_scratch(c, (size_t)batch * tokens * c->d.n_q * p->max_segs * kServeRecord);
     }
     c->serve_tiles.n = 0;
     int tile_segs = 1;
