@@ -65,3 +65,12 @@ def test_backends_lists_every_kind():
     text = out.getvalue()
     for k in ("cpu", "apple", "amd-hip", "cuda"):
         assert k in text
+
+
+@pytest.mark.parametrize("flags", [["--samples", "0"], ["--samples", "1025"], ["--new-tokens", "0"], ["--window", "0"],
+                                   ["--sinks", "4"], ["--top-p", "0"], ["--min-p", "1.5"], ["--top-k", "-1"],
+                                   ["--prompt-tokens", "0"]])
+def test_sample_rejects_bad_limits_before_any_device_work(flags):
+    with pytest.raises(SystemExit) as e:
+        cli.main(["sample", "--backend", "cuda", *flags])
+    assert e.value.code == 2

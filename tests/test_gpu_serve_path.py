@@ -126,3 +126,22 @@ def test_refusals():
     assert m.seq_len(0) == 10
     m.decode_drawn([0], [1], [0.1])
     assert m.seq_len(0) == 11
+
+
+def test_cli_sample(capsys):
+    import json
+
+    from zynfer_b200 import cli
+    base = ["sample", "--backend", "cuda", "--prompt-tokens", "1100", "--samples", "3", "--new-tokens", "4", "--seed", "7"]
+
+    def run(*flags):
+        assert cli.main([*base, *flags]) == 0
+        return json.loads(capsys.readouterr().out)
+
+    a, b = run("--temperature", "0.9", "--top-p", "0.95"), run("--temperature", "0.9", "--top-p", "0.95")
+    assert a["ids"] == b["ids"] and a["logprobs"] == b["logprobs"]       # the seed decides
+    assert np.array(a["ids"]).shape == (3, 4) and all(x < 0 for x in a["logprobs"])
+    greedy = run("--temperature", "0")
+    assert greedy["ids"][0] == greedy["ids"][1] == greedy["ids"][2] and greedy["logprobs"] == [0.0] * 3
+    windowed = run("--temperature", "0", "--window", "128", "--sinks", "4")
+    assert np.array(windowed["ids"]).shape == (3, 4)

@@ -4,6 +4,9 @@
     python -m zynfer_b200.cli forward-golden MODEL.zynfer [--tokens 151643,2,3] [--golden LOGITS.f32] [--backend cuda]
     python -m zynfer_b200.cli decode-bench [--backend cuda] [--artifact MODEL.zynfer] [--batch B] [--prefill-tokens T]
                                            [--decode-steps S] [--warmup W] [--iters I]
+    python -m zynfer_b200.cli sample [--artifact MODEL.zynfer] [--tokens 151643,2,3 | --prompt-tokens T] [--samples N]
+                                     [--new-tokens S] [--temperature T] [--top-k K] [--top-p P] [--min-p M] [--seed S]
+                                     [--window W [--sinks K]]
 
 `--backend` (else ZYNFER_BACKEND, else the default kind) resolves through the
 reference's rules (src/main.zig:58-64,110-114; backend.zig:106-130, mirrored in
@@ -25,6 +28,14 @@ warmup, iters, metal_init_ns, peak_rss_bytes, energy_per_token,
 cpu_prefill_ns, cpu_decode_ns_per_token, apple_prefill_ns,
 apple_decode_ns_per_token, apple_block_path) plus this backend's cuda_* keys.
 Keys of backends that did not run are null, as block-bench prints them.
+
+sample (no counterpart in the reference) draws N continuations of one prompt:
+the prompt is prefilled once in chunks, forked N - 1 times over the paged
+cache, and every decode step's attention reads the common prompt once for all
+of them; each token is drawn from a random number of the seeded generator
+under the rule of zynfer_cu_sample_rows. With --window the model's attention
+is windowed (the first --sinks positions stay visible) in prefill and decode.
+Prints one JSON line: the ids and summed log-probabilities of each sample.
 """
 from __future__ import annotations
 
@@ -208,6 +219,70 @@ def decode_bench(args, out=None) -> int:
     return 0
 
 
+def check_sample(args):
+    """The sample command's limits, before any device work."""
+    if args.samples < 1 or args.samples > 1024 or args.new_tokens < 1:
+        raise CliError("sample: --samples 1..1024, --new-tokens at least 1")
+    if args.window is not None and args.window < 1:
+        raise CliError("sample: --window must be at least 1")
+    if args.sinks < 0 or (args.sinks and args.window is None):
+        raise CliError("sample: --sinks goes with --window")
+    if args.top_k < 0 or not 0.0 < args.top_p <= 1.0 or not 0.0 <= args.min_p <= 1.0:
+        raise CliError("sample: --top-k >= 0, 0 < --top-p <= 1, 0 <= --min-p <= 1")
+    if not args.tokens and args.prompt_tokens < 1:
+        raise CliError("sample: --prompt-tokens at least 1")
+
+
+def sample(args, out=None) -> int:
+    out = out or sys.stdout
+    kind = resolve(args.backend)
+    check_sample(args)
+    from . import cuda
+    from . import workload
+    window = cuda.WINDOW_ALL if args.window is None else args.window
+    chunk = 1024  # prompt tokens per prefill call
+
+    def sizes(n):
+        blocks = n // 16 + 1 + args.samples * (args.new_tokens // 16 + 2)  # the prompt once, and each sample's own
+        return dict(max_batch=args.samples, max_seqs=args.samples, max_seq_len=n + args.new_tokens, kv_blocks=blocks,
+                    max_prefill=min(chunk, n))
+
+    gpu = cuda.Gpu(args.device)
+    try:
+        if args.artifact:
+            from . import artifact as A
+            with A.Artifact(args.artifact) as art:
+                ids = parse_tokens(args.tokens) if args.tokens else list(workload.prompt(0, args.prompt_tokens, args.seed, art.meta().vocab))
+                model = cuda.Model(gpu, art.arch(), _weights_kind(art), **sizes(len(ids)))
+                model.load_artifact(art)
+        else:
+            ids = parse_tokens(args.tokens) if args.tokens else list(workload.prompt(0, args.prompt_tokens, args.seed, cuda.QWEN3_0_6B.vocab))
+            model = cuda.Model(gpu, cuda.QWEN3_0_6B, cuda.W_Q8, **sizes(len(ids)))
+            model.fill_synthetic(args.seed, 0.02, 0.0)
+        # every prompt token but the last goes into the cache; the last is the first step's input
+        for at in range(0, len(ids) - 1, chunk):
+            model.prefill_chunk(0, ids[at:min(at + chunk, len(ids) - 1)], window=window, sinks=args.sinks, want_logits=False)
+        slots = list(range(args.samples))
+        for s in slots[1:]:
+            model.seq_fork(s, 0, len(ids) - 1)
+        rng = np.random.default_rng(args.seed)
+        tokens, got, logprob, ns = [ids[-1]] * args.samples, [], np.zeros(args.samples), 0
+        for _ in range(args.new_tokens):
+            tokens, lp = model.decode_drawn(slots, tokens, rng.random(args.samples, dtype=np.float32), temperature=args.temperature,
+                                            top_k=args.top_k, top_p=args.top_p, min_p=args.min_p, window=window, sinks=args.sinks)
+            got.append(tokens)
+            logprob += lp
+            ns += gpu.last_step_ns
+        path, launches = gpu.last_path, gpu.step_launches
+    finally:
+        gpu.close()
+    line = {"backend": kind.value, "prompt_tokens": len(ids), "samples": args.samples, "new_tokens": args.new_tokens,
+            "ids": np.stack(got, 1).tolist(), "logprobs": [float(x) for x in logprob], "cuda_decode_ns_per_step": int(ns / args.new_tokens),
+            "cuda_block_path": path, "cuda_launches_per_step": launches}
+    out.write(json.dumps(line) + "\n")
+    return 0
+
+
 def backends(args, out=None) -> int:
     out = out or sys.stdout
     """printBackends (main.zig): every kind with whether this build has it."""
@@ -238,6 +313,20 @@ def parse(argv=None):
     db.add_argument("--iters", type=int, default=3)
     db.add_argument("--seed", type=int, default=20250601)
     db.add_argument("--backend", dest="backend_sub", default=None)
+    sp = sub.add_parser("sample")
+    sp.add_argument("--artifact", default=None)
+    sp.add_argument("--tokens", default=None)
+    sp.add_argument("--prompt-tokens", type=int, default=512)
+    sp.add_argument("--samples", type=int, default=8)
+    sp.add_argument("--new-tokens", type=int, default=32)
+    sp.add_argument("--temperature", type=float, default=1.0)
+    sp.add_argument("--top-k", type=int, default=0)
+    sp.add_argument("--top-p", type=float, default=1.0)
+    sp.add_argument("--min-p", type=float, default=0.0)
+    sp.add_argument("--seed", type=int, default=20250601)
+    sp.add_argument("--window", type=int, default=None)
+    sp.add_argument("--sinks", type=int, default=0)
+    sp.add_argument("--backend", dest="backend_sub", default=None)
     args = ap.parse_args(argv)
     if getattr(args, "backend_sub", None):
         args.backend = args.backend_sub
@@ -246,7 +335,7 @@ def parse(argv=None):
 
 def main(argv=None) -> int:
     args = parse(argv)
-    return {"backends": backends, "forward-golden": forward_golden, "decode-bench": decode_bench}[args.cmd](args)
+    return {"backends": backends, "forward-golden": forward_golden, "decode-bench": decode_bench, "sample": sample}[args.cmd](args)
 
 
 if __name__ == "__main__":

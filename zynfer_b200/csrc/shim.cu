@@ -966,7 +966,7 @@ int plan_serve(ZynferCuCtx* c, uint32_t batch, uint32_t tokens, uint32_t window,
     return serve_scratch(c, (size_t)batch * c->d.n_q * p->max_segs * kServeRecord);
 }
 
-void enqueue_serve(ZynferCuCtx* c, const ServePlan& p, ServeAttnArgs a) {
+int enqueue_serve(ZynferCuCtx* c, const ServePlan& p, ServeAttnArgs a) {  // returns its launches
     a.nsplit = p.nsplit;
     a.max_segs = p.max_segs;
     a.part = c->serve_part;
@@ -975,7 +975,9 @@ void enqueue_serve(ZynferCuCtx* c, const ServePlan& p, ServeAttnArgs a) {
     a.early = p.items > 0 ? 1 : 0;
     if (p.items) launch_attn_tile(c->tm_kv, c->serve_rows, c->serve_tiles, a, p.items, c->stream);
     if (!p.chunk) launch_attn_span(c->serve_rows, a, p.ctas, c->stream);
-    if (p.chunk ? p.nsplit > 1 : p.items > 0) launch_serve_merge(c->serve_rows, a, c->stream);
+    const bool merge = p.chunk ? p.nsplit > 1 : p.items > 0;
+    if (merge) launch_serve_merge(c->serve_rows, a, c->stream);
+    return (p.items ? 1 : 0) + (p.chunk ? 0 : 1) + (merge ? 1 : 0);
 }
 
 // Changed block-table rows to the device; the pinned copy may be rewritten by
@@ -1871,8 +1873,7 @@ int zynfer_cu_decode_drawn(ZynferCuCtx* c, const uint32_t* seqs, const uint32_t*
         qa.max_blocks = c->max_blocks; qa.n_pool_blocks = c->n_blocks;
         qa.q_out = c->dq; qa.err = c->derr;
         launch_qkv_post(qa, c->stream);
-        enqueue_serve(c, plan, serve_args(c, l, batch, 1, window, sinks, c->dq, c->qd, c->dattn, c->qd, false));
-        c->step_launches += 2;
+        c->step_launches += 1 + enqueue_serve(c, plan, serve_args(c, l, batch, 1, window, sinks, c->dq, c->qd, c->dattn, c->qd, false));
         set_prefetch(c, Ld.wgu, Ld.sgu, 2 * I, H);
         linear(c, ZYNFER_CU_K_LINEAR, Ld.wo, Ld.so, &Ld.tm_o, H, c->qd, c->dattn, N, c->dx1, kEpiResid, c->dx, nullptr,
                nullptr);
