@@ -62,8 +62,11 @@ struct Lay {
     static constexpr int SMEM = BARS + 512;
     static_assert(CTAS * (SMEM + 1024) <= 233472, "tile attention shared memory");
     static_assert(BARS >= kRows * kD * 4, "the results are staged over Q, K and V");
-    // TMEM columns: the accumulator, then two regions of S with P over it
-    static constexpr int S_COL = kD, S_STEP = TERMS == 1 ? 64 : 128;
+    // TMEM columns: the accumulator (f32 queries: another for the products of P's
+    // small terms, so that a sum is rounded, toward 0 by the MMA, 4 times per tile at
+    // its full size instead of 12), then two regions of S with P over it
+    static constexpr int ACCS = TERMS == 1 ? 1 : 2;
+    static constexpr int S_COL = ACCS * kD, S_STEP = TERMS == 1 ? 64 : 128;
     static constexpr int COLS = TERMS == 1 ? 256 : 512;
 };
 
@@ -333,8 +336,8 @@ __global__ void __launch_bounds__(kThreads, Lay<TERMS>::CTAS)
                     for (int t = TERMS - 1; t >= 0; --t)
 #pragma unroll
                         for (int kk = 0; kk < TILE / 16; ++kk)
-                            mma_ts(tmem, p + t * (TILE / 2) + kk * 8, sdesc(v + kk * 2048, kHalf), id_o,
-                                   j > 0 || t < TERMS - 1 || kk);
+                            mma_ts(tmem + (t > 0 ? kD : 0), p + t * (TILE / 2) + kk * 8, sdesc(v + kk * 2048, kHalf), id_o,
+                                   j > 0 || (t > 0 && t < TERMS - 1) || kk);
                     mma_commit(&empty_v[vs]);
                     mma_commit(o_full);
                     if (i == n) mma_commit(done);
@@ -446,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, Lay<TERMS>::CTAS)
                     if (!alive) break;
                     tc_fence_after();
 #pragma unroll 1
-                    for (int d = 0; d < kD; d += 32) {
+                    for (int d = 0; d < L::ACCS * kD; d += 32) {
                         uint32_t o[32];
                         tmem_ld32(tmem + lane_base + d, o);
                         tmem_wait_ld();
@@ -490,16 +493,20 @@ __global__ void __launch_bounds__(kThreads, Lay<TERMS>::CTAS)
             bool finite = fabsf(l) < INFINITY;
 #pragma unroll 1
             for (int d = 0; d < kD; d += 32) {
-                uint32_t u[32];
-                if (n > 0) tmem_ld32(tmem + lane_base + d, u);
-                else
+                uint32_t u[32], low_u[32];
+                if (n > 0) {
+                    tmem_ld32(tmem + lane_base + d, u);
+                    if (L::ACCS == 2) tmem_ld32(tmem + kD + lane_base + d, low_u);
+                } else {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) u[e] = 0u;
+                    for (int e = 0; e < 32; ++e) u[e] = low_u[e] = 0u;
+                }
                 tmem_wait_ld();
                 float o[32];
 #pragma unroll
                 for (int e = 0; e < 32; ++e) {
                     o[e] = __uint_as_float(u[e]);
+                    if (L::ACCS == 2) o[e] += __uint_as_float(low_u[e]);
                     finite = finite && fabsf(o[e]) < INFINITY;
                     o[e] *= inv;
                 }

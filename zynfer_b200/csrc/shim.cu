@@ -274,6 +274,10 @@ bool take_launch_fault(ZynferCuCtx* c) {
 // Path label "<call>:<linear kernel families>[:<mode>]" into the context's
 // fixed buffer (no allocation): e.g. "decode:gemv+tcgen05:graph".
 void set_path(ZynferCuCtx* c, const char* call, unsigned paths, const char* mode) {
+    if (!paths && !mode) {
+        strncpy(c->path, call, sizeof(c->path) - 1);
+        return;
+    }
     char fam[48] = "";
     const char* names[5] = {"auto", "gemv", "simt", "tcgen05", "mma"};
     for (int b = 1; b < 5; ++b)

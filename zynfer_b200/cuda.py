@@ -199,11 +199,11 @@ def _dtype(t) -> int:
     return dt
 
 
-def _row_values(t, rows: int, kinds, name: str):
-    """Address of a dense tensor of one value per row (None: 0)."""
+def _row_values(t, shape, kinds, name: str):
+    """Address of a dense tensor of one value per row (None: null)."""
     if t is None:
         return None
-    if _kind(t) not in kinds or t.dim() != 1 or t.shape[0] != rows or not t.is_contiguous():
+    if t.shape != shape or _kind(t) not in kinds or not t.is_contiguous():
         raise InvalidArgument(f"{name} must be a dense {kinds[0]} tensor of one value per row")
     return t.data_ptr()
 
@@ -298,7 +298,8 @@ class Gpu:
                 L.zynfer_cu_destroy(h)
             self.h = None
             raise _ERRORS.get(rc, CudaError)(msg)
-        self._rule = DrawRule()
+        self._rule = DrawRule()  # the fields of the call being made
+        self._rule_ref = C.byref(self._rule)
         _LIVE.add(self)
 
     def check(self, rc: int):
@@ -355,14 +356,14 @@ class Gpu:
         if logits.dim() != 2 or logits.stride(1) != 1:
             raise InvalidArgument("logits must be [rows, vocab] with unit inner stride")
         rows, vocab = logits.shape
-        rule = self._rule
-        rule.temperature = _row_values(temperature, rows, _F32, "temperature")
-        rule.top_k = _row_values(top_k, rows, _I32, "top_k")
-        rule.top_p = _row_values(top_p, rows, _F32, "top_p")
-        rule.min_p = _row_values(min_p, rows, _F32, "min_p")
+        n, rule = (rows,), self._rule
+        rule.temperature = _row_values(temperature, n, _F32, "temperature")
+        rule.top_k = _row_values(top_k, n, _I32, "top_k")
+        rule.top_p = _row_values(top_p, n, _F32, "top_p")
+        rule.min_p = _row_values(min_p, n, _F32, "min_p")
         call = (self.h, logits.data_ptr(), _dtype(logits), logits.stride(0) if rows > 1 else vocab, rows, vocab,
-                _row_values(uniforms, rows, _F32, "uniforms"), C.byref(rule), _row_values(ids, rows, _I32, "ids"),
-                _row_values(logprobs, rows, _F32, "logprobs"))
+                _row_values(uniforms, n, _F32, "uniforms"), self._rule_ref, _row_values(ids, n, _I32, "ids"),
+                _row_values(logprobs, n, _F32, "logprobs"))
         self._enqueue(stream, lib().zynfer_cu_sample_rows, call)
 
     def wait_stream(self, stream):
@@ -531,18 +532,18 @@ class Model:
         self.gpu._enqueue(stream, lib().zynfer_cu_kv_write,
                           (self.gpu.h, seq, layer, pos, k.shape[1], k.data_ptr(), v.data_ptr(), _dtype(k)))
 
-    def _serve_rows(self, t, lead):
-        """Row stride of a [.., n_q, head_dim] tensor whose leading dimensions `lead` are rows at one stride."""
-        a, shape, st = self.arch, tuple(t.shape), t.stride()
-        if shape != (*lead, a.n_q, a.head_dim):
-            raise InvalidArgument(f"expected a tensor of shape {(*lead, a.n_q, a.head_dim)}, not {shape}")
-        if st[-1] != 1 or st[-2] != a.head_dim:
-            raise InvalidArgument("a row's heads must be dense")
-        if len(lead) == 2 and lead[1] > 1:
-            if lead[0] > 1 and st[0] != lead[1] * st[1]:
-                raise InvalidArgument("rows must lie at one stride")
-            return st[1]
-        return st[0] if lead[0] > 1 else a.n_q * a.head_dim
+    def _row_stride(self, t, n: int, tokens=None):
+        """Stride of the rows of a [n, n_q, head_dim] or [n, tokens, n_q, head_dim] tensor, which lie at one stride."""
+        a, shape, st = self.arch, t.shape, t.stride()
+        if tokens is None:
+            ok, step = shape == (n, a.n_q, a.head_dim), st[0] if n > 1 else 0
+        else:
+            ok, step = shape == (n, tokens, a.n_q, a.head_dim), st[1] if tokens > 1 else (st[0] if n > 1 else 0)
+            ok = ok and (tokens == 1 or n == 1 or st[0] == tokens * st[1])
+        if not ok or st[-1] != 1 or st[-2] != a.head_dim:
+            raise InvalidArgument(f"expected rows of dense [{a.n_q}, {a.head_dim}] heads at one stride, {n} sequences"
+                                  f"{'' if tokens is None else f' of {tokens} tokens'}; got shape {tuple(shape)}, strides {st}")
+        return step or a.n_q * a.head_dim
 
     def attn_shared(self, layer: int, seqs, q, out, stream=None):
         """Decode attention of one query per sequence (device q and out [B, n_q, head_dim], f32 or bf16, rows at
@@ -550,10 +551,9 @@ class Model:
         ids, n, keep = _ids(seqs)
         if q.dtype != out.dtype:
             raise InvalidArgument("q and out must have one type")
-        lead = (n,)
         self.gpu._enqueue(stream, lib().zynfer_cu_attn_shared,
-                          (self.gpu.h, layer, ids, n, q.data_ptr(), self._serve_rows(q, lead), out.data_ptr(),
-                           self._serve_rows(out, lead), _dtype(q)))
+                          (self.gpu.h, layer, ids, n, q.data_ptr(), self._row_stride(q, n), out.data_ptr(),
+                           self._row_stride(out, n), _dtype(q)))
 
     def attn_window(self, layer: int, seqs, q, out, window: int = WINDOW_ALL, sinks: int = 0, stream=None):
         """Attention of the last T cached positions of each sequence (device q and out [B, T, n_q, head_dim], or
@@ -562,11 +562,11 @@ class Model:
         dims = q.dim()
         if q.dtype != out.dtype or dims not in (3, 4) or window < 0 or sinks < 0:
             raise InvalidArgument("q and out must be [B, n_q, d] or [B, T, n_q, d] of one type; window and sinks not negative")
-        lead = (n,) if dims == 3 else (n, q.shape[1])
+        tokens = q.shape[1] if dims == 4 else None
         self.gpu._enqueue(stream, lib().zynfer_cu_attn_window,
-                          (self.gpu.h, layer, ids, n, q.shape[1] if dims == 4 else 1, min(window, WINDOW_ALL),
-                           min(sinks, WINDOW_ALL), q.data_ptr(), self._serve_rows(q, lead), out.data_ptr(),
-                           self._serve_rows(out, lead), _dtype(q)))
+                          (self.gpu.h, layer, ids, n, 1 if tokens is None else tokens, min(window, WINDOW_ALL),
+                           min(sinks, WINDOW_ALL), q.data_ptr(), self._row_stride(q, n, tokens), out.data_ptr(),
+                           self._row_stride(out, n, tokens), _dtype(q)))
 
     def rmsnorm_qk_rope(self, qkv, rows: int, q_norm, k_norm, pos0: int, q_out, k_out):
         """Per-head q/k RMSNorm + RoPE of `rows` tokens (device pointers, heads-major outputs)."""
