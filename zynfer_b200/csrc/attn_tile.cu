@@ -51,6 +51,7 @@ constexpr int kHalf = TILE * 128, kTileBytes = 2 * kHalf;  // a K or V tile: two
 constexpr int kHalfDims = 64;
 constexpr float kLag = 8.0f;     // log2 of the growth of a row's maximum that is left to lag
 constexpr unsigned kAll = 0xFFFFFFFFu;
+using u64x2 = unsigned long long;
 
 template <int TERMS>
 struct Lay {
@@ -132,6 +133,24 @@ __device__ __forceinline__ void mma_commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
                  : "memory");
 }
+
+// Two f32 operations in one instruction.
+__device__ __forceinline__ u64x2 fma2(u64x2 a, u64x2 b, u64x2 c) {
+    u64x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ u64x2 add2(u64x2 a, u64x2 b) {
+    u64x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ u64x2 pack2(float x, float y) {
+    u64x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ void unpack2(u64x2 v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
 
 // What a CTA works on.
 struct Job {
@@ -460,14 +479,16 @@ __global__ void __launch_bounds__(kThreads, Lay<TERMS>::CTAS)
                 }
             }
             const float neg = m_ref == -INFINITY ? 0.0f : -m_ref;
-            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            const u64x2 scale_2 = pack2(scale2, scale2), neg_2 = pack2(neg, neg);
+            u64x2 sum[2] = {0ull, 0ull};
             uint32_t p[TERMS][32];
 #pragma unroll
             for (int e = 0; e < 32; ++e) {
-                const float x0 = exp2_fast(fmaf(s[2 * e], scale2, neg));
-                const float x1 = exp2_fast(fmaf(s[2 * e + 1], scale2, neg));
-                sum[(2 * e) & 3] += x0;
-                sum[(2 * e + 1) & 3] += x1;
+                float x0, x1;
+                unpack2(fma2(pack2(s[2 * e], s[2 * e + 1]), scale_2, neg_2), x0, x1);
+                x0 = exp2_fast(x0);
+                x1 = exp2_fast(x1);
+                sum[e & 1] = add2(sum[e & 1], pack2(x0, x1));
                 uint32_t u[TERMS];
                 split_pair<TERMS>(x0, x1, u);
 #pragma unroll
@@ -475,7 +496,9 @@ __global__ void __launch_bounds__(kThreads, Lay<TERMS>::CTAS)
             }
 #pragma unroll
             for (int k = 0; k < TERMS; ++k) tmem_st32(s_at + k * (TILE / 2), p[k]);
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            float l0, l1;
+            unpack2(add2(sum[0], sum[1]), l0, l1);
+            l += l0 + l1;
             tmem_wait_st();
             tc_fence_before();
             mbar_arrive(&p_full[i & 1]);
