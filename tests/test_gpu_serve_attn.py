@@ -471,3 +471,33 @@ def test_few_queries_with_many_keys(lens, tokens, window, sinks, dtype):
     m.gpu.sync()
     for i, n in enumerate(lens):
         check(out[i], reference(q[i], k[i], v[i], window_seen(n, tokens, window, sinks)), v[i], dtype)
+
+
+@pytest.mark.parametrize("plen,grows", [(30000, 0), (40000, 1)])
+def test_workspace_stays_and_grows(plen, grows):
+    """Calls allocate nothing until one needs more partial results than model_init left room for: two rows
+    that share a very long prompt, split over many CTAs, in a batch of many rows. (The shorter prompt saves
+    too few block reads to be shared.)"""
+    rows = 300
+    m = make(n_kv=4, max_batch=rows, max_seqs=rows, max_seq_len=plen + 16, kv_blocks=plen // 16 + 2 * rows + 4)
+    kv = share(m, 2, [plen, 0], [[3, 9], [1 + i % 16 for i in range(rows - 2)]])
+    q = normal(21, rows, 8, D)
+    out = torch.full_like(q, float("nan"))
+    torch.cuda.synchronize()
+
+    def call(seqs):
+        m.attn_shared(0, seqs, q[:len(seqs)], out[:len(seqs)])
+        m.gpu.sync()
+        for i, s in list(enumerate(seqs))[:12]:
+            k, v = kv[s]
+            check(out[i:i + 1], reference(q[i:i + 1], k, v, torch.ones(1, k.shape[1], dtype=torch.bool, device="cuda")), v, "f32")
+
+    before = m.gpu.alloc_events()[0]
+    call([0, 1])
+    call(list(range(2, 40)))
+    assert m.gpu.alloc_events()[0] == before
+    call(list(range(rows)))
+    assert m.gpu.alloc_events()[0] == before + grows
+    call(list(range(rows)))
+    call([1, 0, 5])
+    assert m.gpu.alloc_events()[0] == before + grows

@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         return (long long)a.n_kv * pref[l] + (long long)(r / (nblk + kSpanLead)) * nblk + max(0, r % (nblk + kSpanLead) - kSpanLead);
     };
     const int nwarps = gridDim.x * kWarps;
-    const int per = (int)max((units + nwarps - 1) / nwarps, (long long)a.min_per);
+    const int per = (int)((units + nwarps - 1) / nwarps);
     const long long reach = (long long)kWarps * per;  // units of a CTA
     if (warp == 0 && lane <= kWarps) sm.bound[lane] = first_block(blockIdx.x * reach + (long long)lane * per);
     __syncthreads();

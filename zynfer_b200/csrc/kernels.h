@@ -208,7 +208,6 @@ struct ServeAttnArgs {
     float* part;               // [row][n_q][max_segs][kServeRecord]
     int max_segs;
     unsigned* counters;        // [row][n_q], zero between launches
-    int min_per;               // span kernel: units a warp takes at least
     int early;                 // span kernel: launched behind a tile kernel
     uint32_t* err;
 };

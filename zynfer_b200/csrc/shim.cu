@@ -905,12 +905,25 @@ int plan_shared(ZynferCuCtx* c, uint32_t batch, bool bf16, int* max_segs) {
     return items;
 }
 
+// Room for `words` of partial results. model_init leaves enough for most calls
+// (an allocation costs about 0.45 ms); one that needs more doubles it, so that the
+// outgrown buffers, which stay in c->allocs until destroy, never take more than the last.
 int serve_scratch(ZynferCuCtx* c, size_t words) {
     if (words <= c->serve_part_words) return ZYNFER_CU_OK;
-    int rc = dalloc(c, &c->serve_part, words);  // the smaller buffer stays in c->allocs until destroy
-    if (rc == ZYNFER_CU_OK) c->serve_part_words = words;
-    else c->serve_part_words = 0;
-    return rc;
+    words = std::max(words, 2 * c->serve_part_words);
+    float* grown = nullptr;
+    int rc = dalloc(c, &grown, words);
+    if (rc) return rc;
+    c->serve_part = grown;
+    c->serve_part_words = words;
+    return ZYNFER_CU_OK;
+}
+
+// One wave of tile CTAs (two to an SM) with a record for each of their 128 query rows, and
+// eight records per row and query head of a batch.
+size_t serve_initial_words(const ZynferCuCtx* c) {
+    const size_t sms = c->caps.sm_count > 0 ? c->caps.sm_count : 148;
+    return (128 * 2 * sms + (size_t)c->d.max_batch * c->d.n_q * 8) * kServeRecord;
 }
 
 // The launches of a planned call.
@@ -919,7 +932,7 @@ struct ServePlan {
     int items = 0;       // CTAs of the tile kernel
     int nsplit = 1;      // chunk: CTAs that share a tile's blocks
     int ctas = 0;        // of the span kernel
-    int min_per = 1, max_segs = 1;
+    int max_segs = 1;
 };
 
 int plan_serve(ZynferCuCtx* c, uint32_t batch, uint32_t tokens, uint32_t window, uint32_t sinks, bool shared, bool bf16,
@@ -954,7 +967,7 @@ int plan_serve(ZynferCuCtx* c, uint32_t batch, uint32_t tokens, uint32_t window,
     c->serve_tiles.n = 0;
     int tile_segs = 1;
     if (shared) p->items = plan_shared(c, batch, bf16, &tile_segs);
-    // the span kernel's list of blocks, at least min_per to a warp
+    // the span kernel's list of blocks, at least one to a warp
     long long blocks = 0;
     int longest = 1;
     for (uint32_t i = 0; i < batch; ++i) {
@@ -963,9 +976,9 @@ int plan_serve(ZynferCuCtx* c, uint32_t batch, uint32_t tokens, uint32_t window,
         blocks += n;
         longest = std::max(longest, n);
     }
-    const long long total = (blocks + (long long)kSpanLead * batch) * c->d.n_kv, share = (long long)kSpanWarps * p->min_per;
-    p->ctas = (int)std::min<long long>(sms, (total + share - 1) / share);
-    const long long per = std::max<long long>(p->min_per, (total + (long long)p->ctas * kSpanWarps - 1) / ((long long)p->ctas * kSpanWarps));
+    const long long total = (blocks + (long long)kSpanLead * batch) * c->d.n_kv;
+    p->ctas = (int)std::min<long long>(sms, (total + kSpanWarps - 1) / kSpanWarps);
+    const long long warps = (long long)p->ctas * kSpanWarps, per = (total + warps - 1) / warps;
     p->max_segs = tile_segs + (int)((longest - 1) / (per * kSpanWarps) + 2);
     return serve_scratch(c, (size_t)batch * c->d.n_q * p->max_segs * kServeRecord);
 }
@@ -975,7 +988,6 @@ int enqueue_serve(ZynferCuCtx* c, const ServePlan& p, ServeAttnArgs a) {  // ret
     a.max_segs = p.max_segs;
     a.part = c->serve_part;
     a.counters = c->serve_cnt;
-    a.min_per = p.min_per;
     a.early = p.items > 0 ? 1 : 0;
     if (p.items) launch_attn_tile(c->tm_kv, c->serve_rows, c->serve_tiles, a, p.items, c->stream);
     if (!p.chunk) launch_attn_span(c->serve_rows, a, p.ctas, c->stream);
@@ -1244,6 +1256,8 @@ int zynfer_cu_model_init(ZynferCuCtx* c, const ZynferCuModelDesc* desc) {
     ALLOC(c->dids, B);
     ALLOC(c->dcnt, B * m.n_kv);
     ALLOC(c->serve_cnt, B * m.n_q);
+    c->serve_part_words = serve_initial_words(c);
+    ALLOC(c->serve_part, c->serve_part_words);
     ALLOC(c->dpart, B * m.n_kv * (size_t)decode_max_segs(c->max_blocks) * 2 * (hd + 4));
     c->hist_cap = std::max<size_t>(B * 4096, 1 << 16);
     ALLOC(c->dhist, c->hist_cap);
