@@ -113,6 +113,7 @@ struct ZynferCuCtx {
     std::vector<uint32_t> block_refs;  // sequences holding each pool block (shared prefixes hold one block several times)
     std::vector<std::vector<int>> seq_blocks;
     std::vector<uint32_t> seq_len;
+    std::vector<uint8_t> seq_mark;      // [max_seqs] scratch of validate_batch, zero between calls
     std::vector<char> table_dirty;  // host row changed since its last upload
     int* table_host = nullptr;  // pinned [max_seqs][max_blocks]
     int* table_dev = nullptr;
@@ -666,14 +667,23 @@ int upload_table_rows(ZynferCuCtx* c, const uint32_t* seqs, uint32_t n) {
 int validate_batch(ZynferCuCtx* c, const uint32_t* seqs, uint32_t batch, uint32_t extra) {
     if (!c->ready) return fail(c, ZYNFER_CU_INVALID, "model not initialised");
     if (batch == 0 || batch > c->d.max_batch) return fail(c, ZYNFER_CU_INVALID, "batch must be 1..max_batch");
-    for (uint32_t i = 0; i < batch; ++i) {
-        if (seqs[i] >= c->d.max_seqs) return fail(c, ZYNFER_CU_INVALID, "sequence id out of range");
-        for (uint32_t j = 0; j < i; ++j)
-            if (seqs[j] == seqs[i]) return fail(c, ZYNFER_CU_INVALID, "a sequence appears twice in one batch");
-        if (c->seq_len[seqs[i]] + extra > c->d.max_seq_len)
-            return fail(c, ZYNFER_CU_INVALID, "KV cache full: step would exceed max_seq_len");
+    const char* why = nullptr;
+    uint32_t marked = 0;
+    for (; marked < batch && !why; ++marked) {
+        const uint32_t s = seqs[marked];
+        if (s >= c->d.max_seqs) {
+            why = "sequence id out of range";
+            break;
+        }
+        if (c->seq_mark[s]) {
+            why = "a sequence appears twice in one batch";
+            break;
+        }
+        c->seq_mark[s] = 1;
+        if (c->seq_len[s] + extra > c->d.max_seq_len) why = "KV cache full: step would exceed max_seq_len";
     }
-    return ZYNFER_CU_OK;
+    for (uint32_t i = 0; i < marked; ++i) c->seq_mark[seqs[i]] = 0;
+    return why ? fail(c, ZYNFER_CU_INVALID, why) : ZYNFER_CU_OK;
 }
 
 int stage_batch(ZynferCuCtx* c, const uint32_t* seqs, const uint32_t* tokens, uint32_t B) {
@@ -1237,6 +1247,7 @@ int zynfer_cu_model_init(ZynferCuCtx* c, const ZynferCuModelDesc* desc) {
     c->seq_blocks.assign(m.max_seqs, {});
     for (auto& bl : c->seq_blocks) bl.reserve(c->max_blocks);  // decode never grows a block list
     c->seq_len.assign(m.max_seqs, 0);
+    c->seq_mark.assign(m.max_seqs, 0);
     c->table_dirty.assign(m.max_seqs, 0);
     if ((rc = halloc(c, &c->table_host, (size_t)m.max_seqs * c->max_blocks)) != ZYNFER_CU_OK) return rc;
     std::fill(c->table_host, c->table_host + (size_t)m.max_seqs * c->max_blocks, -1);
