@@ -298,11 +298,11 @@ __global__ void __launch_bounds__(kThreads, Lay<TERMS>::CTAS)
                 if (i + kChunk < n) next = rows_of(i / kChunk + 1);
             }
             bool ok = true;
-            if (round > 0) ok = mbar_wait_bounded(&empty[s], (uint32_t)((round - 1) & 1), a.err);
+            if (round > 0) ok = mbar_wait_try(&empty[s], (uint32_t)((round - 1) & 1), a.err);
             if (!__all_sync(kAll, ok)) {
                 // the copies in flight land before the CTA ends
                 for (int k = max(0, i - stages); k < i; ++k)
-                    mbar_wait_bounded(&full[k % stages], (uint32_t)((k / stages) & 1), nullptr);
+                    mbar_wait_try(&full[k % stages], (uint32_t)((k / stages) & 1), nullptr);
                 break;
             }
             const int y = __shfl_sync(kAll, now, (i % kChunk) * kTileBlocks + blk);
@@ -327,7 +327,7 @@ __global__ void __launch_bounds__(kThreads, Lay<TERMS>::CTAS)
             int ks = 0, kround = 0, vs = 0, vround = 0;
             for (int i = 0; i <= n; ++i) {
                 if (i < n) {
-                    if (!mbar_wait_bounded(&full_k[ks], (uint32_t)(kround & 1), a.err)) break;
+                    if (!mbar_wait_try(&full_k[ks], (uint32_t)(kround & 1), a.err)) break;
                     tc_fence_after();
                     const uint32_t k = smem_addr(smem + L::K + ks * kTileBytes);
                     const uint32_t d = tmem + L::S_COL + (i & 1) * L::S_STEP;
@@ -346,8 +346,8 @@ __global__ void __launch_bounds__(kThreads, Lay<TERMS>::CTAS)
                 }
                 if (i > 0) {
                     const int j = i - 1;
-                    if (!mbar_wait_bounded(&full_v[vs], (uint32_t)(vround & 1), a.err)) break;
-                    if (!mbar_wait_bounded(&p_full[j & 1], (uint32_t)((j >> 1) & 1), a.err)) break;
+                    if (!mbar_wait_try(&full_v[vs], (uint32_t)(vround & 1), a.err)) break;
+                    if (!mbar_wait_try(&p_full[j & 1], (uint32_t)((j >> 1) & 1), a.err)) break;
                     tc_fence_after();
                     const uint32_t v = smem_addr(smem + L::V + vs * kTileBytes);
                     const uint32_t p = tmem + L::S_COL + (j & 1) * L::S_STEP;
@@ -423,7 +423,7 @@ __global__ void __launch_bounds__(kThreads, Lay<TERMS>::CTAS)
         bool alive = true;
 #pragma unroll 1
         for (int i = 0; i < n; ++i) {
-            alive = __all_sync(kAll, mbar_wait_bounded(&s_full[i & 1], (uint32_t)((i >> 1) & 1), a.err));
+            alive = __all_sync(kAll, mbar_wait_try(&s_full[i & 1], (uint32_t)((i >> 1) & 1), a.err));
             if (!alive) break;
             tc_fence_after();
             const uint32_t s_at = tmem + L::S_COL + (i & 1) * L::S_STEP + lane_base;
@@ -464,7 +464,7 @@ __global__ void __launch_bounds__(kThreads, Lay<TERMS>::CTAS)
                     // the accumulator, once P V of the tile before is done. S(i) came
                     // after P V of tile i - 2, and that of tile i waits for this warp: o_full
                     // is in phase i - 1 or i, which its parity tells apart
-                    alive = __all_sync(kAll, mbar_wait_bounded(o_full, (uint32_t)((i - 1) & 1), a.err));
+                    alive = __all_sync(kAll, mbar_wait_try(o_full, (uint32_t)((i - 1) & 1), a.err));
                     if (!alive) break;
                     tc_fence_after();
 #pragma unroll 1
@@ -507,7 +507,7 @@ __global__ void __launch_bounds__(kThreads, Lay<TERMS>::CTAS)
         // whole rows are stored together
         // (a barrier of its own: o_full may be one or two phases on by now, which its
         // parity does not tell apart)
-        if (n > 0) alive = __all_sync(kAll, alive && mbar_wait_bounded(done, 0u, a.err));
+        if (n > 0) alive = __all_sync(kAll, alive && mbar_wait_try(done, 0u, a.err));
         tc_fence_after();
         const bool direct = list.n == 0 && job.nseg == 1;
         const int n_q = a.n_kv * kG;

@@ -69,6 +69,16 @@ __device__ __forceinline__ uint32_t pack_bf16(float x0, float x1) {
 }
 __device__ __forceinline__ void fence_proxy_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+// mbar_wait_bounded with the barrier tried once in line: most are complete when they
+// are asked for, and the loop costs such a wait 245 cycles (the tile kernel's MMA
+// thread, which waits three times per tile) where one try costs 41.
+static __device__ __noinline__ bool mbar_wait_loop(uint64_t* bar, uint32_t parity, uint32_t* err) {
+    return mbar_wait_bounded(bar, parity, err);
+}
+__device__ __forceinline__ bool mbar_wait_try(uint64_t* bar, uint32_t parity, uint32_t* err) {
+    return mbar_try_wait(bar, parity) || mbar_wait_loop(bar, parity, err);
+}
+
 // A partial result of one query head held by a warp: lane l has dims 4 l ..
 // 4 l + 3.
 struct Partial {
