@@ -56,7 +56,7 @@ using u64x2 = unsigned long long;
 template <int TERMS>
 struct Lay {
     static constexpr int CTAS = TERMS == 1 ? 2 : 1;      // per SM
-    static constexpr int KST = TERMS == 1 ? 2 : 3, VST = 3;
+    static constexpr int KST = 2, VST = 3;  // K's ring is S's: one barrier tells that S is there and K's place free
     static constexpr int QTERM = kRows * 256;
     static constexpr int K = TERMS * QTERM, V = K + KST * kTileBytes;
     static constexpr int BARS = V + VST * kTileBytes;
@@ -223,34 +223,27 @@ __global__ void __launch_bounds__(kThreads, Lay<TERMS>::CTAS)
                      const __grid_constant__ TileListT<N> list, const __grid_constant__ ServeAttnArgs a) {
     using L = Lay<TERMS>;
     extern __shared__ __align__(1024) uint8_t smem[];
+    // A barrier per buffer: no waiter can be two phases behind. (A commit costs the MMA thread
+    // 65 cycles, so what ends at once shares one.)
     uint64_t* full_k = reinterpret_cast<uint64_t*>(smem + L::BARS);
-    uint64_t* empty_k = full_k + L::KST;
-    uint64_t* full_v = empty_k + L::KST;
-    uint64_t* empty_v = full_v + L::VST;
-    uint64_t* s_full = empty_v + L::VST;  // [2] S of tile i (buffer i & 1) is in TMEM
-    uint64_t* p_full = s_full + 2;        // [2] its P is (a barrier per buffer: P of tile i + 1 may be there before
-                                          // the MMA warp has looked for that of tile i)
-    uint64_t* o_full = p_full + 2;        // P V of tile i is done
-    uint64_t* done = o_full + 1;          // that of the last one is
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+    uint64_t* s_full = full_k + L::KST;   // S of tile i (buffer i & 1) is in TMEM, its K read
+    uint64_t* full_v = s_full + L::KST;
+    uint64_t* o_full = full_v + L::VST;   // P V of tile i (buffer i % VST) is done, its V read
+    uint64_t* p_full = o_full + L::VST;   // [2] P of tile i (buffer i & 1) is in TMEM
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(p_full + 2);
     uint32_t* bad_rows = tmem_slot + 1;   // [4] bit per row: not finite
 
     const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
     if (threadIdx.x == 0) {
         for (int s = 0; s < L::KST; ++s) {
             mbar_init(&full_k[s], 2);
-            mbar_init(&empty_k[s], 1);
+            mbar_init(&s_full[s], 1);
+            mbar_init(&p_full[s], 128);
         }
         for (int s = 0; s < L::VST; ++s) {
             mbar_init(&full_v[s], 1);
-            mbar_init(&empty_v[s], 1);
+            mbar_init(&o_full[s], 1);
         }
-        mbar_init(&s_full[0], 1);
-        mbar_init(&s_full[1], 1);
-        mbar_init(&p_full[0], 128);
-        mbar_init(&p_full[1], 128);
-        mbar_init(o_full, 1);
-        mbar_init(done, 1);
         for (int w = 0; w < 4; ++w) bad_rows[w] = 0u;
         fence_barrier_init();
     }
@@ -275,7 +268,7 @@ __global__ void __launch_bounds__(kThreads, Lay<TERMS>::CTAS)
         // eight of a K tile, which S waits for, are shared.
         const int is_v = warp == 5, stages = is_v ? L::VST : L::KST;
         uint64_t* full = is_v ? full_v : full_k;
-        uint64_t* empty = is_v ? empty_v : empty_k;
+        uint64_t* empty = is_v ? o_full : s_full;
         uint8_t* ring = smem + (is_v ? L::V : L::K);
         const int* table = a.block_table + (size_t)job.slot * a.max_blocks;
         const int v0 = job.t_lo * kTileBlocks, row0 = a.kv_row0 + job.head * a.n_pool_blocks * 2 * kKvBlock + is_v * kKvBlock;
@@ -337,8 +330,7 @@ __global__ void __launch_bounds__(kThreads, Lay<TERMS>::CTAS)
                         for (int kk = 0; kk < 8; ++kk)
                             mma_ss(d, sdesc(qs + t * L::QTERM + (kk >> 2) * (kRows * 128) + (kk & 3) * 32, 16),
                                    sdesc(k + (kk >> 2) * kHalf + (kk & 3) * 32, 16), id_s, t < TERMS - 1 || kk);
-                    mma_commit(&empty_k[ks]);
-                    mma_commit(&s_full[i & 1]);
+                    mma_commit(&s_full[ks]);
                     if (++ks == L::KST) {
                         ks = 0;
                         ++kround;
@@ -357,9 +349,7 @@ __global__ void __launch_bounds__(kThreads, Lay<TERMS>::CTAS)
                         for (int kk = 0; kk < TILE / 16; ++kk)
                             mma_ts(tmem + (t > 0 ? kD : 0), p + t * (TILE / 2) + kk * 8, sdesc(v + kk * 2048, kHalf), id_o,
                                    j > 0 || (t > 0 && t < TERMS - 1) || kk);
-                    mma_commit(&empty_v[vs]);
-                    mma_commit(o_full);
-                    if (i == n) mma_commit(done);
+                    mma_commit(&o_full[vs]);
                     if (++vs == L::VST) {
                         vs = 0;
                         ++vround;
@@ -461,10 +451,10 @@ __global__ void __launch_bounds__(kThreads, Lay<TERMS>::CTAS)
                 l *= c;
                 m_ref = m_new;
                 if (i > 0) {
-                    // the accumulator, once P V of the tile before is done. S(i) came
-                    // after P V of tile i - 2, and that of tile i waits for this warp: o_full
-                    // is in phase i - 1 or i, which its parity tells apart
-                    alive = __all_sync(kAll, mbar_wait_try(o_full, (uint32_t)((i - 1) & 1), a.err));
+                    // the accumulator, once P V of the tile before is done (that of tile
+                    // i waits for this warp)
+                    const int j = i - 1;
+                    alive = __all_sync(kAll, mbar_wait_try(&o_full[j % L::VST], (uint32_t)((j / L::VST) & 1), a.err));
                     if (!alive) break;
                     tc_fence_after();
 #pragma unroll 1
@@ -505,9 +495,7 @@ __global__ void __launch_bounds__(kThreads, Lay<TERMS>::CTAS)
         }
         // ---- the result: through shared memory (Q, K and V are read), so that
         // whole rows are stored together
-        // (a barrier of its own: o_full may be one or two phases on by now, which its
-        // parity does not tell apart)
-        if (n > 0) alive = __all_sync(kAll, alive && mbar_wait_try(done, 0u, a.err));
+        if (n > 0) alive = __all_sync(kAll, alive && mbar_wait_try(&o_full[(n - 1) % L::VST], (uint32_t)(((n - 1) / L::VST) & 1), a.err));
         tc_fence_after();
         const bool direct = list.n == 0 && job.nseg == 1;
         const int n_q = a.n_kv * kG;
