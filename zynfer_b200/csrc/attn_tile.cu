@@ -368,31 +368,37 @@ __global__ void __launch_bounds__(kThreads, Lay<TERMS>::CTAS)
             auto place = [&](int qr, int k) {
                 return reinterpret_cast<uint4*>(smem + k * L::QTERM + half * (kRows * 128) + qr * 128 + (((c & 7) ^ (qr & 7)) << 4));
             };
-            constexpr int kAhead = TERMS == 1 ? 8 : 4;
-#pragma unroll 1
-            for (int g = 0; g < 16; g += kAhead) {
-                float4 x[kAhead][2];
+            if constexpr (TERMS == 1) {
+                // as they lie: asynchronous copies, all in flight at once (rows that are not there: zeros)
 #pragma unroll
-                for (int e = 0; e < kAhead; ++e) {
-                    const int qr = 8 * (g + e) + 2 * warp + (lane >> 4), m = qr >> 1;
-                    x[e][0] = x[e][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    if (m < job.count) {
-                        const size_t at = (size_t)(list.n ? rows.r[job.first + m].row : job.first + m) * a.q_stride +
-                                          (size_t)(job.head * kG + (qr & 1)) * kD + 8 * c;
-                        if constexpr (TERMS == 1) {
-                            x[e][0] = __ldcg(reinterpret_cast<const float4*>(static_cast<const uint16_t*>(a.q) + at));
-                        } else {
+                for (int g = 0; g < 16; ++g) {
+                    const int qr = 8 * g + 2 * warp + (lane >> 4), m = min(qr >> 1, job.count - 1);
+                    const size_t at = (size_t)(list.n ? rows.r[job.first + m].row : job.first + m) * a.q_stride +
+                                      (size_t)(job.head * kG + (qr & 1)) * kD + 8 * c;
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(place(qr, 0))),
+                                 "l"(static_cast<const uint16_t*>(a.q) + at), "r"((qr >> 1) < job.count ? 16 : 0)
+                                 : "memory");
+                }
+                asm volatile("cp.async.wait_all;" ::: "memory");
+            } else {
+                constexpr int kAhead = 4;
+#pragma unroll 1
+                for (int g = 0; g < 16; g += kAhead) {
+                    float4 x[kAhead][2];
+#pragma unroll
+                    for (int e = 0; e < kAhead; ++e) {
+                        const int qr = 8 * (g + e) + 2 * warp + (lane >> 4), m = qr >> 1;
+                        x[e][0] = x[e][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        if (m < job.count) {
+                            const size_t at = (size_t)(list.n ? rows.r[job.first + m].row : job.first + m) * a.q_stride +
+                                              (size_t)(job.head * kG + (qr & 1)) * kD + 8 * c;
                             x[e][0] = __ldcg(reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + at));
                             x[e][1] = __ldcg(reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + at + 4));
                         }
                     }
-                }
 #pragma unroll
-                for (int e = 0; e < kAhead; ++e) {
-                    const int qr = 8 * (g + e) + 2 * warp + (lane >> 4);
-                    if constexpr (TERMS == 1) {
-                        *reinterpret_cast<float4*>(place(qr, 0)) = x[e][0];
-                    } else {
+                    for (int e = 0; e < kAhead; ++e) {
+                        const int qr = 8 * (g + e) + 2 * warp + (lane >> 4);
                         uint32_t t[4][TERMS];
                         split_pair<TERMS>(x[e][0].x, x[e][0].y, t[0]);
                         split_pair<TERMS>(x[e][0].z, x[e][0].w, t[1]);
