@@ -33,6 +33,7 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "serve_common.cuh"
 #include "tc_gemm.h"
@@ -56,7 +57,7 @@ using u64x2 = unsigned long long;
 template <int TERMS>
 struct Lay {
     static constexpr int CTAS = TERMS == 1 ? 2 : 1;      // per SM
-    static constexpr int KST = 2, VST = 3;  // K's ring is S's: one barrier tells that S is there and K's place free
+    static constexpr int KST = 2, VST = 2;  // K's ring is S's: one barrier tells that S is there and K's place free
     static constexpr int QTERM = kRows * 256;
     static constexpr int K = TERMS * QTERM, V = K + KST * kTileBytes;
     static constexpr int BARS = V + VST * kTileBytes;
@@ -317,45 +318,42 @@ __global__ void __launch_bounds__(kThreads, Lay<TERMS>::CTAS)
             // after it was read.
             constexpr uint32_t id_s = idesc(TILE, false), id_o = idesc(kD, true);
             const uint32_t qs = smem_addr(smem);
-            int ks = 0, kround = 0, vs = 0, vround = 0;
-            for (int i = 0; i <= n; ++i) {
+            // tile i with buffer `s` known, so that descriptors are constants
+            auto step = [&](int i, auto buffer) -> bool {
+                constexpr int s = decltype(buffer)::value, o = 1 - s;
                 if (i < n) {
-                    if (!mbar_wait_try(&full_k[ks], (uint32_t)(kround & 1), a.err)) break;
+                    if (!mbar_wait_try(&full_k[s], (uint32_t)((i >> 1) & 1), a.err)) return false;
                     tc_fence_after();
-                    const uint32_t k = smem_addr(smem + L::K + ks * kTileBytes);
-                    const uint32_t d = tmem + L::S_COL + (i & 1) * L::S_STEP;
+                    const uint32_t k = qs + L::K + s * kTileBytes;
 #pragma unroll
                     for (int t = TERMS - 1; t >= 0; --t)  // the small terms first: fewer roundings at the sum's size
 #pragma unroll
                         for (int kk = 0; kk < 8; ++kk)
-                            mma_ss(d, sdesc(qs + t * L::QTERM + (kk >> 2) * (kRows * 128) + (kk & 3) * 32, 16),
+                            mma_ss(tmem + L::S_COL + s * L::S_STEP,
+                                   sdesc(qs + t * L::QTERM + (kk >> 2) * (kRows * 128) + (kk & 3) * 32, 16),
                                    sdesc(k + (kk >> 2) * kHalf + (kk & 3) * 32, 16), id_s, t < TERMS - 1 || kk);
-                    mma_commit(&s_full[ks]);
-                    if (++ks == L::KST) {
-                        ks = 0;
-                        ++kround;
-                    }
+                    mma_commit(&s_full[s]);
                 }
                 if (i > 0) {
                     const int j = i - 1;
-                    if (!mbar_wait_try(&full_v[vs], (uint32_t)(vround & 1), a.err)) break;
-                    if (!mbar_wait_try(&p_full[j & 1], (uint32_t)((j >> 1) & 1), a.err)) break;
+                    if (!mbar_wait_try(&full_v[o], (uint32_t)((j >> 1) & 1), a.err)) return false;
+                    if (!mbar_wait_try(&p_full[o], (uint32_t)((j >> 1) & 1), a.err)) return false;
                     tc_fence_after();
-                    const uint32_t v = smem_addr(smem + L::V + vs * kTileBytes);
-                    const uint32_t p = tmem + L::S_COL + (j & 1) * L::S_STEP;
+                    const uint32_t v = qs + L::V + o * kTileBytes;
 #pragma unroll
                     for (int t = TERMS - 1; t >= 0; --t)
 #pragma unroll
                         for (int kk = 0; kk < TILE / 16; ++kk)
-                            mma_ts(tmem + (t > 0 ? kD : 0), p + t * (TILE / 2) + kk * 8, sdesc(v + kk * 2048, kHalf), id_o,
-                                   j > 0 || (t > 0 && t < TERMS - 1) || kk);
-                    mma_commit(&o_full[vs]);
-                    if (++vs == L::VST) {
-                        vs = 0;
-                        ++vround;
-                    }
+                            mma_ts(tmem + (t > 0 ? kD : 0), tmem + L::S_COL + o * L::S_STEP + t * (TILE / 2) + kk * 8,
+                                   sdesc(v + kk * 2048, kHalf), id_o, j > 0 || (t > 0 && t < TERMS - 1) || kk);
+                    mma_commit(&o_full[o]);
                 }
-            }
+                return true;
+            };
+            for (int i = 0; i <= n; i += 2)
+                if (!step(i, std::integral_constant<int, 0>{}) ||
+                    (i < n && !step(i + 1, std::integral_constant<int, 1>{})))
+                    break;
         }
         __syncwarp();
     } else if (warp < 4) {
