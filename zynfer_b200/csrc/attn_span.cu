@@ -20,6 +20,10 @@
 // memory; what crosses CTAs meets in global records that the last CTA of the
 // row joins in a fixed order (an atomic counter tells which is last; nothing
 // waits). A row with a common prompt leaves its records to serve_attn.cu's join.
+//
+// Measured: 64 rows that see 1028 positions each, 8 kv heads: 46 us, 5.8 TB/s, 89 % of
+// the card's copy rate. One such row: 25 us for a lone call, of which the kernel's
+// chain (parameters, block table, K and V, joins in and across CTAs) is 11.4.
 #include <algorithm>
 #include <type_traits>
 

@@ -9,9 +9,19 @@
 // P back into TMEM over S as the next MMA's A operand, O += P V into TMEM.
 // S has two buffers: the tensor cores form tile i + 1 while the exponentials of
 // tile i are taken. Warps 0-3: softmax; 4, 7 and 5: loads of K and of V, each a ring
-// of its own (K's places are free again after S, V's after P V); 6: MMAs.
-// With bf16 queries two CTAs share an SM, so that the start and the end of one
-// (a third of its time at a window of 1024) run beside the middle of the other.
+// of two (K's places are free again after S, V's after P V); 6: MMAs, one thread.
+// With bf16 queries two CTAs share an SM, so that the start and the end of one run
+// beside the middle of the other.
+//
+// Measured: 8192 bf16 queries, 8 kv heads, window 1024: 91 us, 0.72 PFLOP/s, 44 % of
+// the card's dense rate; 64 f32 rows over 4096 common positions: 18 us of a lone
+// call's 55 (4 tiles of keys a CTA). Bound by the two chains of a tile, about 2000 cycles with two
+// CTAs on an SM: the MMA thread's (three barriers, twelve MMAs queued behind the
+// other CTA's, 656 cycles of tensor pipe each CTA) and the softmax's (S out of TMEM
+// and the maximum 550, the exponentials 700, of which the special-function units
+// need 512). So a barrier is tried before it is waited for, what ends together
+// shares a commit, and the MMA loop's descriptors are constants (101 us before
+// these three and the asynchronous copies of Q).
 //
 // The cache's layout is the MMA's: a block row is 256 bytes whose 16-byte
 // chunks are XOR-swizzled by token & 7 inside each 128-byte half, so 16-row
