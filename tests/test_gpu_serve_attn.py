@@ -501,3 +501,35 @@ def test_workspace_stays_and_grows(plen, grows):
     call(list(range(rows)))
     call([1, 0, 5])
     assert m.gpu.alloc_events()[0] == before + grows
+
+
+@pytest.mark.parametrize("tokens,length,window", [(64, 8192, zc.WINDOW_ALL), (200, 6000, zc.WINDOW_ALL), (1500, 3100, 2900)])
+def test_long_f32_sums_keep_their_precision(tokens, length, window):
+    """f32 queries over thousands of keys. The matrix units round each of the 64 additions that 1024 keys take
+    toward 0, half of 2^-23 on average of a sum that is half its final size on average: 64 * 2^-25 = 1.9e-6 of
+    the result's norm; products, exponentials and the sums in shared memory add well below 1e-6. Bound: 4e-6."""
+    m = make(n_kv=2, max_seq_len=8192)
+    k, v = normal(31, 2, length, D, dtype=torch.bfloat16), normal(32, 2, length, D, dtype=torch.bfloat16)
+    m.kv_write(0, 0, 0, k, v)
+    q = normal(33, 1, tokens, 4, D, scale=1.5)
+    out = torch.full_like(q, float("nan"))
+    torch.cuda.synchronize()
+    m.attn_window(0, [0], q, out, window=window, sinks=3)
+    m.gpu.sync()
+    want = reference(q[0], k, v, window_seen(length, tokens, window, 3))
+    assert float((out[0].double() - want).norm() / want.norm()) <= 4e-6
+
+
+def test_long_f32_sums_follow_a_growing_maximum():
+    """Scores that grow along the cache: the sums kept so far are scaled down each time the maximum grows."""
+    length, tokens = 4000, 100
+    m = make(n_kv=2, max_seq_len=4096)
+    k, v = normal(34, 2, length, D, dtype=torch.float32), normal(35, 2, length, D, dtype=torch.bfloat16)
+    k = (k * torch.linspace(0.1, 6.0, length, device="cuda")[None, :, None]).bfloat16()
+    m.kv_write(0, 0, 0, k, v)
+    q = normal(36, 1, tokens, 4, D, scale=1.5)
+    out = torch.full_like(q, float("nan"))
+    torch.cuda.synchronize()
+    m.attn_window(0, [0], q, out)
+    m.gpu.sync()
+    check(out[0], reference(q[0], k, v, window_seen(length, tokens, zc.WINDOW_ALL, 0)), v, "f32")
