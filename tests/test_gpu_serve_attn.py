@@ -533,3 +533,33 @@ def test_long_f32_sums_follow_a_growing_maximum():
     m.attn_window(0, [0], q, out)
     m.gpu.sync()
     check(out[0], reference(q[0], k, v, window_seen(length, tokens, zc.WINDOW_ALL, 0)), v, "f32")
+
+
+@pytest.mark.parametrize("dims", ["same", "growing"])
+def test_long_single_tokens_keep_their_precision(dims):
+    """One query over 16384 positions in each of 16 rows: a warp takes about 900 positions, 55 additions of 16
+    products each where they are not added up apart, rounded toward 0. Apart after every 512 positions: 32
+    additions, half of 2^-23 on average of a sum that is half its final size on average: 1e-6 of the result's
+    norm; the joins and exponentials add below 1e-6. Bound: 2e-6. Where the
+    maximum keeps growing, the sums are scaled down with it: the bound of the other tests."""
+    rows, length = 16, 16384
+    m = make(n_kv=4, max_batch=rows, max_seqs=rows, max_seq_len=length, kv_blocks=rows * length // 16)
+    kv = {}
+    for i in range(rows):
+        k, v = normal(40 + i, 4, length, D, dtype=torch.bfloat16), normal(80 + i, 4, length, D, dtype=torch.bfloat16)
+        if dims == "growing":
+            k = (k.float() * torch.linspace(0.1, 4.0, length, device="cuda")[None, :, None]).bfloat16()
+        m.kv_write(i, 0, 0, k, v)
+        m.gpu.sync()
+        if i in (0, 9):
+            kv[i] = (k, v)
+    q = normal(39, rows, 8, D, scale=1.5)
+    out = torch.full_like(q, float("nan"))
+    torch.cuda.synchronize()
+    m.attn_window(0, range(rows), q, out)
+    m.gpu.sync()
+    for i, (k, v) in kv.items():
+        want = reference(q[i:i + 1], k, v, torch.ones(1, length, dtype=torch.bool, device="cuda"))
+        if dims == "same":
+            assert float((out[i:i + 1].double() - want).norm() / want.norm()) <= 2e-6
+        check(out[i:i + 1], want, v, "f32")

@@ -15,7 +15,7 @@
 //
 // Measured: 8192 bf16 queries, 8 kv heads, window 1024: 91 us, 0.72 PFLOP/s, 44 % of
 // the card's dense rate; 64 f32 rows over 4096 common positions: 18 us of a lone
-// call's 55 (4 tiles of keys a CTA). Bound by the two chains of a tile, about 2000 cycles with two
+// call's 57 (4 tiles of keys a CTA). Bound by the two chains of a tile, about 2000 cycles with two
 // CTAs on an SM: the MMA thread's (three barriers, twelve MMAs queued behind the
 // other CTA's, 656 cycles of tensor pipe each CTA) and the softmax's (S out of TMEM
 // and the maximum 550, the exponentials 700, of which the special-function units
