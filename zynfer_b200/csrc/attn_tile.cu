@@ -30,10 +30,11 @@
 // as the transposed operand). A block that is not there is a box past the end
 // of the tensor: zeros.
 //
-// bf16 queries: one MMA term, P rounded to bf16 (8 bits, the output's own
-// precision; its sum is taken from the f32 values). f32 queries: Q and P are
-// split into three bf16 terms each (24 bits, nothing is lost) against the
-// exact bf16 K and V: three times the MMAs, and f32 sums throughout.
+// bf16 queries: Q is one MMA term as it lies, P two (16 bits; its sum is taken from
+// the f32 values), so that the result has one rounding, its own. With P as one term
+// the error was that of two roundings: 2.3e-3 of the result against 1.7e-3. f32
+// queries: Q and P are split into three bf16 terms each (24 bits, nothing is lost)
+// against the exact bf16 K and V: three times the MMAs, and f32 sums throughout.
 // The accumulator is rescaled only when a row's maximum grows by more than
 // 2^8 (the reference point of its exponentials may lag behind by that much).
 //
@@ -72,6 +73,7 @@ using u64x2 = unsigned long long;
 template <int TERMS>
 struct Lay {
     static constexpr int CTAS = TERMS == 1 ? 2 : 1;      // per SM
+    static constexpr int PTERMS = TERMS == 1 ? 2 : 3;    // of P (TERMS: of Q)
     static constexpr int KST = 2, VST = 2;  // K's ring is S's: one barrier tells that S is there and K's place free
     static constexpr int QTERM = kRows * 256;
     static constexpr int K = TERMS * QTERM, V = K + KST * kTileBytes;
@@ -87,6 +89,7 @@ struct Lay {
     static constexpr int ACCS = TERMS == 1 ? 1 : 2;
     static constexpr int S_COL = ACCS * kD, S_STEP = TERMS == 1 ? 64 : 128;
     static constexpr int COLS = TERMS == 1 ? 256 : 512;
+    static_assert(PTERMS * (TILE / 2) <= S_STEP && S_COL + 2 * S_STEP <= COLS, "P lies over S");
 };
 
 __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
@@ -229,8 +232,7 @@ __device__ __forceinline__ Job find_job(const ServeRowsT<N>& rows, const TileLis
     return j;
 }
 
-// Three (or one) bf16 terms of p, packed in pairs: nothing is left of p after
-// the third.
+// bf16 terms of x0 and x1, packed in pairs: nothing is left after the third.
 template <int TERMS>
 __device__ __forceinline__ void split_pair(float x0, float x1, uint32_t (&t)[TERMS]) {
 #pragma unroll
@@ -367,11 +369,14 @@ __global__ void __launch_bounds__(kThreads, Lay<TERMS>::CTAS)
                     const uint32_t v = qs + L::V + o * kTileBytes;
                     const bool more = TERMS == 1 ? j > 0 : j % kFlush > 0;
 #pragma unroll
-                    for (int t = TERMS - 1; t >= 0; --t)
+                    for (int t = L::PTERMS - 1; t >= 0; --t) {
+                        const int apart = L::ACCS == 2 && t > 0;  // in the small terms' accumulator
+                        const bool begins = t == L::PTERMS - 1 || (L::ACCS == 2 && t == 0);  // the first product of its accumulator
 #pragma unroll
                         for (int kk = 0; kk < TILE / 16; ++kk)
-                            mma_ts(tmem + (t > 0 ? kD : 0), tmem + L::S_COL + o * L::S_STEP + t * (TILE / 2) + kk * 8,
-                                   sdesc(v + kk * 2048, kHalf), id_o, more || (t > 0 && t < TERMS - 1) || kk);
+                            mma_ts(tmem + apart * kD, tmem + L::S_COL + o * L::S_STEP + t * (TILE / 2) + kk * 8,
+                                   sdesc(v + kk * 2048, kHalf), id_o, more || !begins || kk);
+                    }
                     mma_commit(&o_full[o]);
                 }
                 return true;
@@ -524,7 +529,7 @@ __global__ void __launch_bounds__(kThreads, Lay<TERMS>::CTAS)
             const float neg = m_ref == -INFINITY ? 0.0f : -m_ref;
             const u64x2 scale_2 = pack2(scale2, scale2), neg_2 = pack2(neg, neg);
             u64x2 sum[2] = {0ull, 0ull};
-            uint32_t p[TERMS][32];
+            uint32_t p[L::PTERMS][32];
 #pragma unroll
             for (int e = 0; e < 32; ++e) {
                 float x0, x1;
@@ -532,13 +537,13 @@ __global__ void __launch_bounds__(kThreads, Lay<TERMS>::CTAS)
                 x0 = exp2_fast(x0);
                 x1 = exp2_fast(x1);
                 sum[e & 1] = add2(sum[e & 1], pack2(x0, x1));
-                uint32_t u[TERMS];
-                split_pair<TERMS>(x0, x1, u);
+                uint32_t u[L::PTERMS];
+                split_pair<L::PTERMS>(x0, x1, u);
 #pragma unroll
-                for (int k = 0; k < TERMS; ++k) p[k][e] = u[k];
+                for (int k = 0; k < L::PTERMS; ++k) p[k][e] = u[k];
             }
 #pragma unroll
-            for (int k = 0; k < TERMS; ++k) tmem_st32(s_at + k * (TILE / 2), p[k]);
+            for (int k = 0; k < L::PTERMS; ++k) tmem_st32(s_at + k * (TILE / 2), p[k]);
             float l0, l1;
             unpack2(add2(sum[0], sum[1]), l0, l1);
             l += l0 + l1;
