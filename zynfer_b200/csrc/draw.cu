@@ -52,6 +52,7 @@ constexpr int kWarps = kThreads / kWarp;
 constexpr int kList = kThreads;        // tokens of a bin that are sorted
 constexpr float kOne = 8589934592.0f;  // 2^33, the weight of the largest logit
 constexpr float kEnd = 23.6f;          // exp(-kEnd) 2^33 < 1/2: weights beyond are 0
+constexpr float kTiny = 1e-30f;        // exp(-kTiny) is 1
 constexpr int kIndexBits = 18;         // vocab <= 2^18
 constexpr float kMagic = 8388608.0f;   // 2^23: x + 2^23 holds rint(x) in its low bits
 constexpr unsigned kAll = 0xFFFFFFFFu;
@@ -85,8 +86,9 @@ struct RowRule {
         const float d = l - m;
         return (odd && l == m ? 0.0f : d) * inv_t;
     }
-    __device__ __forceinline__ int bin(float x) const {
-        return __float_as_int(__fmaf_rn(fminf(-x, end), bin_scale, kMagic)) - 0x4B000000;
+    // (0 <= fminf(-x, end) <= end, which bin_scale takes to NB - 1; `last` holds it there whatever x is)
+    __device__ __forceinline__ int bin(float x, int last) const {
+        return (int)min((uint32_t)(__float_as_int(__fmaf_rn(fminf(-x, end), bin_scale, kMagic)) - 0x4B000000), (uint32_t)last);
     }
     // does a token of exponential e weigh anything? (NaN does not)
     __device__ __forceinline__ bool weighs(float e) const { return e >= least; }
@@ -348,7 +350,8 @@ __global__ void __launch_bounds__(kThreads, 2) draw_kernel(const __grid_constant
     rule.end = fminf(-rule.exponent(least), kEnd);  // (with a logit of -inf in the row: where weights end)
     if (!(rule.end >= 0.0f)) rule.end = kEnd;
     if (min_p > 0.0f) rule.end = fminf(rule.end, 0.01f - logf(min_p));
-    rule.bin_scale = rule.end > 0.0f ? (float)(NB - 1) / rule.end : 0.0f;
+    // (a range below kTiny weighs one, and its bins' scale could leave the floats: one bin, which the order divides)
+    rule.bin_scale = rule.end > kTiny ? (float)(NB - 1) / rule.end : 0.0f;
     const bool counts = k > 0;
 
     // Adds this CTA's tokens into the bins (bin0 >= 0: those of that bin between
@@ -362,7 +365,7 @@ __global__ void __launch_bounds__(kThreads, 2) draw_kernel(const __grid_constant
         for (int from = 0; from < n; from += kBatch) {
             each(from, min(n, from + kBatch), [&](float l, int i) {
                 const float x = rule.exponent(l), e = expf(x);
-                int b = rule.bin(x);
+                int b = rule.bin(x, NB - 1);
                 if (bin0 >= 0) {
                     if (b != bin0) return;
                     const u64 c = composite(l, i0 + i);
@@ -525,7 +528,7 @@ __global__ void __launch_bounds__(kThreads, 2) draw_kernel(const __grid_constant
                 each(0, n, [&](float l, int i) {
                     if (!(l <= l_hi) || l < l_lo) return;
                     const float x = rule.exponent(l);
-                    if (rule.bin(x) != bin0 || !rule.weighs(expf(x))) return;
+                    if (rule.bin(x, NB - 1) != bin0 || !rule.weighs(expf(x))) return;
                     const u64 c = composite(l, i0 + i);
                     if (c >= c_lo && c <= c_hi) f(c);
                 });
