@@ -400,7 +400,7 @@ ZYNFER_CU_API int zynfer_cu_attn_window(ZynferCuCtx *ctx, uint32_t layer, const 
  * zynfer_cu_decode_drawn (host arrays [batch]); a null array is its neutral
  * value in every row. */
 typedef struct ZynferCuDrawRule {
-    const float *temperature;  /* 1; <= 0 or NaN takes the largest logit */
+    const float *temperature;  /* 1; <= 0 or NaN takes the largest logit; at least 2^-128 else */
     const int32_t *top_k;      /* 0 (or less): every token */
     const float *top_p;        /* 1 (or more, or NaN): every token; <= 0: the first */
     const float *min_p;        /* 0 (or less, or NaN): every token; at most 1 */

@@ -51,3 +51,21 @@ def test_logits_next_to_equal(gpu, rows, vocab, step):
     l = torch.zeros(rows, vocab, device="cuda")
     l[:, vocab // 3] = step
     equal_weights(gpu, l, 1.0)
+
+
+@pytest.mark.parametrize("rows,vocab", SHAPES)
+def test_logits_whole_denormals_apart(gpu, rows, vocab):
+    """The bins are a few times the smallest number wide: no token falls between them. The weights are all one."""
+    l = -torch.arange(vocab, device="cuda", dtype=torch.float64)[None].repeat(rows, 1) * 2.0 ** -149
+    equal_weights(gpu, l.float(), 1e-26)
+
+
+@pytest.mark.parametrize("t", [4e-39, 1e-42])
+def test_very_small_temperatures(gpu, t):
+    """Differences of 1e-40 at temperatures near them (1e-42 counts as 2^-128)."""
+    vocab, u = 1000, np.linspace(0.02, 0.98, 12).astype(np.float32)
+    x = (-1e-40 * torch.arange(vocab, dtype=torch.float64)).float().cuda()[None].repeat(12, 1)
+    for k, p in ((0, 1.0), (0, 0.7), (40, 1.0), (40, 0.7)):
+        ids, lp = draw(gpu, x, u, t=t, k=k, p=p)
+        for r in range(12):
+            check_row(x[r], float(u[r]), max(float(np.float32(t)), 1.0 / MAX), k, float(np.float32(p)), 0.0, int(ids[r]), float(lp[r]))

@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(kThreads, 2) draw_kernel(const __grid_constant
     }
 
     // ---- bins even in (m - l) / T, up to the last weight
-    // (1 / T beyond the floats: the largest of them gives the same zeros)
+    // (1 / T beyond the floats: the largest of them, as for a temperature of 2^-128)
     RowRule rule{top, fminf(1.0f / T, 3.402823466e38f), 0.0f, 0.0f, fmaxf(min_p, 5.8207667e-11f), top == INFINITY};
     rule.end = fminf(-rule.exponent(least), kEnd);  // (with a logit of -inf in the row: where weights end)
     if (!(rule.end >= 0.0f)) rule.end = kEnd;
@@ -516,9 +516,11 @@ __global__ void __launch_bounds__(kThreads, 2) draw_kernel(const __grid_constant
                 c_lo = max(c_lo, hi - ((1ull << shift) - 1ull));
                 c_hi = hi;
             }
-            // the bin's logits lie between these (a bin's width and a few roundings of
-            // slack): a comparison leaves few tokens to look at closely
-            const float width = rule.bin_scale > 0.0f ? T / rule.bin_scale : INFINITY, slack = width + 1e-6f * fabsf(top);
+            // the bin's logits lie between these (a bin's width, of the 1 / T that the
+            // exponents take, and a few roundings of slack, those of a width below the
+            // normal numbers among them): a comparison leaves few tokens to look at closely
+            const float width = rule.bin_scale > 0.0f ? (1.0f / rule.bin_scale) / rule.inv_t : INFINITY;
+            const float slack = width + 1e-6f * fabsf(top) + 1e-41f;
             const float l_hi = bin0 < 2 ? INFINITY : top - ((float)bin0 * width - slack) * (1.0f - 1e-6f);
             const float l_lo = bin0 >= NB - 2 ? -INFINITY : top - ((float)bin0 * width + slack) * (1.0f + 1e-6f);
             u64 mx = 0ull, mn = ~0ull;
