@@ -533,17 +533,19 @@ class Model:
                           (self.gpu.h, seq, layer, pos, k.shape[1], k.data_ptr(), v.data_ptr(), _dtype(k)))
 
     def _row_stride(self, t, n: int, tokens=None):
-        """Stride of the rows of a [n, n_q, head_dim] or [n, tokens, n_q, head_dim] tensor, which lie at one stride."""
+        """Stride of the rows of a [n, n_q, head_dim] or [n, tokens, n_q, head_dim] tensor, which lie at one stride
+        and do not overlap (a broadcast tensor's rows are one)."""
         a, shape, st = self.arch, t.shape, t.stride()
+        dense = a.n_q * a.head_dim
         if tokens is None:
-            ok, step = shape == (n, a.n_q, a.head_dim), st[0] if n > 1 else 0
+            ok, step = shape == (n, a.n_q, a.head_dim), st[0] if n > 1 else dense
         else:
-            ok, step = shape == (n, tokens, a.n_q, a.head_dim), st[1] if tokens > 1 else (st[0] if n > 1 else 0)
+            ok, step = shape == (n, tokens, a.n_q, a.head_dim), st[1] if tokens > 1 else (st[0] if n > 1 else dense)
             ok = ok and (tokens == 1 or n == 1 or st[0] == tokens * st[1])
-        if not ok or st[-1] != 1 or st[-2] != a.head_dim:
+        if not ok or st[-1] != 1 or st[-2] != a.head_dim or step < dense:
             raise InvalidArgument(f"expected rows of dense [{a.n_q}, {a.head_dim}] heads at one stride, {n} sequences"
                                   f"{'' if tokens is None else f' of {tokens} tokens'}; got shape {tuple(shape)}, strides {st}")
-        return step or a.n_q * a.head_dim
+        return step
 
     def attn_shared(self, layer: int, seqs, q, out, stream=None):
         """Decode attention of one query per sequence (device q and out [B, n_q, head_dim], f32 or bf16, rows at
