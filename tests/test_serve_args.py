@@ -9,10 +9,22 @@ torch = pytest.importorskip("torch")
 D = 128
 
 
+class NoGpu(zc.Gpu):
+    """A context that is none: its argument checks alone, and a call that gets past them is an error of the test."""
+
+    def __init__(self):
+        self.h, self.device = None, 0
+        self._rule = zc.DrawRule()
+        self._rule_ref = None
+
+    def _enqueue(self, *call):
+        raise AssertionError("a call reached the library")
+
+
 @pytest.fixture
 def model():
-    """A model without a context: its argument checks alone."""
     m = object.__new__(zc.Model)
+    m.gpu = NoGpu()
     m.arch = zc.Arch(vocab=512, hidden=512, inter=512, layers=1, n_q=4, n_kv=2, max_pos=512)
     return m
 
@@ -46,3 +58,40 @@ def test_strides_of_rows(model):
                          (torch.zeros(3, 4, D).transpose(1, 2), 3, None), (torch.zeros(3, 4, 64), 3, None)):
         with pytest.raises(zc.InvalidArgument):
             model._row_stride(t, n, tokens)
+
+
+def test_tensors_off_the_gpu_are_refused(model, monkeypatch):
+    """Host tensors, and with every other argument on the GPU each one alone."""
+    monkeypatch.setattr(zc, "lib", lambda: type("Lib", (), {"__getattr__": lambda self, name: name})())
+    host = torch.zeros
+
+    class Device:
+        """A tensor that says it lies on cuda:`index`."""
+
+        def __init__(self, t, index=0):
+            self.t, self.index, self.is_cuda, self.device = t, index, True, f"cuda:{index}"
+
+        def get_device(self):
+            return self.index
+
+        def __getattr__(self, name):
+            return getattr(self.t, name)
+
+    q = lambda: host(2, 4, D)  # noqa: E731
+    kv = lambda: host(2, 5, D)  # noqa: E731
+    f, i = lambda: host(2), lambda: host(2, dtype=torch.int32)  # noqa: E731
+    calls = [
+        (lambda a, b: model.attn_shared(0, [0, 1], a, b), [q, q]),
+        (lambda a, b: model.attn_window(0, [0, 1], a, b, window=3), [q, q]),
+        (lambda a, b: model.kv_write(0, 0, 0, a, b), [kv, kv]),
+        (lambda l, u, ids, lp, t, k, p, m: model.gpu.sample_rows(l, u, ids, lp, t, k, p, m), [lambda: host(2, 64), f, i, f, f, i, f, f]),
+    ]
+    for call, make in calls:
+        with pytest.raises(zc.InvalidArgument, match="cuda:0"):
+            call(*(x() for x in make))
+        for bad in range(len(make)):
+            for wrong in (make[bad](), Device(make[bad](), 1)):
+                with pytest.raises(zc.InvalidArgument, match="cuda:0"):
+                    call(*(wrong if n == bad else Device(x()) for n, x in enumerate(make)))
+        with pytest.raises(AssertionError):
+            call(*(Device(x()) for x in make))

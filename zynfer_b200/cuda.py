@@ -199,13 +199,20 @@ def _dtype(t) -> int:
     return dt
 
 
-def _row_values(t, shape, kinds, name: str):
+def _on_device(t, device: int, name: str):
+    """Address of a tensor, which lies on the context's GPU: a kernel would fault on any other."""
+    if not t.is_cuda or t.get_device() != device:
+        raise InvalidArgument(f"{name} must be on cuda:{device}, not {t.device}")
+    return t.data_ptr()
+
+
+def _row_values(t, shape, kinds, device: int, name: str):
     """Address of a dense tensor of one value per row (None: null)."""
     if t is None:
         return None
     if t.shape != shape or _kind(t) not in kinds or not t.is_contiguous():
         raise InvalidArgument(f"{name} must be a dense {kinds[0]} tensor of one value per row")
-    return t.data_ptr()
+    return _on_device(t, device, name)
 
 
 _F32, _I32 = ("float32",), ("int32", "uint32")
@@ -292,6 +299,7 @@ class Gpu:
         h = VP()
         rc = L.zynfer_cu_create(device, C.byref(h))
         self.h = h
+        self.device = device
         if rc != OK:
             msg = L.zynfer_cu_last_error(h).decode() if h else "create failed"
             if h:
@@ -356,14 +364,14 @@ class Gpu:
         if logits.dim() != 2 or logits.stride(1) != 1:
             raise InvalidArgument("logits must be [rows, vocab] with unit inner stride")
         rows, vocab = logits.shape
-        n, rule = (rows,), self._rule
-        rule.temperature = _row_values(temperature, n, _F32, "temperature")
-        rule.top_k = _row_values(top_k, n, _I32, "top_k")
-        rule.top_p = _row_values(top_p, n, _F32, "top_p")
-        rule.min_p = _row_values(min_p, n, _F32, "min_p")
-        call = (self.h, logits.data_ptr(), _dtype(logits), logits.stride(0) if rows > 1 else vocab, rows, vocab,
-                _row_values(uniforms, n, _F32, "uniforms"), self._rule_ref, _row_values(ids, n, _I32, "ids"),
-                _row_values(logprobs, n, _F32, "logprobs"))
+        n, rule, dev = (rows,), self._rule, self.device
+        rule.temperature = _row_values(temperature, n, _F32, dev, "temperature")
+        rule.top_k = _row_values(top_k, n, _I32, dev, "top_k")
+        rule.top_p = _row_values(top_p, n, _F32, dev, "top_p")
+        rule.min_p = _row_values(min_p, n, _F32, dev, "min_p")
+        call = (self.h, _on_device(logits, dev, "logits"), _dtype(logits), logits.stride(0) if rows > 1 else vocab, rows, vocab,
+                _row_values(uniforms, n, _F32, dev, "uniforms"), self._rule_ref, _row_values(ids, n, _I32, dev, "ids"),
+                _row_values(logprobs, n, _F32, dev, "logprobs"))
         self._enqueue(stream, lib().zynfer_cu_sample_rows, call)
 
     def wait_stream(self, stream):
@@ -530,7 +538,8 @@ class Model:
                  k.dtype == v.dtype and k.is_contiguous() and v.is_contiguous(),
                  "k and v must be dense [n_kv, n, head_dim] tensors of one type")
         self.gpu._enqueue(stream, lib().zynfer_cu_kv_write,
-                          (self.gpu.h, seq, layer, pos, k.shape[1], k.data_ptr(), v.data_ptr(), _dtype(k)))
+                          (self.gpu.h, seq, layer, pos, k.shape[1], _on_device(k, self.gpu.device, "k"),
+                           _on_device(v, self.gpu.device, "v"), _dtype(k)))
 
     def _row_stride(self, t, n: int, tokens=None):
         """Stride of the rows of a [n, n_q, head_dim] or [n, tokens, n_q, head_dim] tensor, which lie at one stride
@@ -554,8 +563,8 @@ class Model:
         if q.dtype != out.dtype:
             raise InvalidArgument("q and out must have one type")
         self.gpu._enqueue(stream, lib().zynfer_cu_attn_shared,
-                          (self.gpu.h, layer, ids, n, q.data_ptr(), self._row_stride(q, n), out.data_ptr(),
-                           self._row_stride(out, n), _dtype(q)))
+                          (self.gpu.h, layer, ids, n, _on_device(q, self.gpu.device, "q"), self._row_stride(q, n),
+                           _on_device(out, self.gpu.device, "out"), self._row_stride(out, n), _dtype(q)))
 
     def attn_window(self, layer: int, seqs, q, out, window: int = WINDOW_ALL, sinks: int = 0, stream=None):
         """Attention of the last T cached positions of each sequence (device q and out [B, T, n_q, head_dim], or
@@ -567,8 +576,8 @@ class Model:
         tokens = q.shape[1] if dims == 4 else None
         self.gpu._enqueue(stream, lib().zynfer_cu_attn_window,
                           (self.gpu.h, layer, ids, n, 1 if tokens is None else tokens, min(window, WINDOW_ALL),
-                           min(sinks, WINDOW_ALL), q.data_ptr(), self._row_stride(q, n, tokens), out.data_ptr(),
-                           self._row_stride(out, n, tokens), _dtype(q)))
+                           min(sinks, WINDOW_ALL), _on_device(q, self.gpu.device, "q"), self._row_stride(q, n, tokens),
+                           _on_device(out, self.gpu.device, "out"), self._row_stride(out, n, tokens), _dtype(q)))
 
     def rmsnorm_qk_rope(self, qkv, rows: int, q_norm, k_norm, pos0: int, q_out, k_out):
         """Per-head q/k RMSNorm + RoPE of `rows` tokens (device pointers, heads-major outputs)."""
