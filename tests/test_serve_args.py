@@ -95,3 +95,33 @@ def test_tensors_off_the_gpu_are_refused(model, monkeypatch):
                     call(*(wrong if n == bad else Device(x()) for n, x in enumerate(make)))
         with pytest.raises(AssertionError):
             call(*(Device(x()) for x in make))
+
+
+class Library:
+    """The native library as a list of the calls that reach it."""
+
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        return lambda *a: self.calls.append((name, a)) or 0
+
+
+PATHS = [
+    (lambda m, w, s: m.prefill_chunk(0, [1, 2], window=w, sinks=s), 4),
+    (lambda m, w, s: m.decode_drawn([0, 1], [1, 2], [0.1, 0.2], window=w, sinks=s), 4),
+]
+
+
+@pytest.mark.parametrize("call,at", PATHS)
+def test_windows_of_the_model_path_do_not_wrap(model, monkeypatch, call, at):
+    lib = Library()
+    monkeypatch.setattr(zc, "lib", lambda: lib)
+    for window, sinks in ((-1, 0), (5, -1), (-2 ** 32, 3)):
+        with pytest.raises(zc.InvalidArgument):
+            call(model, window, sinks)
+    assert not lib.calls
+    for window, sinks, want in ((0, 0, (0, 0)), (7, 3, (7, 3)), (zc.WINDOW_ALL, 0, (zc.WINDOW_ALL, 0)),
+                                (2 ** 32, 2 ** 40, (zc.WINDOW_ALL, zc.WINDOW_ALL)), (2 ** 32 + 10, 1, (zc.WINDOW_ALL, 1))):
+        call(model, window, sinks)
+        assert lib.calls[-1][1][at:at + 2] == want

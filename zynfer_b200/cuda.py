@@ -230,6 +230,13 @@ def _ids(seqs):
     return a.ctypes.data, a.size, a
 
 
+def _mask(window: int, sinks: int):
+    """A window and sinks as the library takes them: 32 bits, anything above as the largest."""
+    if window < 0 or sinks < 0:
+        raise InvalidArgument("window and sinks must not be negative")
+    return min(window, WINDOW_ALL), min(sinks, WINDOW_ALL)
+
+
 def _require(ok: bool, what: str):
     if not ok:
         raise InvalidArgument(what)
@@ -571,12 +578,13 @@ class Model:
         [B, n_q, head_dim] for T = 1) over the last `window` positions up to each and the first `sinks`. Asynchronous."""
         ids, n, keep = _ids(seqs)
         dims = q.dim()
-        if q.dtype != out.dtype or dims not in (3, 4) or window < 0 or sinks < 0:
-            raise InvalidArgument("q and out must be [B, n_q, d] or [B, T, n_q, d] of one type; window and sinks not negative")
+        if q.dtype != out.dtype or dims not in (3, 4):
+            raise InvalidArgument("q and out must be [B, n_q, d] or [B, T, n_q, d] of one type")
+        window, sinks = _mask(window, sinks)
         tokens = q.shape[1] if dims == 4 else None
         self.gpu._enqueue(stream, lib().zynfer_cu_attn_window,
-                          (self.gpu.h, layer, ids, n, 1 if tokens is None else tokens, min(window, WINDOW_ALL),
-                           min(sinks, WINDOW_ALL), _on_device(q, self.gpu.device, "q"), self._row_stride(q, n, tokens),
+                          (self.gpu.h, layer, ids, n, 1 if tokens is None else tokens, window, sinks,
+                           _on_device(q, self.gpu.device, "q"), self._row_stride(q, n, tokens),
                            _on_device(out, self.gpu.device, "out"), self._row_stride(out, n, tokens), _dtype(q)))
 
     def rmsnorm_qk_rope(self, qkv, rows: int, q_norm, k_norm, pos0: int, q_out, k_out):
@@ -619,6 +627,7 @@ class Model:
 
     def prefill_chunk(self, seq: int, tokens, window: int = WINDOW_ALL, sinks: int = 0, want_logits: bool = True):
         """Append a chunk of a prompt to a sequence, with windowed attention; the last token's logits and argmax."""
+        window, sinks = _mask(window, sinks)
         t = np.ascontiguousarray(tokens, np.uint32)
         logits = np.empty(self.arch.vocab, np.float32) if want_logits else None
         am = np.zeros(1, np.uint32)
@@ -633,6 +642,7 @@ class Model:
         t = np.ascontiguousarray(tokens, np.uint32)
         u = np.ascontiguousarray(uniforms, np.float32)
         _require(t.size == s.size and u.size == s.size, "one token and one random number per sequence")
+        window, sinks = _mask(window, sinks)
 
         def per_row(x, kind):
             return None if x is None else np.ascontiguousarray(np.broadcast_to(np.asarray(x, kind), (s.size,)))
