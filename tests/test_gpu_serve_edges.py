@@ -4,7 +4,7 @@ splits, and plans of batches whose prompts are nested."""
 import numpy as np
 import pytest
 
-from test_gpu_serve_attn import DTYPES, D, make, normal, reference, window_seen
+from test_gpu_serve_attn import DTYPES, D, check, make, normal, reference, window_seen
 from zynfer_b200 import cuda as zc
 
 pytestmark = pytest.mark.gpu
@@ -52,3 +52,105 @@ def test_bf16_results_are_rounded_once(case):
     norm = want.norm()
     once = float((want.bfloat16().double() - want).norm() / norm)
     assert float((out.double() - want).norm() / norm) <= once + 1e-4
+
+
+# ways a row is split: (sequences, cached positions, queries of each, own positions of forked rows)
+SPLITS = {"one token": (3, 3000, 1), "short": (8, 40, 1), "few queries": (2, 3000, 40), "chunk": (1, 900, 700), "prompt": (64, 992, 0)}
+
+
+def split_case(how, dtype, edit):
+    """K and V [rows, n_kv, L, D], q [rows, T, n_q, D] and the model that has them in its cache, after edit(q, k, v) (the
+    rows of "prompt" share every position but their last 3)."""
+    rows, length, tokens = SPLITS[how]
+    own = 3 if how == "prompt" else 0
+    m = make(n_kv=4, max_batch=rows, max_seqs=rows, max_seq_len=length + own + 16, kv_blocks=rows * (length // 16 + 3) if not own else length // 16 + 4 * rows)
+    k, v = (normal(seed, 1 if own else rows, 4, length, D, dtype=torch.bfloat16) for seed in (211, 212))
+    if own:
+        k, v = (torch.cat([x.expand(rows, -1, -1, -1), normal(seed, rows, 4, own, D, dtype=torch.bfloat16)], 2) for x, seed in ((k, 213), (v, 214)))
+    q = normal(215, rows, max(1, tokens), 8, D, dtype=DTYPES[dtype], scale=1.5)
+    edit(q, k, v)
+    torch.cuda.synchronize()
+    for i in range(rows):
+        if own and i:
+            m.seq_fork(i, 0, length)
+        first = length if own and i else 0
+        a, b = k[i, :, first:].contiguous(), v[i, :, first:].contiguous()
+        if own and not i:  # the prompt is forked before the first row's own positions
+            torch.cuda.synchronize()
+            m.kv_write(0, 0, 0, a[:, :length].contiguous(), b[:, :length].contiguous())
+            m.gpu.sync()
+            continue
+        torch.cuda.synchronize()
+        m.kv_write(i, 0, first, a, b)
+        m.gpu.sync()
+    if own:
+        a, b = k[0, :, length:].contiguous(), v[0, :, length:].contiguous()
+        torch.cuda.synchronize()
+        m.kv_write(0, 0, length, a, b)
+        m.gpu.sync()
+    out = torch.full_like(q, 7.0)
+    torch.cuda.synchronize()
+    if own:
+        m.attn_shared(0, range(rows), q[:, 0], out[:, 0])
+    else:
+        m.attn_window(0, range(rows), q, out)
+    m.gpu.sync()
+    return q, k, v, out
+
+
+def expect(q, k, v, out, dtype, nan):
+    """nan [rows, T, n_q]: query heads that are NaN in every dim; the others follow the formula."""
+    tokens, length = q.shape[1], k.shape[2]
+    seen = window_seen(length, tokens, zc.WINDOW_ALL, 0)
+    for i in range(q.shape[0]):
+        assert torch.isnan(out[i][nan[i]]).all()
+        want = reference(torch.nan_to_num(q[i]), torch.nan_to_num(k[i]), torch.nan_to_num(v[i]), seen)
+        check(out[i][~nan[i]], want[~nan[i]], torch.nan_to_num(v[i]), dtype)
+
+
+def none(q):
+    return torch.zeros(q.shape[:3], dtype=torch.bool, device="cuda")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("how", list(SPLITS))
+def test_a_nan_query_gives_nan_however_its_row_is_split(how, dtype):
+    def edit(q, k, v):
+        q[-1, -1, 5, 17] = float("nan")
+    q, k, v, out = split_case(how, dtype, edit)
+    nan = none(q)
+    nan[-1, -1, 5] = True
+    expect(q, k, v, out, dtype, nan)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("how,where", [("one token", slice(512, 1536)), ("one token", slice(2999, 3000)), ("short", slice(39, 40)),
+                                       ("few queries", slice(512, 1536)), ("prompt", slice(994, 995)), ("prompt", slice(992, 995))])
+def test_nan_scores_that_fill_a_piece_reach_the_result(how, where, dtype):
+    """Every key of a piece of the last row is NaN in one kv head: the piece has no maximum, its sum is NaN."""
+    def edit(q, k, v):
+        k[-1, 2, where] = float("nan")
+    q, k, v, out = split_case(how, dtype, edit)
+    nan = none(q)
+    seen = window_seen(k.shape[2], q.shape[1], zc.WINDOW_ALL, 0)[:, where].any(1)
+    nan[-1, seen, 4:6] = True
+    expect(q, k, v, out, dtype, nan)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("how", ["one token", "few queries", "prompt"])
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_nan_behind_a_weight_of_zero_reaches_the_result(how, which, dtype):
+    """A NaN key or value among keys whose weights are too small for f32 beside the first positions'."""
+    def edit(q, k, v):
+        k[:, :, :64] *= 30.0
+        at = 500 if how == "prompt" else k.shape[2] - 100
+        (k if which == "k" else v)[-1 if how != "prompt" else slice(None), 1, at] = float("nan")
+    q, k, v, out = split_case(how, dtype, edit)
+    rows = slice(None) if how == "prompt" else slice(-1, None)
+    nan = none(q)
+    nan[rows, -1, 2:4] = True
+    hit = out[rows, -1, 2:4]
+    assert torch.isnan(hit).all()
+    clean = torch.isfinite(out[:, -1])
+    assert clean[~nan[:, -1]].all()

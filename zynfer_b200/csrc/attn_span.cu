@@ -75,10 +75,10 @@ __device__ __forceinline__ uint32_t term_of(float x0, float x1, int term) {
     return t;
 }
 
-// x joined with a record in shared memory.
+// x joined with a record in shared memory (NaN and infinities as in join_records).
 __device__ __forceinline__ void join_shared(Partial& x, const float* rec) {
     const float m = rec[0], l = rec[1];
-    if (m == -INFINITY) return;
+    if (m == -INFINITY && l == 0.0f) return;  // nothing seen
     const float4 v = *reinterpret_cast<const float4*>(rec + 4 + 4 * (threadIdx.x % kWarp));
     const float mn = fmaxf(x.m, m);
     const float c0 = x.m == -INFINITY ? 0.0f : exp2_fast(x.m - mn), c1 = exp2_fast(m - mn);
@@ -86,7 +86,7 @@ __device__ __forceinline__ void join_shared(Partial& x, const float* rec) {
     x.l = x.l * c0 + l * c1;
     const float f[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x.acc[e] = (c0 == 0.0f ? 0.0f : x.acc[e] * c0) + f[e] * c1;
+    for (int e = 0; e < 4; ++e) x.acc[e] = x.acc[e] * c0 + f[e] * c1;
 }
 
 template <int N>

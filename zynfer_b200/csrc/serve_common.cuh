@@ -87,7 +87,9 @@ struct Partial {
 using SlowRow = Partial;
 __device__ __forceinline__ Partial no_partial() { return Partial{-INFINITY, 0.0f, {0.0f, 0.0f, 0.0f, 0.0f}}; }
 
-// x joined with `cnt` records in global memory, in order: 2^(m - M) weighs each.
+// x joined with `cnt` records in global memory, in order: 2^(m - M) weighs each. A
+// record of nothing seen is m = -inf with zeros; one of NaN scores alone is m = -inf
+// with l NaN, and that goes into the sum as a NaN or infinity does whose weight is 0.
 // Lane j reads the (m, l) of record j and weighs it, so a batch of up to 32
 // costs one exponential and, with kAhead accumulators requested before any is
 // used, about cnt / kAhead round trips.
@@ -113,14 +115,14 @@ __device__ __forceinline__ void join_records(Partial& x, const float* base, int 
                 c = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - M);
                 const float cx = x.m == -INFINITY ? 0.0f : exp2_fast(x.m - M);
                 x.m = M;
-                x.l = (cx == 0.0f ? 0.0f : x.l * cx) + warp_sum(c == 0.0f ? 0.0f : ml.y * c);
+                x.l = x.l * cx + warp_sum(ml.y * c);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x.acc[e] = cx == 0.0f ? 0.0f : x.acc[e] * cx;
+                for (int e = 0; e < 4; ++e) x.acc[e] *= cx;
             }
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) {
                 const float ck = __shfl_sync(0xFFFFFFFFu, c, (i + k) & (kWarp - 1));
-                if (i + k < some && ck != 0.0f) {
+                if (i + k < some) {
                     x.acc[0] += v[k].x * ck;
                     x.acc[1] += v[k].y * ck;
                     x.acc[2] += v[k].z * ck;
