@@ -154,3 +154,52 @@ def test_nan_behind_a_weight_of_zero_reaches_the_result(how, which, dtype):
     assert torch.isnan(hit).all()
     clean = torch.isfinite(out[:, -1])
     assert clean[~nan[:, -1]].all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("how", list(SPLITS))
+def test_an_infinite_value_that_is_seen_is_infinite(how, dtype):
+    """sum p v with p > 0: infinity of its sign in its dims, NaN where two of both signs meet, the formula elsewhere."""
+    own = SPLITS[how][1] + 1 if how == "prompt" else SPLITS[how][1] - 1  # the last row alone sees it, and its last query
+
+    def edit(q, k, v):
+        v[-1, 2, 3, 5:9] = float("inf") if how != "prompt" else v[-1, 2, 3, 5:9]
+        v[-1, 2, own, 8] = v[-1, 2, own, 90] = -float("inf")
+    q, k, v, out = split_case(how, dtype, edit)
+    hit = out[-1, -1, 4:6]
+    if how != "prompt":
+        assert (hit[:, 5:8] == float("inf")).all() and torch.isnan(hit[:, 8]).all()
+    else:
+        assert (hit[:, 8] == -float("inf")).all()
+    assert (hit[:, 90] == -float("inf")).all()
+    odd = torch.zeros(out.shape, dtype=torch.bool, device="cuda")
+    odd[-1, :, 4:6, 5:9] = odd[-1, -1, 4:6, 90] = True
+    seen = window_seen(k.shape[2], q.shape[1], zc.WINDOW_ALL, 0)
+    clean = torch.where(torch.isfinite(v), v, torch.zeros_like(v))
+    for i in range(q.shape[0]):
+        want = reference(q[i], k[i], clean[i], seen)
+        check(out[i][~odd[i]], want[~odd[i]], clean[i], dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("how", list(SPLITS))
+def test_an_infinite_key_weighs_nothing_or_everything(how, dtype):
+    """A score of -infinity is a weight of 0, one of +infinity has no softmax."""
+    at = SPLITS[how][1] + 2 if how == "prompt" else 1
+
+    def edit(q, k, v):
+        k[-1, 1, at, 77] = float("inf")
+    q, k, v, out = split_case(how, dtype, edit)
+    seen = window_seen(k.shape[2], q.shape[1], zc.WINDOW_ALL, 0)
+    nan = none(q)
+    nan[-1, :, 2:4] = q[-1, :, 2:4, 77] > 0
+    assert not nan.all() and (q[..., 77] != 0).all()
+    for i in range(q.shape[0]):
+        assert torch.isnan(out[i][nan[i]]).all()
+        kk = torch.where(torch.isfinite(k[i]), k[i], torch.zeros_like(k[i]))
+        want = reference(q[i], kk, v[i], seen)
+        if i == q.shape[0] - 1:
+            without = seen.clone()
+            without[:, at] = False
+            want[:, 2:4] = reference(q[i], kk, v[i], without)[:, 2:4]
+        check(out[i][~nan[i]], want[~nan[i]], v[i], dtype)

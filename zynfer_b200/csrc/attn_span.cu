@@ -89,6 +89,19 @@ __device__ __forceinline__ void join_shared(Partial& x, const float* rec) {
     for (int e = 0; e < 4; ++e) x.acc[e] = x.acc[e] * c0 + f[e] * c1;
 }
 
+// A piece whose result is not finite once more, position by position, a warp together:
+// P's rows and terms that are 0 make a NaN of an infinite V, and the terms of an
+// infinite q one of its scores. rec: the records of both heads; null: the output.
+static __device__ __noinline__ void redo_piece(const ServeAttnArgs& a, const ServeRow& row, int head, int low, const Span& span,
+                                               int v0, int v1, float* rec, size_t rec_step) {
+#pragma unroll 1
+    for (int h = 0; h < kG; ++h) {
+        const Partial x = slow_row(a, row.row, head * kG + h, row.slot, row.len - 1, low, a.sinks, span, v0, min(v1, span.total));
+        if (rec) store_record(rec + h * rec_step, x, 1);
+        else store_row(a, row.row, head * kG + h, x);
+    }
+}
+
 template <int N>
 __global__ void __launch_bounds__(kThreads, 1)
     attn_span_kernel(const __grid_constant__ ServeRowsT<N> rows_param, const __grid_constant__ ServeAttnArgs a) {
@@ -257,7 +270,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t qf[8][2];
     float acc[16][4];
     float m_run = -INFINITY, l_run = 0.0f;  // lanes t = 0, 1: head t
-    int pos = 0, low = 0, since = 0;  // since: blocks since the last flush
+    int pos = 0, low = 0, since = 0, blk0 = 0;  // since: blocks since the last flush; blk0: the piece's first
     Span span{};
     bool seg_start = true;
 
@@ -383,6 +396,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             m_run = -INFINITY;
             l_run = 0.0f;
             since = 0;
+            blk0 = cc.blk;
             seg_start = false;
         }
         const int nb = (i + 1 < n && cc.blk + 1 < cc.nblk) ? 2 : 1;
@@ -423,6 +437,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                     acc[nt][e] = x + (mid + lo_sum);
                 }
             const bool writer = (g & 5) == 0 && g < 4;
+            bool finite = fabsf(Lh) < INFINITY;
+#pragma unroll
+            for (int nt = 0; nt < 16; ++nt) finite = finite && fabsf(acc[nt][0]) < INFINITY && fabsf(acc[nt][1]) < INFINITY;
+            const bool redo = !__all_sync(kAll, finite || !writer);
             const long long f0 = (long long)a.n_kv * pref[cc.b] + (long long)cc.head * cc.nblk;
             const bool whole = f0 >= lo && f0 + cc.nblk <= lo + n;
             const int nrec = cur.nrec();
@@ -430,7 +448,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 pdl_wait();  // (the output may still be read)
                 waited = true;
             }
-            if (whole && nrec == 0) {
+            if (redo) {
+                const int k = f0 < lo ? 0 : 1;
+                const size_t at = ((size_t)cc.b * (a.n_kv * kG) + cc.head * kG) * a.max_segs + nrec;
+                redo_piece(a, cur, cc.head, low, span, blk0, cc.blk + 1,
+                           !whole ? sm.rec[k][warp] : (nrec > 0 ? a.part + at * kRecord : nullptr),
+                           whole ? (size_t)a.max_segs * kRecord : (size_t)kRecord);
+                if (!whole && lane == 0) sm.rec_gid[k][warp] = cc.b * a.n_kv + cc.head;
+            } else if (whole && nrec == 0) {
                 if (writer) {
                     const size_t at = (size_t)cur.row * a.out_stride + (size_t)(cc.head * kG + hsel) * kD + 2 * t;
                     const float inv = Lh == 0.0f ? 0.0f : 1.0f / Lh;
