@@ -356,9 +356,9 @@ ZYNFER_CU_API int zynfer_cu_rmsnorm_qk_rope(ZynferCuCtx *ctx, const float *qkv, 
                                             const float *k_norm, uint32_t pos0, float *q_out, float *k_out);
 /* ---- serving attention and draws (device pointers) ----
  * These calls read the cache that prefill, decode and zynfer_cu_kv_write
- * fill. They return once their kernels are enqueued on the context stream
- * (zynfer_cu_sync waits, and reports a failed device check); the batch's
- * lengths and slots are taken at the call. dtype is ZYNFER_CU_DT_F32 or
+ * fill. They return once their kernels are enqueued, on the context stream or
+ * the one named to zynfer_cu_use_stream (zynfer_cu_sync waits for either, and
+ * reports a failed device check); the batch's lengths and slots are taken at the call. dtype is ZYNFER_CU_DT_F32 or
  * ZYNFER_CU_DT_BF16, for q and out alike; row i of q starts i * q_stride
  * elements in and holds [n_q][head_dim]; out is laid out the same with
  * out_stride and does not overlap q. Strides are at least n_q * head_dim and
@@ -417,11 +417,19 @@ typedef struct ZynferCuDrawRule {
  * weights are whole numbers: the same inputs give the same tokens. A row
  * without any weight gives id 0. logprobs (nullable) receives the drawn
  * token's (l - max l) / temperature - ln(S / 2^33) (-inf without weight).
- * Needs no model. Asynchronous, on the context stream; arrays 4-byte
+ * Needs no model. Asynchronous as above; arrays 4-byte
  * aligned, logits aligned to their type. */
 ZYNFER_CU_API int zynfer_cu_sample_rows(ZynferCuCtx *ctx, const void *logits, int dtype, uint64_t stride,
                                         uint32_t rows, uint32_t vocab, const float *uniforms,
                                         const ZynferCuDrawRule *rule, uint32_t *ids, float *logprobs);
+/* The stream of these four calls (kv_write, attn_shared, attn_window,
+ * sample_rows): until the next zynfer_cu_use_stream they run on `stream` (a
+ * cudaStream_t of the context's device; NULL = the default stream), so in order
+ * with a caller's work there, and still after all earlier and before all later
+ * work of the context. ZYNFER_CU_OWN_STREAM: the context stream, as after
+ * create. The stream may be destroyed after zynfer_cu_sync. */
+#define ZYNFER_CU_OWN_STREAM ((void *)(intptr_t)-1)
+ZYNFER_CU_API int zynfer_cu_use_stream(ZynferCuCtx *ctx, void *stream);
 /* Order between the context stream and a caller's cudaStream_t (NULL = the
  * default stream): wait_stream makes the context's later work wait for what
  * `stream` holds now, stream_wait the other way round. */

@@ -73,9 +73,28 @@ struct GraphEntry {
 
 }  // namespace
 
+// Where a context's work goes: its own stream, or in a serving call the one that the
+// caller named (zynfer_cu_use_stream). All of it runs in the order of the calls: work
+// that moves from one stream to the other waits for what came before by an event.
+// Calls that stay on one stream record and wait for nothing.
+struct WorkStream {
+    cudaStream_t own = nullptr, named = nullptr, last = nullptr;
+    cudaEvent_t moved = nullptr;
+    bool has_named = false, on_named = false;
+    operator cudaStream_t() {
+        const cudaStream_t now = on_named && has_named ? named : own;
+        if (now != last) {  // (a failure is the call's: cudaGetLastError)
+            cudaEventRecord(moved, last);
+            cudaStreamWaitEvent(now, moved, 0);
+            last = now;
+        }
+        return now;
+    }
+};
+
 struct ZynferCuCtx {
     int device = -1;
-    cudaStream_t stream = nullptr;
+    WorkStream stream;
     std::string err;
     char path[96] = "none";  // label of the last call's kernels; a fixed buffer, written without allocating
     unsigned step_paths = 0;  // linear families (bit kPath*) launched since the last reset
@@ -773,6 +792,13 @@ void enqueue_prefill_layers(ZynferCuCtx* c, uint32_t seq, int T, uint32_t l0, ui
 
 // ---- serving attention (serve_attn.cu)
 
+// A serving call: its work goes to the stream that the caller named.
+struct ServingCall {
+    WorkStream& s;
+    explicit ServingCall(ZynferCuCtx* c) : s(c->stream) { s.on_named = true; }
+    ~ServingCall() { s.on_named = false; }
+};
+
 // The checks of a serving-attention call's batch; c->serve_rows receives its
 // slots and lengths, `extra` positions past the cached ones included.
 int serve_batch(ZynferCuCtx* c, const uint32_t* seqs, uint32_t batch, uint32_t tokens, uint32_t extra) {
@@ -1103,12 +1129,14 @@ int zynfer_cu_create(int device, ZynferCuCtx** out) {
         *out = c;
         return ZYNFER_CU_UNSUPPORTED;
     }
-    e = cudaStreamCreateWithFlags(&c->stream, cudaStreamNonBlocking);
+    e = cudaStreamCreateWithFlags(&c->stream.own, cudaStreamNonBlocking);
     if (e != cudaSuccess) {
         c->err = cudaGetErrorString(e);
         *out = c;
         return ZYNFER_CU_LAUNCH;
     }
+    c->stream.last = c->stream.own;
+    cudaEventCreateWithFlags(&c->stream.moved, cudaEventDisableTiming);
     cudaEventCreate(&c->ev0);
     cudaEventCreate(&c->ev1);
     cudaEventCreateWithFlags(&c->ev_order, cudaEventDisableTiming);
@@ -1123,7 +1151,7 @@ void zynfer_cu_destroy(ZynferCuCtx* c) {
     // During process teardown the runtime may already be unloading: then the
     // driver reclaims everything and no CUDA call may be made.
     if (c->device >= 0 && cudaSetDevice(c->device) == cudaSuccess) {
-        if (c->stream) cudaStreamSynchronize(c->stream);
+        if (c->stream.own) cudaStreamSynchronize(c->stream);
         for (auto& kv : c->graphs) cudaGraphExecDestroy(kv.second.exec);
         for (auto& t : c->tev) {
             cudaEventDestroy(t.a);
@@ -1132,9 +1160,10 @@ void zynfer_cu_destroy(ZynferCuCtx* c) {
         if (c->ev0) cudaEventDestroy(c->ev0);
         if (c->ev1) cudaEventDestroy(c->ev1);
         if (c->ev_order) cudaEventDestroy(c->ev_order);
+        if (c->stream.moved) cudaEventDestroy(c->stream.moved);
         for (void* p : c->allocs) cudaFree(p);
         for (void* p : c->pinned) cudaFreeHost(p);
-        if (c->stream) cudaStreamDestroy(c->stream);
+        if (c->stream.own) cudaStreamDestroy(c->stream.own);
     }
     delete c;
 }
@@ -1680,6 +1709,7 @@ int zynfer_cu_kv_write(ZynferCuCtx* c, uint32_t seq, uint32_t layer, uint32_t po
             return fail(c, ZYNFER_CU_INVALID, "kv_write: a written block is shared with another sequence");
     if (take_launch_fault(c)) return ZYNFER_CU_LAUNCH;
     cudaSetDevice(c->device);
+    ServingCall on(c);
     int rc = ensure_blocks(c, seq, pos + n);
     if (rc) return rc;
     if ((rc = settle_tables(c, &seq, 1))) return rc;
@@ -1705,6 +1735,7 @@ int zynfer_cu_attn_window(ZynferCuCtx* c, uint32_t layer, const uint32_t* seqs, 
     if ((rc = serve_batch(c, seqs, batch, tokens, 0))) return rc;
     if (take_launch_fault(c)) return ZYNFER_CU_LAUNCH;
     cudaSetDevice(c->device);
+    ServingCall on(c);
     if ((rc = settle_tables(c, seqs, batch))) return rc;
     const bool bf16 = dtype == ZYNFER_CU_DT_BF16;
     ServePlan plan;
@@ -1726,6 +1757,7 @@ int zynfer_cu_attn_shared(ZynferCuCtx* c, uint32_t layer, const uint32_t* seqs, 
     if ((rc = validate_batch(c, seqs, batch, 0))) return rc;
     if (take_launch_fault(c)) return ZYNFER_CU_LAUNCH;
     cudaSetDevice(c->device);
+    ServingCall on(c);
     if ((rc = settle_tables(c, seqs, batch))) return rc;
     const bool bf16 = dtype == ZYNFER_CU_DT_BF16;
     ServePlan plan;
@@ -1756,6 +1788,7 @@ int zynfer_cu_sample_rows(ZynferCuCtx* c, const void* logits, int dtype, uint64_
     if (reinterpret_cast<uintptr_t>(logits) % esz) return fail(c, ZYNFER_CU_INVALID, "logits are misaligned");
     if (take_launch_fault(c)) return ZYNFER_CU_LAUNCH;
     cudaSetDevice(c->device);
+    ServingCall on(c);
     DrawArgs a{};
     a.logits = logits; a.bf16 = dtype == ZYNFER_CU_DT_BF16; a.stride = stride; a.rows = (int)rows; a.vocab = (int)vocab;
     a.uniforms = uniforms; a.temperature = rule->temperature; a.top_k = rule->top_k; a.top_p = rule->top_p;
@@ -1764,6 +1797,13 @@ int zynfer_cu_sample_rows(ZynferCuCtx* c, const void* logits, int dtype, uint64_
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_fail(c, e, "draw launch");
     set_path(c, "sample_rows", 0, nullptr);
+    return ZYNFER_CU_OK;
+}
+
+int zynfer_cu_use_stream(ZynferCuCtx* c, void* stream) {
+    if (!c || c->device < 0) return ZYNFER_CU_INVALID;
+    c->stream.has_named = stream != ZYNFER_CU_OWN_STREAM;
+    c->stream.named = c->stream.has_named ? static_cast<cudaStream_t>(stream) : nullptr;
     return ZYNFER_CU_OK;
 }
 

@@ -123,6 +123,7 @@ _SIGS = {
     "zynfer_cu_attn_shared": (C.c_int, [VP, U32, VP, U32, VP, U64, VP, U64, C.c_int]),
     "zynfer_cu_attn_window": (C.c_int, [VP, U32, VP, U32, U32, U32, U32, VP, U64, VP, U64, C.c_int]),
     "zynfer_cu_sample_rows": (C.c_int, [VP, VP, C.c_int, U64, U32, U32, VP, C.POINTER(DrawRule), VP, VP]),
+    "zynfer_cu_use_stream": (C.c_int, [VP, VP]),
     "zynfer_cu_wait_stream": (C.c_int, [VP, VP]),
     "zynfer_cu_stream_wait": (C.c_int, [VP, VP]),
     "zynfer_cu_prefill_chunk": (C.c_int, [VP, U32, VP, U32, U32, U32, VP, VP]),
@@ -315,6 +316,7 @@ class Gpu:
             raise _ERRORS.get(rc, CudaError)(msg)
         self._rule = DrawRule()  # the fields of the call being made
         self._rule_ref = C.byref(self._rule)
+        self._stream = None  # of the serving calls: a cudaStream_t, None before the first
         _LIVE.add(self)
 
     def check(self, rc: int):
@@ -366,8 +368,8 @@ class Gpu:
                     stream=None):
         """The next token of each row of device logits [rows, vocab] (f32 or bf16, rows at any stride) from the
         random numbers uniforms [rows] into ids [rows] (32-bit) and, where given, logprobs [rows]; temperature,
-        top_k (int32), top_p and min_p are device tensors [rows] or None (zynfer_cu_sample_rows). Asynchronous;
-        `stream` (a torch stream) orders the call after its work and its later work after the call."""
+        top_k (int32), top_p and min_p are device tensors [rows] or None (zynfer_cu_sample_rows). Asynchronous:
+        on `stream` (a torch stream or a cudaStream_t; None: torch's current stream)."""
         if logits.dim() != 2 or logits.stride(1) != 1:
             raise InvalidArgument("logits must be [rows, vocab] with unit inner stride")
         rows, vocab = logits.shape
@@ -383,19 +385,23 @@ class Gpu:
 
     def wait_stream(self, stream):
         """Later work of this context waits for what `stream` (a torch stream or a cudaStream_t) holds now."""
-        self.check(lib().zynfer_cu_wait_stream(self.h, VP(int(getattr(stream, "cuda_stream", stream or 0)))))
+        self.check(lib().zynfer_cu_wait_stream(self.h, int(getattr(stream, "cuda_stream", stream or 0))))
 
     def stream_wait(self, stream):
         """Later work of `stream` waits for what this context has enqueued so far."""
-        self.check(lib().zynfer_cu_stream_wait(self.h, VP(int(getattr(stream, "cuda_stream", stream or 0)))))
+        self.check(lib().zynfer_cu_stream_wait(self.h, int(getattr(stream, "cuda_stream", stream or 0))))
 
     def _enqueue(self, stream, fn, args):
-        """An asynchronous call; with a stream, after its work so far and before its later work."""
-        if stream is not None:
-            self.wait_stream(stream)
+        """An asynchronous call on `stream`; None is torch's current stream, on which the call's tensors are in use
+        (the context's own waits for no other)."""
+        if stream is None:
+            import torch
+            stream = torch.cuda.current_stream(self.device)
+        handle = int(getattr(stream, "cuda_stream", stream))
+        if handle != self._stream:
+            self.check(lib().zynfer_cu_use_stream(self.h, handle))
+            self._stream = handle
         self.check(fn(*args))
-        if stream is not None:
-            self.stream_wait(stream)
 
     def phase_trace(self):
         """Phase timestamps (ns) of the last persistent decode step run with timing on."""
@@ -539,7 +545,7 @@ class Model:
 
     def kv_write(self, seq: int, layer: int, pos: int, k, v, stream=None):
         """K and V rows (device, dense [n_kv, n, head_dim], f32 or bf16) into positions pos .. pos + n - 1 of a
-        sequence's cache of one layer. Asynchronous."""
+        sequence's cache of one layer. Asynchronous, on `stream` as Gpu.sample_rows."""
         a = self.arch
         _require(len(k.shape) == 3 and k.shape == v.shape and k.shape[0] == a.n_kv and k.shape[2] == a.head_dim and
                  k.dtype == v.dtype and k.is_contiguous() and v.is_contiguous(),
@@ -565,7 +571,8 @@ class Model:
 
     def attn_shared(self, layer: int, seqs, q, out, stream=None):
         """Decode attention of one query per sequence (device q and out [B, n_q, head_dim], f32 or bf16, rows at
-        any stride) over all cached positions; leading blocks that sequences share are read once. Asynchronous."""
+        any stride) over all cached positions; leading blocks that sequences share are read once. Asynchronous, on
+        `stream` as Gpu.sample_rows."""
         ids, n, keep = _ids(seqs)
         if q.dtype != out.dtype:
             raise InvalidArgument("q and out must have one type")
@@ -575,7 +582,8 @@ class Model:
 
     def attn_window(self, layer: int, seqs, q, out, window: int = WINDOW_ALL, sinks: int = 0, stream=None):
         """Attention of the last T cached positions of each sequence (device q and out [B, T, n_q, head_dim], or
-        [B, n_q, head_dim] for T = 1) over the last `window` positions up to each and the first `sinks`. Asynchronous."""
+        [B, n_q, head_dim] for T = 1) over the last `window` positions up to each and the first `sinks`.
+        Asynchronous, on `stream` as Gpu.sample_rows."""
         ids, n, keep = _ids(seqs)
         dims = q.dim()
         if q.dtype != out.dtype or dims not in (3, 4):
