@@ -1,7 +1,8 @@
 """Serving attention where it is easily wrong (B200 only), against the formula
 in 64 bits: the precision of bf16 results, infinities and NaN that cross
 splits, and plans of batches whose prompts are nested."""
-import numpy as np
+import time
+
 import pytest
 
 from test_gpu_serve_attn import DTYPES, D, check, make, normal, reference, window_seen
@@ -203,3 +204,28 @@ def test_an_infinite_key_weighs_nothing_or_everything(how, dtype):
             without[:, at] = False
             want[:, 2:4] = reference(q[i], kk, v[i], without)[:, 2:4]
         check(out[i][~nan[i]], want[~nan[i]], v[i], dtype)
+
+
+def test_a_chain_of_forks_is_planned_in_linear_time():
+    """Each of 1024 sequences forked from the one before, one block longer: every depth is a run of its own. The host's
+    part of a call is well below a millisecond where it is linear (it was 0.2 s)."""
+    rows, n_kv = 1024, 2
+    m = make(n_kv=n_kv, max_batch=rows, max_seqs=rows, max_seq_len=16 * rows, kv_blocks=rows + 2)
+    k, v = normal(221, n_kv, 16 * rows, D, dtype=torch.bfloat16), normal(222, n_kv, 16 * rows, D, dtype=torch.bfloat16)
+    for i in range(rows):
+        if i:
+            m.seq_fork(i, i - 1, 16 * i)
+        m.kv_write(i, 0, 16 * i, k[:, 16 * i:16 * i + 16].contiguous(), v[:, 16 * i:16 * i + 16].contiguous())
+    q = normal(223, rows, 2 * n_kv, D, scale=1.5)
+    out = torch.empty_like(q)
+    took = []
+    for _ in range(4):
+        torch.cuda.synchronize()
+        began = time.perf_counter()
+        m.attn_shared(0, range(rows), q, out)
+        took.append(time.perf_counter() - began)
+        m.gpu.sync()
+    assert min(took) < 0.02
+    for i in (0, 1, 2, 63, 64, 511, 1000, 1023):
+        n = 16 * (i + 1)
+        check(out[i:i + 1], reference(q[i:i + 1], k[:, :n], v[:, :n], all_seen(n)), v, "f32")
