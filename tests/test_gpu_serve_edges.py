@@ -229,3 +229,55 @@ def test_a_chain_of_forks_is_planned_in_linear_time():
     for i in (0, 1, 2, 63, 64, 511, 1000, 1023):
         n = 16 * (i + 1)
         check(out[i:i + 1], reference(q[i:i + 1], k[:, :n], v[:, :n], all_seen(n)), v, "f32")
+
+
+def nested(layers=1):
+    """64 sequences: a start of 16 positions, two questions of 960 behind it, 32 samples of each with 0 to 2 positions of
+    their own; slots 0 .. 31 the first question's, 32 .. 63 the second's. The model, K and V of every sequence."""
+    arch = zc.Arch(vocab=512, hidden=512, inter=512, layers=layers, n_q=8, n_kv=4, max_pos=1040)
+    m = zc.Model(zc.Gpu(0), arch, zc.W_BF16, max_batch=64, max_seqs=65, max_seq_len=1040, kv_blocks=400, max_prefill=16)
+    m.fill_synthetic(1, 0.05, 0.1)
+    start = [normal(s, 4, 16, D, dtype=torch.bfloat16) for s in (231, 232)]
+    kv = {}
+
+    def write(seq, pos, k, v):
+        for layer in range(layers):
+            m.kv_write(seq, layer, pos, k, v)
+    write(64, 0, *start)
+    for first, seed in ((0, 233), (32, 235)):
+        m.seq_fork(first, 64, 16)
+        question = [normal(s, 4, 960, D, dtype=torch.bfloat16) for s in (seed, seed + 1)]
+        write(first, 16, *question)
+        for s in range(first + 1, first + 32):
+            m.seq_fork(s, first, 976)
+        for s in range(first, first + 32):
+            own = [normal(300 + 2 * s + e, 4, s % 3, D, dtype=torch.bfloat16) for e in (0, 1)]
+            write(s, 976, *own)
+            kv[s] = [torch.cat(x, 1) for x in zip(start, question, own)]
+    return m, kv
+
+
+ORDERS = {"in order": list(range(64)), "in turn": [32 * (i % 2) + i // 2 for i in range(64)], "mixed": [(37 * i + 11) % 64 for i in range(64)]}
+
+
+@pytest.mark.parametrize("order", list(ORDERS))
+def test_nested_prompts_in_any_order(order):
+    m, kv = nested()
+    q = normal(240, 64, 8, D, scale=1.5)
+    out = torch.full_like(q, float("nan"))
+    m.attn_shared(0, ORDERS[order], q, out)
+    m.gpu.sync()
+    for i, s in enumerate(ORDERS[order]):
+        k, v = kv[s]
+        check(out[i:i + 1], reference(q[i:i + 1], k, v, all_seen(k.shape[1])), v, "f32")
+
+
+def test_nested_prompts_are_shared_in_any_order():
+    """Both questions are read once, whatever the order of the batch: the step has the launches of shared prompts (tiles,
+    own blocks, join) in each layer. In turn, neighbours have no more than the start in common."""
+    launches = {}
+    for order, seqs in ORDERS.items():
+        m, _ = nested(layers=2)
+        m.decode_drawn(seqs, [5] * 64, [0.5] * 64, temperature=0.0)
+        launches[order] = m.gpu.step_launches
+    assert len(set(launches.values())) == 1, launches

@@ -871,9 +871,30 @@ int shared_runs(const int* common, int n, SharedRun* out, long long* saved) {
 // 64 x 512 (16128) 26 / 29, 8 x 16384 (57344) 45 / 68.
 constexpr long long kShareBlocks = 8192;
 
+// Are rows with a common block neighbours, whatever the block? A block names its whole
+// prefix, so it is enough that no block is met again after a row without it: the two
+// that tell neighbours apart are one that ends and one that begins.
+bool rows_grouped(ZynferCuCtx* c, const int* common, int n) {
+    int ended[kServeMaxBatch], n_ended = 0;
+    bool grouped = true;
+    for (int i = 0; i + 1 < n && grouped; ++i) {
+        const std::vector<int>& a = c->seq_blocks[c->serve_rows.r[i].slot];
+        const std::vector<int>& b = c->seq_blocks[c->serve_rows.r[i + 1].slot];
+        const size_t d = (size_t)common[i];
+        if (d < a.size()) {
+            c->serve_mark[a[d]] = 1;
+            ended[n_ended++] = a[d];
+        }
+        grouped = !(d < b.size() && c->serve_mark[b[d]] >= 0);
+    }
+    for (int i = 0; i < n_ended; ++i) c->serve_mark[ended[i]] = -1;
+    return grouped;
+}
+
 // Common leading blocks of the rows of c->serve_rows (one query each): the
-// rows reordered so that rows with the same first block are neighbours, in the
-// caller's order otherwise; the runs that share blocks as tiles of 64 rows,
+// rows reordered so that rows with the same blocks are neighbours (by the first block,
+// in the caller's order otherwise; by all of them where that does not do it); the runs
+// that share blocks as tiles of 64 rows,
 // each tile's blocks split over CTAs so that all tiles fill the GPU once.
 // Returns the work items (0: nothing is shared).
 int plan_shared(ZynferCuCtx* c, uint32_t batch, bool bf16, int* max_segs) {
@@ -898,10 +919,27 @@ int plan_shared(ZynferCuCtx* c, uint32_t batch, bool bf16, int* max_segs) {
     for (uint32_t i = 0; i < batch; ++i) order[at[group[i]]++] = (int)i;
     ServeRow given[kServeMaxBatch];
     std::copy(rows.r, rows.r + batch, given);
-    for (uint32_t i = 0; i < batch; ++i) rows.r[i] = given[order[i]];
+    size_t held = 0;  // no more than these can be saved
+    for (uint32_t i = 0; i < batch; ++i) {
+        rows.r[i] = given[order[i]];
+        held += c->seq_blocks[rows.r[i].slot].size();
+    }
+    if ((long long)held * c->d.n_kv < kShareBlocks) {
+        std::copy(given, given + batch, rows.r);
+        return 0;
+    }
+    auto blocks = [&](const ServeRow& r) -> const std::vector<int>& { return c->seq_blocks[r.slot]; };
     for (uint32_t i = 0; i + 1 < batch; ++i)
-        common[i] = group[order[i]] == group[order[i + 1]]
-                        ? common_blocks(c->seq_blocks[rows.r[i].slot], c->seq_blocks[rows.r[i + 1].slot]) : 0;
+        common[i] = group[order[i]] == group[order[i + 1]] ? common_blocks(blocks(rows.r[i]), blocks(rows.r[i + 1])) : 0;
+    if (!rows_grouped(c, common, (int)batch)) {
+        std::sort(rows.r, rows.r + batch, [&](const ServeRow& x, const ServeRow& y) {
+            const std::vector<int>&a = blocks(x), &b = blocks(y);
+            const size_t d = (size_t)common_blocks(a, b);
+            if (d < a.size() && d < b.size()) return a[d] < b[d];
+            return a.size() != b.size() ? a.size() < b.size() : x.row < y.row;
+        });
+        for (uint32_t i = 0; i + 1 < batch; ++i) common[i] = common_blocks(blocks(rows.r[i]), blocks(rows.r[i + 1]));
+    }
     const int tile_blocks = kAttnTileBlocks;
     long long work = 0, saved = 0;
     SharedRun runs[kServeMaxBatch / 2];
