@@ -1,5 +1,8 @@
 """Argument checks of the serving calls that need no GPU: what the binding
 refuses before a pointer reaches the library."""
+import ctypes
+
+import numpy as np
 import pytest
 
 from zynfer_b200 import cuda as zc
@@ -125,3 +128,32 @@ def test_windows_of_the_model_path_do_not_wrap(model, monkeypatch, call, at):
                                 (2 ** 32, 2 ** 40, (zc.WINDOW_ALL, zc.WINDOW_ALL)), (2 ** 32 + 10, 1, (zc.WINDOW_ALL, 1))):
         call(model, window, sinks)
         assert lib.calls[-1][1][at:at + 2] == want
+
+
+def test_indexes_do_not_wrap(model, monkeypatch):
+    """2^32 is no slot, layer, position or token, nor is -1: as a Python number or in an array of wider numbers."""
+    lib = Library()
+    monkeypatch.setattr(zc, "lib", lambda: lib)
+    kv, q = torch.zeros(2, 5, D), torch.zeros(1, 4, D)
+    for x in (2 ** 32, -1, 2 ** 32 + 3, -2 ** 32):
+        wide = np.array([x])
+        for call in (lambda: model.kv_write(x, 0, 0, kv, kv), lambda: model.kv_write(0, x, 0, kv, kv), lambda: model.kv_write(0, 0, x, kv, kv),
+                     lambda: model.attn_shared(x, [0], q, q), lambda: model.attn_shared(0, [x], q, q), lambda: model.attn_shared(0, wide, q, q),
+                     lambda: model.attn_window(x, [0], q, q), lambda: model.attn_window(0, wide, q, q),
+                     lambda: model.prefill_chunk(x, [1]), lambda: model.prefill_chunk(0, wide), lambda: model.prefill_chunk(0, [x]),
+                     lambda: model.decode_drawn(wide, [1], [0.5]), lambda: model.decode_drawn([0], wide, [0.5]),
+                     lambda: model.decode_drawn([0.5], [1], [0.5])):
+            with pytest.raises(zc.InvalidArgument, match="index|whole numbers|sequence id"):
+                call()
+    assert not lib.calls
+
+
+def test_top_k_beyond_32_bits_keeps_every_token(model, monkeypatch):
+    lib = Library()
+    seen = []
+    lib.zynfer_cu_decode_drawn = lambda *a: seen.append(list((ctypes.c_int32 * 4).from_address(a[7]._obj.top_k))) or 0
+    monkeypatch.setattr(zc, "lib", lambda: lib)
+    model.decode_drawn([0, 1, 2, 3], [1, 2, 3, 4], [0.5] * 4, top_k=np.array([2 ** 32 + 5, -2 ** 40, 7, 2 ** 31]))
+    assert seen == [[2 ** 31 - 1, 0, 7, 2 ** 31 - 1]]
+    model.decode_drawn([0, 1, 2, 3], [1, 2, 3, 4], [0.5] * 4, top_k=3)
+    assert seen[-1] == [3] * 4

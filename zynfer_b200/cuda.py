@@ -219,6 +219,21 @@ def _row_values(t, shape, kinds, device: int, name: str):
 _F32, _I32 = ("float32",), ("int32", "uint32")
 
 
+def _u32(*indexes):
+    """Slots, layers and positions fit the library's 32 bits (ctypes would wrap them)."""
+    for x in indexes:
+        if not 0 <= x <= 0xFFFFFFFF:
+            raise InvalidArgument(f"index out of range: {x}")
+
+
+def _u32_array(values, name: str) -> np.ndarray:
+    """Whole numbers as a dense 32-bit array (a cast would wrap them)."""
+    a = np.asarray(values)
+    if a.size and a.dtype != np.uint32 and (a.dtype.kind not in "iu" or a.min() < 0 or a.max() > 0xFFFFFFFF):
+        raise InvalidArgument(f"{name} must be whole numbers of 32 bits")
+    return np.ascontiguousarray(a, np.uint32)
+
+
 def _ids(seqs):
     """Sequence ids as a C array: its address, its length, and the array to keep alive."""
     if not isinstance(seqs, np.ndarray):
@@ -227,7 +242,7 @@ def _ids(seqs):
         except OverflowError:
             raise InvalidArgument("sequence id out of range") from None
         return a.buffer_info()[0], len(a), a
-    a = np.ascontiguousarray(seqs, np.uint32)
+    a = _u32_array(seqs, "sequence ids")
     return a.ctypes.data, a.size, a
 
 
@@ -547,6 +562,7 @@ class Model:
         """K and V rows (device, dense [n_kv, n, head_dim], f32 or bf16) into positions pos .. pos + n - 1 of a
         sequence's cache of one layer. Asynchronous, on `stream` as Gpu.sample_rows."""
         a = self.arch
+        _u32(seq, layer, pos)
         _require(len(k.shape) == 3 and k.shape == v.shape and k.shape[0] == a.n_kv and k.shape[2] == a.head_dim and
                  k.dtype == v.dtype and k.is_contiguous() and v.is_contiguous(),
                  "k and v must be dense [n_kv, n, head_dim] tensors of one type")
@@ -573,6 +589,7 @@ class Model:
         """Decode attention of one query per sequence (device q and out [B, n_q, head_dim], f32 or bf16, rows at
         any stride) over all cached positions; leading blocks that sequences share are read once. Asynchronous, on
         `stream` as Gpu.sample_rows."""
+        _u32(layer)
         ids, n, keep = _ids(seqs)
         if q.dtype != out.dtype:
             raise InvalidArgument("q and out must have one type")
@@ -584,6 +601,7 @@ class Model:
         """Attention of the last T cached positions of each sequence (device q and out [B, T, n_q, head_dim], or
         [B, n_q, head_dim] for T = 1) over the last `window` positions up to each and the first `sinks`.
         Asynchronous, on `stream` as Gpu.sample_rows."""
+        _u32(layer)
         ids, n, keep = _ids(seqs)
         dims = q.dim()
         if q.dtype != out.dtype or dims not in (3, 4):
@@ -636,7 +654,8 @@ class Model:
     def prefill_chunk(self, seq: int, tokens, window: int = WINDOW_ALL, sinks: int = 0, want_logits: bool = True):
         """Append a chunk of a prompt to a sequence, with windowed attention; the last token's logits and argmax."""
         window, sinks = _mask(window, sinks)
-        t = np.ascontiguousarray(tokens, np.uint32)
+        _u32(seq)
+        t = _u32_array(tokens, "tokens")
         logits = np.empty(self.arch.vocab, np.float32) if want_logits else None
         am = np.zeros(1, np.uint32)
         self.gpu.check(lib().zynfer_cu_prefill_chunk(self.gpu.h, seq, _ptr(t), t.size, window, sinks, _ptr(logits), _ptr(am)))
@@ -646,8 +665,8 @@ class Model:
                      window: int = WINDOW_ALL, sinks: int = 0):
         """One decode step whose attention shares common leading blocks (or is windowed) and whose tokens are drawn
         from `uniforms` by a rule per row (scalars or host arrays): ids and log-probabilities."""
-        s = np.ascontiguousarray(seqs, np.uint32)
-        t = np.ascontiguousarray(tokens, np.uint32)
+        s = _u32_array(seqs, "sequence ids")
+        t = _u32_array(tokens, "tokens")
         u = np.ascontiguousarray(uniforms, np.float32)
         _require(t.size == s.size and u.size == s.size, "one token and one random number per sequence")
         window, sinks = _mask(window, sinks)
@@ -655,6 +674,8 @@ class Model:
         def per_row(x, kind):
             return None if x is None else np.ascontiguousarray(np.broadcast_to(np.asarray(x, kind), (s.size,)))
 
+        if top_k is not None:
+            top_k = np.clip(top_k, 0, 0x7FFFFFFF)
         arrays = [per_row(temperature, np.float32), per_row(top_k, np.int32), per_row(top_p, np.float32),
                   per_row(min_p, np.float32)]
         rule = DrawRule(*(None if x is None else x.ctypes.data for x in arrays))
