@@ -364,8 +364,10 @@ ZYNFER_CU_API int zynfer_cu_rmsnorm_qk_rope(ZynferCuCtx *ctx, const float *qkv, 
  * out_stride and does not overlap q. Strides are at least n_q * head_dim and
  * multiples of 8, pointers 16-byte aligned. q is rotated and normalised
  * already (zynfer_cu_rmsnorm_qk_rope); scores are q . k / sqrt(head_dim).
- * Softmax statistics and sums are f32 (attentionInto, ops.zig:285-354). The
- * first calls, and calls larger than any before, allocate workspace. */
+ * Softmax statistics and sums are f32 (attentionInto, ops.zig:285-354); the
+ * probabilities meet V with 16 bits or more where q is bf16, with 24 where it
+ * is f32. model_init allocates workspace (20 MB and 4.2 KB per row of max_batch
+ * and query head); calls that need more allocate it once. */
 
 /* Every position is visible: the window argument for full causal attention. */
 #define ZYNFER_CU_WINDOW_ALL 0xFFFFFFFFu

@@ -13,15 +13,17 @@
 // With bf16 queries two CTAs share an SM, so that the start and the end of one run
 // beside the middle of the other.
 //
-// Measured: 8192 bf16 queries, 8 kv heads, window 1024: 91 us, 0.72 PFLOP/s, 44 % of
-// the card's dense rate; 64 f32 rows over 4096 common positions: 18 us of a lone
-// call's 57 (4 tiles of keys a CTA). Bound by the two chains of a tile, about 2000 cycles with two
-// CTAs on an SM: the MMA thread's (three barriers, twelve MMAs queued behind the
-// other CTA's, 656 cycles of tensor pipe each CTA) and the softmax's (S out of TMEM
-// and the maximum 550, the exponentials 700, of which the special-function units
-// need 512). So a barrier is tried before it is waited for, what ends together
-// shares a commit, and the MMA loop's descriptors are constants (101 us before
-// these three and the asynchronous copies of Q).
+// Measured: 8192 bf16 queries, 8 kv heads, window 1024: 115 us a call, 0.57 PFLOP/s,
+// 35 % of the card's dense rate (0.72 and 44 % with P as one term, which cost the
+// results half their precision); 64 f32 rows over 4096 common positions: 18 us of a
+// lone call's 60 (4 tiles of keys a CTA). Bound by the two chains of a tile, with two
+// CTAs on an SM: the MMA thread's (three barriers, sixteen MMAs queued behind the
+// other CTA's, 912 cycles of tensor pipe each CTA: the pipe is active 55 % of the
+// time) and the softmax's (S out of TMEM and the maximum 550, the exponentials 700,
+// of which the special-function units need 512). So a barrier is tried before it is
+// waited for, what ends together shares a commit, and the MMA loop's descriptors are
+// constants (with one term of P: 101 us before these three and the asynchronous
+// copies of Q, 89 after).
 //
 // The cache's layout is the MMA's: a block row is 256 bytes whose 16-byte
 // chunks are XOR-swizzled by token & 7 inside each 128-byte half, so 16-row

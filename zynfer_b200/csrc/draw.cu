@@ -17,8 +17,9 @@
 // weight of 2^-34 of the largest apart from 0 and the sum of 2^18 of them
 // below 2^53, so products with top_p and u are single f64 roundings.
 //
-// One pass over HBM: a cluster of C CTAs takes a row, each CTA its C-th part,
-// and selects by sums.
+// A cluster of C CTAs takes a row, each CTA its C-th part, and selects by sums. It
+// goes over the row for its range, for the bins and once for each question, the
+// first time from HBM and then from shared memory or, mostly, L2.
 //   1. the largest and smallest logit of the row (one exchange over distributed
 //      shared memory);
 //   2. every CTA adds its tokens' weights (and counts) into NB bins even in
@@ -30,11 +31,12 @@
 //      their weights scanned. A bin of more tokens than that list holds (many
 //      equal logits) is divided again, by (logit, index) itself, until it fits.
 // A few rows are bound by the chain of loads, exchanges and barriers (20 us for
-// one row of 151936), many rows by the instructions per logit (about 40, an
+// one row of 151936), many rows by the instructions per logit (about 55, an
 // accurate exponential among them), not by the bytes. So a row has the more CTAs
 // the fewer rows there are: 16 for up to 4, 8 for up to 37, then 4, 2 and 1 (256
-// rows of bf16: 123 us a call with one CTA a row against 206 with eight, whose
-// barriers left the SMs idle; 88 with half the instructions since); weights are
+// rows of bf16, calls overlapping: 123 us a call with one CTA a row against 206 with
+// eight, whose barriers left the SMs idle; 88 with half the instructions since, and
+// 116 one after another on a stream); weights are
 // split into two 32-bit words without integer conversions; and two CTAs share an
 // SM. Eight CTAs or more hold their parts of a row in shared memory, fewer read
 // them again from L2.

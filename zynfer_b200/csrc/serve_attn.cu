@@ -21,7 +21,7 @@ using namespace serve;
 // own, whose first says how many they are. A launch of its own because a row's
 // join is a chain of round trips: inside the kernel that streams the rows' own
 // blocks it held up the warps that have many short rows (64 rows sharing 4096
-// positions: 64 us of it there, 30 now).
+// positions: 64 us a call with it there, 30 so, calls overlapping).
 template <int N>
 __global__ void __launch_bounds__(128) serve_merge_kernel(const __grid_constant__ ServeRowsT<N> rows_param,
                                                           const __grid_constant__ ServeAttnArgs a) {
