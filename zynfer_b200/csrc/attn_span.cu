@@ -21,8 +21,8 @@
 // row joins in a fixed order (an atomic counter tells which is last; nothing
 // waits). A row with a common prompt leaves its records to serve_attn.cu's join.
 //
-// Measured: 64 rows that see 1028 positions each, 8 kv heads: 53.8 us a call, one after
-// another on a stream, 5.0 TB/s, 77 % of the card's copy rate; 46.4 us and 89 % where
+// Measured: 64 rows that see 1028 positions each, 8 kv heads: 53.1 us a call, one after
+// another on a stream, 5.1 TB/s, 78 % of the card's copy rate; 46.4 us and 89 % where
 // calls on other streams fill the start and the end. One such row: 28 us for a lone
 // call, of which the kernel's chain (parameters, block table, K and V, joins in and
 // across CTAs) is 11.4.
@@ -94,13 +94,15 @@ __device__ __forceinline__ void join_shared(Partial& x, const float* rec) {
 // A piece whose result is not finite once more, position by position, a warp together:
 // P's rows and terms that are 0 make a NaN of an infinite V, and the terms of an
 // infinite q one of its scores. rec: the records of both heads; null: the output.
-static __device__ __noinline__ void redo_piece(const ServeAttnArgs& a, const ServeRow& row, int head, int low, const Span& span,
-                                               int v0, int v1, float* rec, size_t rec_step) {
+// (All by value: what a call passes by address would be kept in local memory.)
+static __device__ __noinline__ void redo_piece(const ServeAttnArgs& a, int row, int slot, int pos, int head, int v0, int v1,
+                                               int skip, float* rec, size_t rec_step) {
+    const Span span = span_of(pos, pos, a.window, a.sinks, skip);
 #pragma unroll 1
     for (int h = 0; h < kG; ++h) {
-        const Partial x = slow_row(a, row.row, head * kG + h, row.slot, row.len - 1, low, a.sinks, span, v0, min(v1, span.total));
+        const Partial x = slow_row(a, row, head * kG + h, slot, pos, window_low(pos, a.window), a.sinks, span, v0, min(v1, span.total));
         if (rec) store_record(rec + h * rec_step, x, 1);
-        else store_row(a, row.row, head * kG + h, x);
+        else store_row(a, row, head * kG + h, x);
     }
 }
 
@@ -453,7 +455,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (redo) {
                 const int k = f0 < lo ? 0 : 1;
                 const size_t at = ((size_t)cc.b * (a.n_kv * kG) + cc.head * kG) * a.max_segs + nrec;
-                redo_piece(a, cur, cc.head, low, span, blk0, cc.blk + 1,
+                redo_piece(a, cur.row, cur.slot, pos, cc.head, blk0, cc.blk + 1, cur.skip(),
                            !whole ? sm.rec[k][warp] : (nrec > 0 ? a.part + at * kRecord : nullptr),
                            whole ? (size_t)a.max_segs * kRecord : (size_t)kRecord);
                 if (!whole && lane == 0) sm.rec_gid[k][warp] = cc.b * a.n_kv + cc.head;
